@@ -404,6 +404,122 @@ void decode_attention_grid(const Tensor& q, const Tensor& k, const Tensor& v, co
                                    part_ml.data_ptr<float>(), B, T, rot, cap, rot ? cos_t.size(0) : 1, splits, scale, eps, stream()), "decode_attention_grid");
 }
 
+// ---- paged key/value cache (csrc/paged.cuh). The values of the tables are checked by the kernels; here their types and shapes.
+// 16-byte loads of whole heads: a tensor whose strides or address do not allow them is copied.
+Tensor whole_heads(const Tensor& t) {
+  const int64_t per = 16 / t.element_size();
+  const bool ok = t.stride(2) == 1 && t.stride(1) % per == 0 && t.stride(0) % per == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : t.contiguous().clone(at::MemoryFormat::Contiguous);
+}
+ghb::PagedPool pool_of(const Tensor& k, const Tensor& v, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const char* what) {
+  const bool fp4 = k.scalar_type() == torch::kUInt8;
+  TORCH_CHECK(k.is_cuda() && (fp4 || is_bf16(k)) && k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && k.is_contiguous() && v.is_contiguous(), what,
+              ": the cache on a GPU is bfloat16, or uint8 codes with scales");
+  const int hd = static_cast<int>(k.size(3)) * (fp4 ? 2 : 1);
+  TORCH_CHECK(hd == 64 || hd == 128 || hd == 256, what, ": head dimension ", hd, " (64, 128 or 256 on a GPU)");
+  TORCH_CHECK(fp4 == ks.has_value() && fp4 == vs.has_value(), what, ": 4-bit codes come with scales");
+  if (fp4) for (const Tensor* s : {&*ks, &*vs})
+    TORCH_CHECK(s->is_contiguous() && s->element_size() == 1 && s->numel() == k.numel() / 8 && s->device() == k.device() && reinterpret_cast<uintptr_t>(s->data_ptr()) % 16 == 0, what,
+                ": scales of the codes, starting on a 16-byte boundary");
+  TORCH_CHECK(v.device() == k.device(), what, ": one device");
+  for (const Tensor* t : {&k, &v}) TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, what, ": the cache starts on a 16-byte boundary");
+  return {k.data_ptr(), v.data_ptr(), fp4 ? static_cast<uint8_t*>(ks->data_ptr()) : nullptr, fp4 ? static_cast<uint8_t*>(vs->data_ptr()) : nullptr, hd, fp4};
+}
+ghb::PagedRows rows_of(const Tensor& k, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start, int64_t n, Tensor& err, const char* what) {
+  TORCH_CHECK(pages.dim() == 2 && q_start.dim() == 1 && lens.dim() == 1 && q_start.numel() == lens.numel() + 1 && pages.size(0) == lens.numel(), what,
+              ": pages [B, width], q_start [B + 1], lens [B] of one batch");
+  for (const Tensor* t : {&pages, &q_start, &lens}) TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->device() == k.device(), what, ": pages, q_start and lens are int32 on the cache's device");
+  TORCH_CHECK((pages.size(1) <= 1 || pages.stride(1) == 1) && q_start.is_contiguous() && lens.is_contiguous(), what, ": tables with unit inner stride");
+  if (start.has_value()) TORCH_CHECK(start->scalar_type() == torch::kInt32 && start->device() == k.device() && start->sizes() == lens.sizes() && start->is_contiguous(), what, ": start int32 [B]");
+  TORCH_CHECK(n <= 0x7fffffff && k.size(0) <= 0x7fffffff && lens.numel() < 0x7fffffff, what, ": sizes");
+  const int64_t page = k.size(2);
+  TORCH_CHECK(page >= 8 && (page & (page - 1)) == 0, what, ": the page size is a power of two from 8 on");
+  TORCH_CHECK(pages.size(1) <= 0x7fffffff / page, what, ": a row's table holds more positions than 32 bits count");
+  return {pages.data_ptr<int>(), static_cast<long>(pages.stride(0)), static_cast<int>(pages.size(1)), q_start.data_ptr<int>(), lens.data_ptr<int>(),
+          start.has_value() ? start->data_ptr<int>() : nullptr, static_cast<int>(lens.numel()), static_cast<int>(n), static_cast<int>(k.size(1)),
+          static_cast<int>(k.size(0)), __builtin_ctzll(page), err.data_ptr<int>()};
+}
+struct Rope { const float* cos; const float* sin; int half, n_pos; };
+Rope rope_of(const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, int hd, const Tensor& like, const char* what) {
+  if (!cos.has_value()) return {nullptr, nullptr, 0, 0};
+  TORCH_CHECK(sin.has_value() && cos->dim() == 2 && cos->sizes() == sin->sizes() && is_f32(*cos) && is_f32(*sin) && cos->is_contiguous() && sin->is_contiguous() &&
+              cos->device() == like.device() && sin->device() == like.device(), what, ": rope is (cos, sin), each contiguous float32 [positions, rotary pairs] on the cache's device");
+  const int64_t half = cos->size(1);
+  TORCH_CHECK(half > 0 && half % 8 == 0 && 2 * half <= hd, what, ": ", 2 * half, " rotary channels (a multiple of 16, at most the head dimension, on a GPU)");
+  for (const Tensor* t : {&*cos, &*sin}) TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, what, ": rope tables start on a 16-byte boundary");
+  return {cos->data_ptr<float>(), sin->data_ptr<float>(), static_cast<int>(half), static_cast<int>(std::min<int64_t>(cos->size(0), 0x7fffffff))};
+}
+void paged_append(Tensor& kc, Tensor& vc, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const Tensor& k_, const Tensor& v_, const Tensor& pages,
+                  const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start, const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, Tensor& err) {
+  const c10::cuda::CUDAGuard guard(kc.device());
+  const ghb::PagedPool pool = pool_of(kc, vc, ks, vs, "paged_append");
+  TORCH_CHECK(k_.dim() == 3 && v_.sizes() == k_.sizes() && k_.size(1) == kc.size(1) && k_.size(2) == pool.hd && k_.device() == kc.device() && v_.device() == kc.device(),
+              "paged_append: k, v [n, ", kc.size(1), ", ", pool.hd, "] on the cache's device, got ", k_.sizes(), " and ", v_.sizes());
+  TORCH_CHECK((is_bf16(k_) || is_f32(k_)) && k_.scalar_type() == v_.scalar_type(), "paged_append: k, v bfloat16 or float32");
+  const ghb::PagedRows r = rows_of(kc, pages, q_start, lens, start, k_.size(0), err, "paged_append");
+  const Rope rope = rope_of(cos, sin, pool.hd, kc, "paged_append");
+  const Tensor k = whole_heads(k_), v = whole_heads(v_);
+  check(ghb::paged_append(r, pool, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), is_f32(k), rope.cos, rope.sin, rope.half, rope.n_pos, stream()),
+        "paged_append");
+}
+void paged_read(const Tensor& kc, const Tensor& vc, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const Tensor& pages, const Tensor& q_start, const Tensor& lens,
+                Tensor& ko, Tensor& vo, bool fill, Tensor& err) {
+  const c10::cuda::CUDAGuard guard(kc.device());
+  const ghb::PagedPool pool = pool_of(kc, vc, ks, vs, "paged_read");
+  for (const Tensor* o : {&ko, &vo})
+    TORCH_CHECK(o->dim() == 3 && is_bf16(*o) && o->is_contiguous() && o->size(1) == kc.size(1) && o->size(2) == pool.hd && o->size(0) == ko.size(0) && o->device() == kc.device() &&
+                reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0, "paged_read: out is two contiguous bfloat16 tensors [n, ", kc.size(1), ", ", pool.hd, "]");
+  const ghb::PagedRows r = rows_of(kc, pages, q_start, lens, c10::nullopt, ko.size(0), err, "paged_read");
+  check(ghb::paged_read(r, pool, ko.data_ptr(), vo.data_ptr(), fill, stream()), "paged_read");
+}
+void paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const Tensor& pages, const Tensor& q_start,
+                     const Tensor& lens, const c10::optional<Tensor>& start, const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, int64_t cap, double scale, Tensor& out,
+                     bool fill, Tensor& err) {
+  const c10::cuda::CUDAGuard guard(kc.device());
+  const ghb::PagedPool pool = pool_of(kc, vc, ks, vs, "paged_attention");
+  TORCH_CHECK(q.dim() == 3 && (is_bf16(q) || is_f32(q)) && q.device() == kc.device() && q.size(2) == pool.hd && q.size(1) > 0 && q.size(1) % kc.size(1) == 0 && q.size(2) == pool.hd,
+              "paged_attention: q bfloat16 or float32 [n, a multiple of ", kc.size(1), ", ", pool.hd, "] on the cache's device, got ", q.sizes());
+  TORCH_CHECK(q.stride(2) == 1, "paged_attention: q with unit inner stride");
+  TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.sizes() == q.sizes() && out.device() == kc.device() && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+              "paged_attention: out is a contiguous bfloat16 tensor of q's shape");
+  const ghb::PagedRows r = rows_of(kc, pages, q_start, lens, start, q.size(0), err, "paged_attention");
+  TORCH_CHECK(kc.size(0) * kc.size(1) * kc.size(2) <= 0x7fffffff, "paged_attention: the cache has more than 2^31 entries of a head");
+  const Rope rope = rope_of(cos, sin, pool.hd, kc, "paged_attention");
+  TORCH_CHECK(cap == 0 || (rope.half > 0 && cap > 0 && cap < rope.n_pos), "paged_attention: a rotary distance cap is >= 1 and inside the rope table");
+  TORCH_CHECK(cap == 0 || rope.half == 8 || rope.half == 16 || rope.half == 32, "paged_attention: under a cap 16, 32 or 64 rotary channels on a GPU, got ", 2 * rope.half);
+  if (q.size(0) == 0) return;
+  const ghb::PagedAttn a{q.data_ptr(), static_cast<long>(q.stride(0)), static_cast<long>(q.stride(1)), is_f32(q), out.data_ptr(), rope.cos, rope.sin, rope.half, rope.n_pos,
+                         static_cast<int>(cap), static_cast<int>(q.size(1)), static_cast<float>(scale), fill};
+  ghb::PagedAttnPlan plan;
+  check(ghb::paged_attention_plan(r, pool, a.Hq, sm_count(), &plan), "paged_attention");
+  // this call's own work space (a captured call's comes from its graph's pool)
+  const Tensor ws = torch::empty({plan.ws_floats + plan.ws_ints}, q.options().dtype(torch::kFloat32));
+  check(ghb::paged_attention(r, pool, a, plan, ws.data_ptr<float>(), reinterpret_cast<int*>(ws.data_ptr<float>() + plan.ws_floats), stream()), "paged_attention");
+}
+void verify_drafts(const Tensor& target, const c10::optional<Tensor>& draft, const Tensor& drafts, const Tensor& u_accept, const Tensor& u_sample, const c10::optional<Tensor>& n_drafts,
+                   Tensor& tokens, Tensor& kept, Tensor& err) {
+  const c10::cuda::CUDAGuard guard(target.device());
+  TORCH_CHECK(target.is_cuda() && target.dim() == 3 && (is_bf16(target) || is_f32(target)) && target.size(1) >= 1 && target.size(2) >= 1 && target.stride(2) == 1,
+              "verify_drafts: target bfloat16 or float32 [B, N + 1, V] with unit inner stride");
+  const int64_t B = target.size(0), N = target.size(1) - 1, V = target.size(2);
+  TORCH_CHECK(B <= (1 << 27) && N < (1 << 24) && V <= 0x7fffffff - 4096, "verify_drafts: sizes");
+  if (draft.has_value())
+    TORCH_CHECK(draft->sizes() == at::IntArrayRef({B, N, V}) && draft->scalar_type() == target.scalar_type() && (draft->stride(2) == 1 || draft->numel() == 0) && draft->device() == target.device(),
+                "verify_drafts: draft [B, N, V] of target's type with unit inner stride");
+  TORCH_CHECK(drafts.scalar_type() == torch::kInt64 && drafts.sizes() == at::IntArrayRef({B, N}) && drafts.is_contiguous() && is_f32(u_accept) && u_accept.sizes() == drafts.sizes() &&
+              u_accept.is_contiguous() && is_f32(u_sample) && u_sample.sizes() == at::IntArrayRef({B}) && u_sample.is_contiguous(),
+              "verify_drafts: drafts int64 [B, N], u_accept float32 [B, N], u_sample float32 [B]");
+  for (const Tensor* t : {&drafts, &u_accept, &u_sample}) TORCH_CHECK(t->device() == target.device(), "verify_drafts: one device");
+  if (n_drafts.has_value()) TORCH_CHECK(n_drafts->scalar_type() == torch::kInt32 && n_drafts->sizes() == u_sample.sizes() && n_drafts->is_contiguous() && n_drafts->device() == target.device(), "verify_drafts: n_drafts int32 [B]");
+  TORCH_CHECK(tokens.scalar_type() == torch::kInt64 && tokens.sizes() == at::IntArrayRef({B, N + 1}) && tokens.is_contiguous() && kept.scalar_type() == torch::kInt64 && kept.numel() == B, "verify_drafts: outputs");
+  const ghb::VerifyArgs a{target.data_ptr(), static_cast<long>(target.stride(0)), static_cast<long>(target.stride(1)), draft.has_value() ? draft->data_ptr() : nullptr,
+                          draft.has_value() ? static_cast<long>(draft->stride(0)) : 0, draft.has_value() ? static_cast<long>(draft->stride(1)) : 0, is_bf16(target),
+                          reinterpret_cast<const long*>(drafts.data_ptr<int64_t>()), u_accept.data_ptr<float>(), u_sample.data_ptr<float>(),
+                          n_drafts.has_value() ? n_drafts->data_ptr<int>() : nullptr, reinterpret_cast<long*>(tokens.data_ptr<int64_t>()),
+                          reinterpret_cast<long*>(kept.data_ptr<int64_t>()), static_cast<int>(B), static_cast<int>(N), static_cast<int>(V), err.data_ptr<int>()};
+  check(ghb::verify_drafts(a, stream()), "verify_drafts");
+}
+
 // ---- fused data-parallel step over peer memory. `peers` is a CPU uint8 tensor holding the pointer table.
 void comm_reduce(const Tensor& peers, int64_t rank, int64_t world, int64_t lo, int64_t n, Tensor& shard, int64_t ticket, int64_t publish_seq,
                  Tensor& acc, Tensor& counter, Tensor& err, int64_t ctas) {
@@ -559,6 +675,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_bwd", &embedding_bwd);
   m.def("decode_attention", &decode_attention);
   m.def("decode_attention_grid", &decode_attention_grid);
+  m.def("paged_append", &paged_append);
+  m.def("paged_read", &paged_read);
+  m.def("paged_attention", &paged_attention);
+  m.def("verify_drafts", &verify_drafts);
   m.def("comm_reduce", &comm_reduce);
   m.def("comm_update", &comm_update);
   m.def("comm_wait_probe", &comm_wait_probe);

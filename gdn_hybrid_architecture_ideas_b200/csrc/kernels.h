@@ -122,4 +122,33 @@ int tp_reduce(const void* args, int N, int* err, int sms, cudaStream_t st);
 int tp_copy_flagged(void* dst, const void* src, size_t bytes, void* flag_dst, const void* flag_src, cudaStream_t st);
 int tp_push_copies(const void* args, const void* seq_src, int pieces, const cudaStream_t* streams, int n_streams);
 
+// ---- paged key/value cache (csrc/paged.cuh has the layout). All pointers are device pointers.
+struct PagedRows {
+  const int* pages; long pages_stride; int width;      // [B, width] page ids
+  const int* q_start; const int* lens; const int* start;      // [B + 1], [B], [B] or null
+  int B, n;             // rows, packed tokens
+  int Hkv, n_pages, page_shift;
+  int* err;
+};
+struct PagedPool { void* k; void* v; uint8_t* k_scale; uint8_t* v_scale; int hd; bool fp4; };
+int paged_append(const PagedRows& r, const PagedPool& c, const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, bool f32,
+                 const float* cos, const float* sin, int half, int n_pos, cudaStream_t st);
+int paged_read(const PagedRows& r, const PagedPool& c, void* ko, void* vo, bool fill, cudaStream_t st);
+struct PagedAttn {
+  const void* q; long q_ts, q_hs; bool q_f32;          // [n, Hq, hd], element strides of a token and a head
+  void* out;                                           // [n, Hq, hd] bf16
+  const float* cos; const float* sin; int half, n_pos, cap;      // cap 0: none (keys are cached rotated)
+  int Hq; float scale; bool fill;
+};
+// Work space of one call: floats of partial results and ints of their descriptions (both may be 0 long).
+struct PagedAttnPlan { int nt, ctas; long ws_floats, ws_ints; };
+int paged_attention_plan(const PagedRows& r, const PagedPool& c, int Hq, int sms, PagedAttnPlan* plan);
+int paged_attention(const PagedRows& r, const PagedPool& c, const PagedAttn& a, const PagedAttnPlan& plan, float* ws, int* meta, cudaStream_t st);
+struct VerifyArgs {
+  const void* target; long t_bs, t_ns; const void* draft; long d_bs, d_ns; bool bf16;      // element strides of a row and a position
+  const long* drafts; const float* u_accept; const float* u_sample; const int* n_drafts;
+  long* tokens; long* kept; int B, N, V; int* err;
+};
+int verify_drafts(const VerifyArgs& a, cudaStream_t st);
+
 }  // namespace ghb

@@ -1,0 +1,215 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// Row b with m drafts x_0 .. x_{m-1}, target probabilities p_i (m + 1 positions) and draft probabilities q_i: draft i is
+// kept while every earlier one is and u_i q_i(x_i) < p_i(x_i). Behind the kept ones comes one drawn token: at the first
+// rejection i from max(p_i - q_i, 0), after the last kept draft from p_m; where that residual is zero everywhere, from p_i.
+// Drawn is the first token whose running sum exceeds u * total. Without draft probabilities each draft counts as certain
+// (q_i(x_i) = 1), so the residual is p_i without x_i.
+//
+// The comparison and the sums run in 64 bits: a product of two float32 is exact there, and running sums of 10^5 terms
+// in another order differ by 1e-16 of the total, so that the token drawn does not depend on how the row was split.
+//
+// Only the row of probabilities that the last token is drawn from is read whole. One cluster of CTAs per row; every warp
+// owns one contiguous range of the vocabulary, sums it (pass 1: all bytes of the row, once), the totals of all warps meet
+// in the shared memory of every CTA of the cluster, each warp finds the range that the threshold falls into, and the one
+// warp that owns it walks it again (pass 2: its range alone, from L1 / L2). No workspace, no atomics, one launch.
+#include <cooperative_groups.h>
+
+#include "paged.cuh"
+
+namespace ghb {
+
+namespace cg = cooperative_groups;
+
+constexpr int VWARPS = 16;
+constexpr int VMAXCL = 8;
+
+template <typename T> __device__ __forceinline__ double to_double(T x) { return static_cast<double>(static_cast<float>(x)); }
+
+// Four consecutive weights at j (j + 3 < V): p, or max(p - q, 0), or p without token x. Anything not above zero (NaN too) is 0.
+template <typename T>
+struct Weights {
+  const T* p; const T* q; int x;       // q null: no subtraction; x: the token left out, or -1
+  bool wide;
+  __device__ __forceinline__ double one(int j) const {
+    double w = to_double(p[j]);
+    if (q) w -= to_double(q[j]);
+    return (w > 0.0 && j != x) ? w : 0.0;
+  }
+  __device__ __forceinline__ void four(int j, double* w) const {
+    float a[4], b[4] = {0.f, 0.f, 0.f, 0.f};
+    if (wide) {
+      load4(p + j, a);
+      if (q) load4(q + j, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { a[i] = static_cast<float>(p[j + i]); if (q) b[i] = static_cast<float>(q[j + i]); }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double d = static_cast<double>(a[i]) - static_cast<double>(b[i]);
+      w[i] = (d > 0.0 && j + i != x) ? d : 0.0;
+    }
+  }
+  static __device__ __forceinline__ void load4(const float* s, float* a) {
+    const float4 u = *reinterpret_cast<const float4*>(s);
+    a[0] = u.x; a[1] = u.y; a[2] = u.z; a[3] = u.w;
+  }
+  static __device__ __forceinline__ void load4(const __nv_bfloat16* s, float* a) {
+    const uint2 u = *reinterpret_cast<const uint2*>(s);
+    const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x)), f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+    a[0] = f0.x; a[1] = f0.y; a[2] = f1.x; a[3] = f1.y;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ double range_sum(const Weights<T>& w, int lo, int hi, int lane) {
+  double s0 = 0.0, s1 = 0.0;
+  int j = lo + lane * 4;
+  for (; j + 128 + 3 < hi; j += 256) {       // two independent groups in flight
+    double a[4], b[4];
+    w.four(j, a); w.four(j + 128, b);
+    s0 += (a[0] + a[1]) + (a[2] + a[3]);
+    s1 += (b[0] + b[1]) + (b[2] + b[3]);
+  }
+  for (; j < hi; j += 128) {
+    if (j + 3 < hi) { double a[4]; w.four(j, a); s0 += (a[0] + a[1]) + (a[2] + a[3]); }
+    else for (int i = j; i < hi; ++i) s0 += w.one(i);
+  }
+  s0 += s1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+  return s0;
+}
+
+// First token of lo .. hi whose running sum, from `before` on, exceeds thr; the last one of positive weight where none does.
+template <typename T>
+__device__ __forceinline__ int range_pick(const Weights<T>& w, int lo, int hi, double before, double thr, int lane) {
+  int live = -1;
+  for (int base = lo; base < hi; base += 128) {
+    const int j = base + lane * 4;
+    double a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = j + i < hi ? w.one(j + i) : 0.0;
+    double run[4] = {a[0], a[0] + a[1], 0.0, 0.0};
+    run[2] = run[1] + a[2]; run[3] = run[2] + a[3];
+    double mine = run[3];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const double up = __shfl_up_sync(0xffffffffu, mine, o); if (lane >= o) mine += up; }
+    double ahead = __shfl_up_sync(0xffffffffu, mine, 1);
+    if (lane == 0) ahead = 0.0;
+    int hit = -1;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) { if (a[i] > 0.0 && before + ahead + run[i] > thr) hit = j + i; }
+    int last = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (a[i] > 0.0) last = j + i;
+    const unsigned m = __ballot_sync(0xffffffffu, hit >= 0);
+    if (m) return __shfl_sync(0xffffffffu, hit, __ffs(m) - 1);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+    live = max(live, last);
+    before += __shfl_sync(0xffffffffu, mine, 31);
+  }
+  return live;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(VWARPS * 32) verify_drafts_kernel(VerifyArgs a) {
+  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ double totals[2][VMAXCL * VWARPS];
+  __shared__ int s_kept;
+  const int CL = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  cluster.barrier_arrive();              // every CTA of the cluster runs before another one writes into its shared memory
+  const int b = blockIdx.x / CL;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* target = static_cast<const T*>(a.target) + b * a.t_bs;
+  const T* draft = a.draft ? static_cast<const T*>(a.draft) + b * a.d_bs : nullptr;
+  const long* drafts = a.drafts + static_cast<long>(b) * a.N;
+  int m = a.n_drafts ? a.n_drafts[b] : a.N;
+  if (m < 0 || m > a.N) { *a.err = ST_DRAFTS; m = m < 0 ? 0 : a.N; }
+  if (warp == 0) {
+    int kept = m;
+    for (int i0 = 0; i0 < m; i0 += 32) {
+      const int i = i0 + lane;
+      bool ok = false;
+      if (i < m) {
+        const long x = drafts[i];
+        if (x < 0 || x >= a.V) *a.err = ST_TOKEN;
+        else {
+          const double q = draft ? to_double(draft[i * a.d_ns + x]) : 1.0;
+          ok = static_cast<double>(a.u_accept[static_cast<long>(b) * a.N + i]) * q < to_double(target[i * a.t_ns + x]);
+        }
+      }
+      const unsigned no = __ballot_sync(0xffffffffu, i < m && !ok);
+      if (no) { kept = i0 + __ffs(no) - 1; break; }
+    }
+    if (lane == 0) s_kept = kept;
+  }
+  __syncthreads();
+  const int kept = s_kept;
+  const bool refused = kept < m;
+  Weights<T> w;
+  w.p = target + kept * a.t_ns;
+  w.q = refused && draft ? draft + kept * a.d_ns : nullptr;
+  w.x = refused && !draft ? static_cast<int>(drafts[kept] >= 0 && drafts[kept] < a.V ? drafts[kept] : -1) : -1;
+  w.wide = (reinterpret_cast<uintptr_t>(w.p) | reinterpret_cast<uintptr_t>(w.q)) % (4 * sizeof(T)) == 0;
+  const int ranges = CL * VWARPS, mine = rank * VWARPS + warp;
+  const int per = ((a.V + ranges - 1) / ranges + 3) & ~3;
+  const int lo = min(a.V, mine * per), hi = min(a.V, lo + per);
+  double total = 0.0;
+  int phase = 0;
+  for (; phase < 2; ++phase) {
+    const double s = range_sum(w, lo, hi, lane);
+    if (phase == 0) cluster.barrier_wait();
+    if (lane < CL) *cluster.map_shared_rank(&totals[phase][mine], lane) = s;
+    cluster.sync();
+    total = 0.0;
+    for (int i = 0; i < ranges; ++i) total += totals[phase][i];
+    if (total > 0.0 || !refused) break;
+    w.q = nullptr; w.x = -1;             // the residual is zero everywhere: the target itself (every CTA sees the same totals)
+  }
+  phase = min(phase, 1);
+  const double thr = static_cast<double>(a.u_sample[b]) * total;
+  int owner = -1, last = -1;
+  double run = 0.0, before = 0.0, before_last = 0.0;
+  for (int i = 0; i < ranges; ++i) {
+    const double t = totals[phase][i];
+    if (t > 0.0) { last = i; before_last = run; }
+    if (owner < 0 && run + t > thr) { owner = i; before = run; }
+    run += t;
+  }
+  if (owner < 0) { owner = last; before = before_last; }
+  long* out = a.tokens + static_cast<long>(b) * (a.N + 1);
+  if (owner == mine) {
+    const int pick = range_pick(w, lo, hi, before, thr, lane);
+    if (lane == 0) out[kept] = pick < 0 ? 0 : pick;
+  }
+  if (rank == 0) {
+    for (int i = threadIdx.x; i <= a.N; i += blockDim.x)
+      if (i != kept) out[i] = i < kept ? drafts[i] : -1;
+    if (threadIdx.x == 0) {
+      a.kept[b] = kept;
+      if (owner < 0) out[kept] = 0;      // a row without any positive probability
+    }
+  }
+}
+
+int verify_drafts(const VerifyArgs& a, cudaStream_t st) {
+  if (a.B == 0) return 0;
+  if (a.V < 1 || a.N < 0 || a.B > 0x7fffffff / VMAXCL) return 1;
+  const int cl = a.V >= 8192 ? VMAXCL : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.B * cl);
+  cfg.blockDim = dim3(VWARPS * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cl; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t rc = a.bf16 ? cudaLaunchKernelEx(&cfg, verify_drafts_kernel<__nv_bfloat16>, a) : cudaLaunchKernelEx(&cfg, verify_drafts_kernel<float>, a);
+  return rc == cudaSuccess ? 0 : 4;
+}
+
+}  // namespace ghb

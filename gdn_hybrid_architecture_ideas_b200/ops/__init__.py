@@ -12,7 +12,9 @@ import os
 
 import torch
 
+from . import paged
 from . import reference as ref
+from .paged import PagedKV
 
 _MODE = os.environ.get("GHB_KERNELS", "native")
 
@@ -235,3 +237,49 @@ def lm_loss_sums(hidden, weight, targets, weights=None, z_loss=0.0, weight_lp=No
     if use_native(hidden):
         return _native().lm_loss_sums(hidden, weight, targets, weights, z_loss, weight_lp)
     return ref.lm_loss_sums(hidden, weight, targets, weights, z_loss)
+
+
+def paged_append(cache, k, v, pages, q_start, lens, start=None, rope=None):
+    """Writes the packed new tokens' keys and values (n, Hkv, hd) into the pages of their rows (`ops.paged` describes the
+    cache and the row tables), in place. rope (cos, sin), each (positions, pairs) float32: the key's first 2 * pairs
+    channels are rotated by the table row (position - start), channel i with channel i + pairs. A decode step is one token a
+    row; a prompt is many. On CUDA: bfloat16 or float32 k, v, head dimension 64 / 128 / 256, a multiple of 16 rotary
+    channels; no read-back, so it can be captured. A wrong table value (page id, length, range, position) is left out and
+    reported on the status word (`check_status`); on the CPU it raises."""
+    if use_native(cache.k):
+        return _native().paged_append(cache, k, v, pages, q_start, lens, start, rope)
+    return paged.paged_append(cache, k, v, pages, q_start, lens, start, rope)
+
+
+def paged_read(cache, pages, q_start, lens, n, out=None):
+    """(k, v), each (n, Hkv, hd): row b's last q_start[b + 1] - q_start[b] cached entries as packed tokens, as they are
+    cached (the inverse of `paged_append`, without undoing a rotation); 4-bit entries as the bfloat16 values they stand
+    for. out: two tensors to write into (their padding rows stay as they are)."""
+    if use_native(cache.k):
+        return _native().paged_read(cache, pages, q_start, lens, n, out)
+    return paged.paged_read(cache, pages, q_start, lens, n, out)
+
+
+def paged_attention(q, cache, pages, q_start, lens, start=None, rope=None, cap=None, scale=None, out=None):
+    """Causal attention (n, Hq, hd) of the packed new tokens over their rows' cached positions, themselves included (append
+    first): token at position p sees start .. p; Hq is a multiple of the cache's heads. q is unrotated. rope without cap: q is
+    rotated at its position, the cached keys are taken as `paged_append` rotated them. rope with cap C (the rotary distance
+    cap): the cache holds unrotated keys, a key at distance d <= C is scored R(p)q . R(t)k, beyond it R(C)q . k. No rope:
+    position-free. A token that sees nothing gets zeros. scale: default hd ** -0.5. Forward only; on CUDA q is bfloat16 or
+    float32, the output bfloat16, under a cap 16, 32 or 64 rotary channels."""
+    if use_native(cache.k):
+        return _native().paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out)
+    return paged.paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out)
+
+
+def verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts=None):
+    """Verification of drafted tokens against the target's probabilities, from given random numbers in [0, 1).
+    target (B, N + 1, V): the target's probabilities at the N drafted positions and the one behind; draft (B, N, V): the
+    probabilities the drafts were drawn from (None: each draft was certain); drafts (B, N) int64; u_accept (B, N), u_sample
+    (B,) float32; n_drafts (B,) int32: drafts of each row (default N). Draft i is kept while all before it are and
+    u_i q_i(x_i) < p_i(x_i); the next token is drawn from max(p - q, 0) at the first refusal, else from the target behind the
+    last draft: the first token whose running sum (in 64 bits) exceeds u_sample times the total. Returns (tokens (B, N + 1):
+    the kept drafts, the drawn token, then -1; kept (B,) int64). The tokens are distributed as the target's own."""
+    if use_native(target):
+        return _native().verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts)
+    return paged.verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts)

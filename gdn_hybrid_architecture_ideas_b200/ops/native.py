@@ -57,13 +57,20 @@ def err_flag(device) -> torch.Tensor:
     return _err[key]
 
 
+# What the kernels over row tables that live on the device report (csrc/paged.cuh); every other code is a wait's.
+STATUS = {301: "paged cache: q_start is not a sequence of ranges of the packed tokens", 302: "paged cache: a row's length is below its new tokens or beyond its pages",
+          303: "paged cache: a start outside the row, or a rotated position before it", 304: "paged cache: a page id outside the cache",
+          305: "paged cache: a position behind the rope table", 306: "verify_drafts: n_drafts outside 0 .. N", 307: "verify_drafts: a drafted token outside the vocabulary"}
+
+
 def check_status(device=None) -> None:
-    """Raises if any kernel reported a protocol timeout since the last check (one host read)."""
+    """Raises if any kernel reported a protocol timeout, or a wrong value in a table on the device, since the last check (one
+    host read)."""
     for key, flag in _err.items():
         code = int(flag.item())
         if code:
             flag.zero_()
-            raise RuntimeError(f"sm_100a kernel reported status {code} on cuda:{key} (a bounded wait gave up)")
+            raise RuntimeError(f"sm_100a kernel reported status {code} on cuda:{key} ({STATUS.get(code, 'a bounded wait gave up')})")
 
 
 BF16 = torch.bfloat16
@@ -686,3 +693,45 @@ def attention(q, k, v, doc, q_far, k_far, cap, pos=None, single_doc=False):
     from . import attention_native
 
     return attention_native.attention(q, k, v, doc, q_far, k_far, cap, pos, single_doc)
+
+
+# ------------------------------------------------------------------------------------------------------------ paged cache, drafts
+
+def paged_append(cache, k, v, pages, q_start, lens, start, rope):
+    cos, sin = (None, None) if rope is None else rope
+    ext().paged_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, pages, q_start, lens, start, cos, sin, err_flag(cache.k.device))
+    _count()
+
+
+def paged_read(cache, pages, q_start, lens, n, out):
+    fill = out is None
+    if fill:
+        shape = (n, cache.n_kv_heads, cache.head_dim)
+        out = (torch.empty(shape, dtype=BF16, device=cache.k.device), torch.empty(shape, dtype=BF16, device=cache.k.device))
+    elif out[0].shape[0] != n:
+        raise ValueError(f"paged_read: out holds {out[0].shape[0]} tokens, n is {n}")
+    ext().paged_read(cache.k, cache.v, cache.k_scale, cache.v_scale, pages, q_start, lens, out[0], out[1], fill, err_flag(cache.k.device))
+    _count()
+    return out
+
+
+def paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out):
+    cos, sin = (None, None) if rope is None else rope
+    if cap is not None and (rope is None or cap < 1):
+        raise ValueError("paged_attention: a rotary distance cap is an integer >= 1 beside a rope table")
+    fill = out is None
+    if fill:
+        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    ext().paged_attention(q.detach(), cache.k, cache.v, cache.k_scale, cache.v_scale, pages, q_start, lens, start, cos, sin, cap or 0,
+                          q.shape[-1] ** -0.5 if scale is None else scale, out, fill, err_flag(cache.k.device))
+    _count(2)
+    return out
+
+
+def verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts):
+    B, N1 = target.shape[:2]
+    tokens = torch.empty(B, N1, dtype=torch.long, device=target.device)
+    kept = torch.empty(B, dtype=torch.long, device=target.device)
+    ext().verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts, tokens, kept, err_flag(target.device))
+    _count()
+    return tokens, kept
