@@ -22,9 +22,13 @@
 // the end of a unit's part. A unit cut by CTA borders leaves partial results (at most two a CTA), joined by a second kernel in
 // the order of the CTAs: no atomics, the same result every time.
 //
-// Loads: cp.async into a ring of tiles private to each warp (no block barrier in the loop); what is not visible
-// (before the start, behind the length, under a bad page id) is not read but filled with zeros.
+// Loads go into a ring of tiles private to each warp (no block barrier in the loop). 4 bits: one more warp loads for all the others
+// (addresses cost as much as the arithmetic of a tile when every warp forms its own: 418 against NNN instructions for 32
+// positions), one bulk copy for the part of a tile that lies in one page, counted on an mbarrier of the stage (waits are
+// bounded); what no row sees gets scales of zero, so that its values are zero. bfloat16: cp.async, 16 bytes a lane, positions that are not visible filled
+// with zeros.
 #include "paged.cuh"
+#include "sm100.cuh"
 
 namespace ghb {
 
@@ -34,43 +38,56 @@ struct AttnK {                       // by value to the kernels
   float* ws; int* meta;
 };
 
-template <bool FP4, int HD> struct Cfg;
-template <> struct Cfg<true, 64> { static constexpr int W = 8, ST = 4, CTAS = 2; };
-template <> struct Cfg<true, 128> { static constexpr int W = 8, ST = 3, CTAS = 2; };
-template <> struct Cfg<true, 256> { static constexpr int W = 4, ST = 3, CTAS = 2; };
-template <> struct Cfg<false, 64> { static constexpr int W = 8, ST = 3, CTAS = 2; };
-template <> struct Cfg<false, 128> { static constexpr int W = 4, ST = 3, CTAS = 2; };
-template <> struct Cfg<false, 256> { static constexpr int W = 4, ST = 3, CTAS = 1; };
+// W warps that compute, ST ring stages each, CTAS a SM, MT 16-position tiles a warp takes at once. With the loading warp the
+// block has a multiple of four warps, which is how registers are shared out; blocks of more query rows need more of them, so
+// fewer warps.
+template <bool FP4, int HD, int NT> struct Cfg;
+template <> struct Cfg<true, 64, 1> { static constexpr int W = 7, ST = 3, CTAS = 2, MT = 4; };
+template <> struct Cfg<true, 64, 3> { static constexpr int W = 11, ST = 4, CTAS = 1, MT = 2; };
+template <> struct Cfg<true, 128, 1> { static constexpr int W = 7, ST = 3, CTAS = 2, MT = 2; };
+template <> struct Cfg<true, 128, 2> { static constexpr int W = 11, ST = 3, CTAS = 1, MT = 2; };
+template <int NT> struct Cfg<true, 256, NT> { static constexpr int W = 7, ST = NT == 1 ? 3 : 2, CTAS = 1, MT = 2; };
+template <> struct Cfg<false, 64, 1> { static constexpr int W = 8, ST = 3, CTAS = 2, MT = 1; };
+template <> struct Cfg<false, 64, 3> { static constexpr int W = 8, ST = 3, CTAS = 1, MT = 1; };
+template <int NT> struct Cfg<false, 128, NT> { static constexpr int W = 4, ST = 3, CTAS = 2, MT = 1; };
+template <int NT> struct Cfg<false, 256, NT> { static constexpr int W = NT == 1 ? 6 : 4, ST = 2, CTAS = 1, MT = 1; };
 
 template <bool FP4, int HD, int NT>
-struct Geo : Cfg<FP4, HD> {
-  using B = Cfg<FP4, HD>;
-  static constexpr int MT = FP4 ? 2 : 1;             // 16-position tiles a warp takes at once
+struct Geo : Cfg<FP4, HD, NT> {
+  using B = Cfg<FP4, HD, NT>;
+  static constexpr int MT = B::MT, ST = B::ST;
   static constexpr int TILE = 16 * MT;
   static constexpr int H = HD / 64;                  // 64-channel slices
-  static constexpr int KB = FP4 ? TILE * HD / 2 : TILE * HD * 2;      // bytes of a tile's keys (values the same)
-  static constexpr int SB = FP4 ? TILE * HD / 16 : 0;                 // bytes of its scales
+  static constexpr int ROW = FP4 ? HD / 2 : HD * 2;  // bytes of a position
+  static constexpr int S = HD / 16;                  // scale bytes of a position
+  static constexpr int KB = TILE * ROW;              // bytes of a tile's keys (values the same)
+  static constexpr int SB = FP4 ? TILE * S : 0;      // bytes of its scales
   static constexpr int STAGE = 2 * KB + 2 * SB;
   static constexpr int UR = 8 * NT;                  // query rows of a unit
   static constexpr int PIECE = B::W * TILE;
-  static constexpr int RING = B::W * B::ST * STAGE;
+  static constexpr int RING = B::W * ST * STAGE;
   static constexpr int MERGE = B::W * UR * HD * 4;
   static constexpr int DATA = RING > MERGE ? RING : MERGE;
   static constexpr int QCOPIES = FP4 ? 1 : 2;        // bfloat16: high and low part
   static constexpr int QB = UR * HD * 2;             // bytes of one copy of the queries
-  static constexpr int SMEM = DATA + 2 * QCOPIES * QB;       // near and far queries
-  static constexpr int THREADS = B::W * 32;
+  // under a cap: near and far queries, the near ones' rotary channels in float32 and as each warp rotated them, a tile of rotations
+  __host__ __device__ static constexpr int q_bytes(bool cap) { return (cap ? 2 : 1) * QCOPIES * QB; }
+  __host__ __device__ static constexpr int turned_bytes(int half) { return NT * (half / 8) * 256 * QCOPIES; }      // of a warp
+  __host__ __device__ static constexpr int smem(int cap_half) {
+    return DATA + q_bytes(cap_half > 0) + UR * 2 * cap_half * 4 + TILE * cap_half * 8 + B::W * turned_bytes(cap_half);
+  }
+  static constexpr int THREADS = (B::W + (FP4 ? 1 : 0)) * 32;        // 4 bits: one more warp, which loads for the others
 };
 
 constexpr float PSHIFT = 14.f;
 
+// size bytes (a multiple of 16, both addresses on 16-byte boundaries) into this CTA's shared memory, counted on the barrier
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t size, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(size), "r"(sm100::smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-template <int BYTES>
-__device__ __forceinline__ void cp_small(uint32_t dst, const void* src, bool on) {
-  if constexpr (BYTES == 16) cp16(dst, src, on);
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(on ? BYTES : 0), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -84,6 +101,16 @@ __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, ui
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the first product of a sum: no addend
+template <bool FP4>
+__device__ __forceinline__ void mma_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (FP4)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -94,11 +121,18 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t hmul2_low(uint32_t a, uint32_t b) {        // both by b's low half
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), __low2half2(*reinterpret_cast<const __half2*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 // eight codes (a 32-bit word) -> four f16 pairs
 __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t* h) {
   asm("{\n\t.reg .b8 c0, c1, c2, c3;\n\tmov.b32 {c0, c1, c2, c3}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, c0;\n\tcvt.rn.f16x2.e2m1x2 %1, c1;\n\t"
       "cvt.rn.f16x2.e2m1x2 %2, c2;\n\tcvt.rn.f16x2.e2m1x2 %3, c3;\n\t}"
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+__device__ __forceinline__ void code_to_f16(uint32_t byte, uint32_t& h) {        // the low byte's two codes
+  asm("{\n\t.reg .b8 c0, c1, c2, c3;\n\tmov.b32 {c0, c1, c2, c3}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, c0;\n\t}" : "=r"(h) : "r"(byte));
 }
 // two E4M3 scales (bytes 0 and 1) -> an f16 pair
 __device__ __forceinline__ uint32_t scales_to_f16(uint32_t two) {
@@ -153,55 +187,79 @@ __device__ __forceinline__ long block_scan(long x, long* s_warp, long* total) {
   return before + inc - x;      // exclusive
 }
 
-template <bool FP4, int HD, int NT>
+template <bool FP4, int HD, int NT, bool CAP>
 __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::CTAS) paged_attention_kernel(const __grid_constant__ AttnK p) {
   using GEO = Geo<FP4, HD, NT>;
   constexpr int H = GEO::H, MT = GEO::MT, TILE = GEO::TILE, UR = GEO::UR, W = GEO::W, ST = GEO::ST;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long s_warp[W];
+  __shared__ long s_warp[GEO::THREADS / 32];
   __shared__ long s_at[2];
   __shared__ float s_mul[UR];                 // a query row's factor on its scores: scale * log2(e) * its power of two
   __shared__ float s_m[W][UR], s_l[W][UR];
+  __shared__ int s_pos[UR];                   // a query row's position
+  __shared__ uint64_t s_full[W][ST], s_free[W][ST];      // 4 bits: a warp's ring stage is loaded; is consumed
+  __shared__ unsigned s_on[W][ST];                       // the stage's chunks that were read
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const PagedRows& R = p.r;
   const int n_ctas = gridDim.x, cta = blockIdx.x, Hkv = R.Hkv, G = p.G;
 
   // ---- this CTA's share of the pieces
-  long total = 0;
-  if (tid < 2) s_at[tid] = -1;
+  auto pieces_of = [&](int i) -> long {
+    if (i >= R.B) return 0;
+    const RowWork w = row_work<GEO>(load_row(R, i), G);
+    return static_cast<long>(w.units) * w.pieces * Hkv;
+  };
+  long total = 0, mine = 0, ex = 0;
   for (int b0 = 0; b0 < R.B; b0 += GEO::THREADS) {
-    long mine = 0, all;
-    if (b0 + tid < R.B) { const RowWork w = row_work<GEO>(load_row(R, b0 + tid), G); mine = static_cast<long>(w.units) * w.pieces * Hkv; }
-    block_scan<GEO::THREADS>(mine, s_warp, &all);
+    long all;
+    mine = pieces_of(b0 + tid);
+    ex = total + block_scan<GEO::THREADS>(mine, s_warp, &all);
     total += all;
   }
   const long use = total < n_ctas ? total : n_ctas;      // CTAs with work: at least one piece each
   int* meta = p.meta + cta * 8;
-  if (cta >= use) {
-    if (tid < 2) meta[tid * 4] = -1;
-    return;
-  }
+  if (tid == 0) meta[0] = 0;                  // parts of the unit that this CTA begins and others end
+  if (cta >= use) return;
   const long lo = total * cta / use, hi = total * (cta + 1) / use;
-  {
+  if (R.B <= GEO::THREADS) {
+    if (lo >= ex && lo < ex + mine) { s_at[0] = tid; s_at[1] = ex; }
+  } else {
     long before = 0;
-    for (int b0 = 0; b0 < R.B; b0 += GEO::THREADS) {
-      long mine = 0, all;
-      if (b0 + tid < R.B) { const RowWork w = row_work<GEO>(load_row(R, b0 + tid), G); mine = static_cast<long>(w.units) * w.pieces * Hkv; }
-      const long ex = before + block_scan<GEO::THREADS>(mine, s_warp, &all);
+    for (int b0 = 0; before <= lo; b0 += GEO::THREADS) {
+      long all;
+      mine = pieces_of(b0 + tid);
+      ex = before + block_scan<GEO::THREADS>(mine, s_warp, &all);
       if (lo >= ex && lo < ex + mine) { s_at[0] = b0 + tid; s_at[1] = ex; }
       before += all;
-      if (before > lo) break;
     }
   }
   __syncthreads();
   int b = static_cast<int>(s_at[0]);
   long row_at = s_at[1];
-  if (tid < 2) meta[tid * 4] = -1;
   __syncthreads();
 
+  if (FP4) {
+    for (int i = tid; i < W * ST; i += GEO::THREADS) { sm100::mbar_init(&s_full[0][0] + i, 1); sm100::mbar_init(&s_free[0][0] + i, 1); }
+    sm100::mbar_fence_init();
+    __syncthreads();
+  }
+  int stage = 0;                              // 4 bits: of the next tile, through all segments (every piece gives every warp one tile)
+  unsigned phase = 0;
+  bool dead = false;                          // a wait gave up: the status word says so, nothing more is waited for
   uint8_t* ring = smem + warp * (ST * GEO::STAGE);
   const uint32_t ring_u = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   uint8_t* sq = smem + GEO::DATA;
+  const int half = p.a.half;
+  float* sq_base = reinterpret_cast<float*>(sq + GEO::q_bytes(CAP));                       // [UR][2 half]
+  float4* s_turn = reinterpret_cast<float4*>(sq_base + UR * 2 * half);                     // [TILE][half / 2]: cos, cos, sin, sin of two pairs
+  uint8_t* s_turned = reinterpret_cast<uint8_t*>(s_turn + TILE * (half >> 1)) + warp * GEO::turned_bytes(half);
+  if constexpr (CAP) {
+    for (int i = tid; i < TILE * (half >> 1); i += GEO::THREADS) {
+      const int d = min(i / (half >> 1), p.a.n_pos - 1), j = i % (half >> 1);
+      const float2 c = *reinterpret_cast<const float2*>(p.a.cos + static_cast<long>(d) * half + 2 * j), sn = *reinterpret_cast<const float2*>(p.a.sin + static_cast<long>(d) * half + 2 * j);
+      s_turn[i] = make_float4(c.x, c.y, sn.x, sn.y);
+    }
+  }
 
   long at = lo;
   while (at < hi) {
@@ -223,53 +281,95 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     const int n_rows = min(UR, row.nq * G - r0);
     const int pos0 = row.len - row.nq;                              // position of the row's first new token
     const int p_first = pos0 + r0 / G, p_last = row.len ? pos0 + (r0 + n_rows - 1) / G : -1;
-    // ---- loads of one tile: positions base .. base + TILE
+    // ---- loads of one tile: positions tile0 + k PIECE .. + TILE. 4 bits: a tile is one or more chunks, each within a page and so
+    // contiguous per head; a lane of the loading warp copies a chunk (keys, values, their scales) in bulk. bfloat16: lane i owns
+    // position i of its warp's tile.
     const int tile0 = wk.base + p0 * GEO::PIECE + warp * TILE;
-    auto page_at = [&](int k) -> int {         // page id of this lane's position of tile k, -1: not read
-      const int tok = tile0 + k * GEO::PIECE + (lane & (TILE - 1));
-      if (k >= n_pieces || tok < row.start || tok > p_last) return -1;
+    const int c_shift = FP4 ? min(R.page_shift, MT == 4 ? 6 : MT == 2 ? 5 : 4) : 0;
+    const int n_chunks = TILE >> c_shift;
+    const unsigned all_on = n_chunks == 32 ? 0xffffffffu : (1u << n_chunks) - 1u;
+    auto page_of = [&](int tok) -> int {       // page id of a chunk or position, -1: not read
+      if (tok + (1 << c_shift) <= row.start || tok > p_last) return -1;
       const int pg = R.pages[b * R.pages_stride + (tok >> R.page_shift)];
       if (pg < 0 || pg >= R.n_pages) { *R.err = ST_PAGE; return -1; }
       return pg;
     };
-    auto issue = [&](int k, int pg) -> unsigned {      // returns the mask of positions that are read
-      const int tok = tile0 + k * GEO::PIECE + (lane & (TILE - 1));
-      const unsigned on = __ballot_sync(0xffffffffu, pg >= 0);
-      if (k < n_pieces) {
-        const uint32_t st = ring_u + (k % ST) * GEO::STAGE;
-        const int e = pg >= 0 ? ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1)) : 0;
-        constexpr int ROW = FP4 ? HD / 2 : HD * 2, CH = ROW / 16;      // bytes and 16-byte chunks of a position
-        const uint8_t* kb = static_cast<const uint8_t*>(p.c.k);
-        const uint8_t* vb = static_cast<const uint8_t*>(p.c.v);
-#pragma unroll
-        for (int i = 0; i < TILE * CH / 32; ++i) {
-          const int idx = i * 32 + lane, pos = idx / CH, sub = idx % CH;
-          const int ee = __shfl_sync(0xffffffffu, e, pos);
-          const bool ok = (on >> pos) & 1;
-          uint32_t dst;
-          if constexpr (FP4) dst = (sub >> 1) * (TILE * 32) + pos * 32 + (sub & 1) * 16;
-          else dst = (sub >> 3) * (TILE * 128) + pos * 128 + (((sub & 7) ^ (pos & 7)) << 4);
-          const long off = static_cast<long>(ee) * ROW + sub * 16;
-          cp16(st + dst, kb + off, ok);
-          cp16(st + GEO::KB + dst, vb + off, ok);
-        }
-        if constexpr (FP4) {
-          constexpr int S = HD / 16;
-          const long off = static_cast<long>(e) * S;
-          cp_small<S>(st + 2 * GEO::KB + lane * S, p.c.k_scale + off, pg >= 0);
-          cp_small<S>(st + 2 * GEO::KB + GEO::SB + lane * S, p.c.v_scale + off, pg >= 0);
+    const int base = wk.base + p0 * GEO::PIECE, n_all = W * n_chunks;               // chunks of a piece, in rounds of 32 lanes
+    int pg = FP4 && warp == W && lane < n_all ? page_of(base + (lane << c_shift)) : -1;
+    auto produce = [&](int k_from, int k_to) {                                      // the loading warp: pieces k_from .. k_to
+      if constexpr (FP4) {
+        const int lo_shift = __ffs(n_chunks) - 1;
+        for (int k = k_from; k < k_to && !dead; ++k) {
+          for (int i0 = 0; i0 < n_all; i0 += 32) {
+            const int i = i0 + lane;
+            const int tok = base + k * GEO::PIECE + (i << c_shift);
+            // the next round's page ids are on their way while this one waits for its stages
+            const bool more = i0 + 32 < n_all;
+            const int i2 = more ? i + 32 : lane, k2 = more ? k : k + 1;
+            const int pg2 = i2 < n_all && k2 < n_pieces ? page_of(base + k2 * GEO::PIECE + (i2 << c_shift)) : -1;
+            const unsigned on = __ballot_sync(0xffffffffu, pg >= 0);
+            const int w = i >> lo_shift;
+            bool ok = true;
+            if (i < n_all && (i & (n_chunks - 1)) == 0) {
+              ok = sm100::mbar_wait(&s_free[w][stage], phase ^ 1u);
+              const unsigned mine = (on >> lane) & all_on;
+              s_on[w][stage] = mine;
+              if (ok) sm100::mbar_expect_tx(&s_full[w][stage], (__popc(mine) << c_shift) * (2 * GEO::ROW + 2 * GEO::S));
+            }
+            if (__any_sync(0xffffffffu, !ok)) { *R.err = ST_WAIT; dead = true; break; }
+            if (pg >= 0) {
+              const int e = ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1));
+              const int at_c = (i & (n_chunks - 1)) << c_shift;
+              const uint32_t st = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (w * ST + stage) * GEO::STAGE;
+              uint64_t* bar = &s_full[w][stage];
+              bulk_load(st + at_c * GEO::ROW, static_cast<const uint8_t*>(p.c.k) + static_cast<long>(e) * GEO::ROW, GEO::ROW << c_shift, bar);
+              bulk_load(st + GEO::KB + at_c * GEO::ROW, static_cast<const uint8_t*>(p.c.v) + static_cast<long>(e) * GEO::ROW, GEO::ROW << c_shift, bar);
+              bulk_load(st + 2 * GEO::KB + at_c * GEO::S, p.c.k_scale + static_cast<long>(e) * GEO::S, GEO::S << c_shift, bar);
+              bulk_load(st + 2 * GEO::KB + GEO::SB + at_c * GEO::S, p.c.v_scale + static_cast<long>(e) * GEO::S, GEO::S << c_shift, bar);
+            }
+            pg = pg2;
+          }
+          if (++stage == ST) { stage = 0; phase ^= 1u; }
         }
       }
-      cp_commit();
+    };
+    // (every stage is free at the start of a unit's part: the first ST pieces wait for nobody, so this may stand before the barrier)
+    if (FP4 && warp == W) produce(0, min(ST, n_pieces));
+    auto issue = [&](int k) -> unsigned {      // bfloat16: returns the mask of positions that are read
+      unsigned on = 0;
+      if constexpr (!FP4) {
+        const int tok = tile0 + k * GEO::PIECE + lane;
+        const int pg = k < n_pieces && lane < TILE ? page_of(tok) : -1;
+        on = __ballot_sync(0xffffffffu, pg >= 0);
+        if (on) {
+          const uint32_t st = ring_u + (k % ST) * GEO::STAGE;
+          const int e = pg >= 0 ? ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1)) : 0;
+          const uint8_t* kb = static_cast<const uint8_t*>(p.c.k);
+          const uint8_t* vb = static_cast<const uint8_t*>(p.c.v);
+          constexpr int CH = GEO::ROW / 16;
+#pragma unroll
+          for (int i = 0; i < TILE * CH / 32; ++i) {
+            const int idx = i * 32 + lane, pos = idx / CH, sub = idx % CH;
+            const int ee = __shfl_sync(0xffffffffu, e, pos);
+            const bool ok = (on >> pos) & 1;
+            const uint32_t dst = (sub >> 3) * (TILE * 128) + pos * 128 + (((sub & 7) ^ (pos & 7)) << 4);
+            const long off = static_cast<long>(ee) * GEO::ROW + sub * 16;
+            cp16(st + dst, kb + off, ok);
+            cp16(st + GEO::KB + dst, vb + off, ok);
+          }
+        }
+        cp_commit();
+      }
       return on;
     };
     unsigned on_ring[ST];
+    if constexpr (!FP4) {
 #pragma unroll
-    for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k, page_at(k));
-    int pg_next = page_at(ST - 1);
+      for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k);
+    }
 
     // ---- the unit's queries: rotated (near at their positions, far by the cap), brought to about one, in the MMA's order
-    for (int r = warp; r < UR; r += W) {
+    for (int r = warp; r < UR && warp < W; r += W) {
       const bool live = r < n_rows && row.len > 0;
       const int rr = r0 + r;
       const long tok = row.q0 + (live ? rr / G : 0);
@@ -289,39 +389,45 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       ex = max(-120, min(120, ex));
       const float down = exp2f(static_cast<float>(-ex));
       if (lane == 0) s_mul[r] = p.a.scale * 1.44269504088896340736f * exp2f(static_cast<float>(ex));
+      if (lane == 0) s_pos[r] = live ? pos0 + rr / G : -1;
       int qpos = pos0 + rr / G - row.start;
-      if (live && p.a.half > 0 && qpos >= p.a.n_pos) { *R.err = ST_ROPE; qpos = p.a.n_pos - 1; }
-      qpos = max(qpos, 0);
+      if (live && half > 0 && qpos >= p.a.n_pos) { *R.err = ST_ROPE; qpos = p.a.n_pos - 1; }
+      qpos = CAP ? p.a.cap : max(qpos, 0);
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {
-        const int c = lane + 32 * i, half = p.a.half;
-        float near = x[i], far = x[i];
+        const int c = lane + 32 * i;
+        float turned = x[i];                   // by the position, under a cap by the cap
         if (live && c < 2 * half) {
           const bool lowside = c < half;
           const int ai = lowside ? c : c - half;
           const float y = qv(lowside ? c + half : c - half), sg = lowside ? -y : y;
-          near = x[i] * p.a.cos[static_cast<long>(qpos) * half + ai] + sg * p.a.sin[static_cast<long>(qpos) * half + ai];
-          if (p.a.cap) far = x[i] * p.a.cos[static_cast<long>(p.a.cap) * half + ai] + sg * p.a.sin[static_cast<long>(p.a.cap) * half + ai];
+          turned = x[i] * p.a.cos[static_cast<long>(qpos) * half + ai] + sg * p.a.sin[static_cast<long>(qpos) * half + ai];
         }
+        // the order of the plain products (a lane owns the 16 channels 16 t .. of each slice), and of the rotating ones (its
+        // channels are 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16)
         const int cc = c & 63;
-        const int idx = ((((r >> 3) * (HD / 16) + (c >> 6) * 4 + ((cc & 15) >> 2)) * 32 + (r & 7) * 4 + (cc >> 4)) << 2) + (cc & 3);
-        if constexpr (FP4) {
-          reinterpret_cast<__half*>(sq)[idx] = __float2half_rn(near * down);
-          if (p.a.cap) reinterpret_cast<__half*>(sq + GEO::QB)[idx] = __float2half_rn(far * down);
-        } else {
-          const __nv_bfloat16 n1 = __float2bfloat16(near), f1 = __float2bfloat16(far);
-          reinterpret_cast<__nv_bfloat16*>(sq)[idx] = n1;
-          // (an infinite part has no remainder: inf - inf would turn it into NaN a second time, which it is in the product anyway)
-          reinterpret_cast<__nv_bfloat16*>(sq + GEO::QB)[idx] = __float2bfloat16(isfinite(near) ? near - __bfloat162float(n1) : 0.f);
-          if (p.a.cap) {
-            reinterpret_cast<__nv_bfloat16*>(sq + 2 * GEO::QB)[idx] = f1;
-            reinterpret_cast<__nv_bfloat16*>(sq + 3 * GEO::QB)[idx] = __float2bfloat16(isfinite(far) ? far - __bfloat162float(f1) : 0.f);
+        const int plain_at = ((((r >> 3) * (HD / 16) + (c >> 6) * 4 + ((cc & 15) >> 2)) * 32 + (r & 7) * 4 + (cc >> 4)) << 2) + (cc & 3);
+        const int near_at = ((((r >> 3) * (HD / 16) + (c >> 4)) * 32 + (r & 7) * 4 + ((c & 7) >> 1)) << 2) + ((c >> 2) & 2) + (c & 1);
+        auto put = [&](uint8_t* to, int idx, float v) {
+          if constexpr (FP4) {
+            reinterpret_cast<__half*>(to)[idx] = __float2half_rn(v);
+          } else {
+            const __nv_bfloat16 hi = __float2bfloat16(v);
+            reinterpret_cast<__nv_bfloat16*>(to)[idx] = hi;
+            // (an infinity has no remainder)
+            reinterpret_cast<__nv_bfloat16*>(to + GEO::QB)[idx] = __float2bfloat16(isfinite(v) ? v - __bfloat162float(hi) : 0.f);
           }
+        };
+        put(sq, plain_at, turned * down);
+        if constexpr (CAP) {
+          put(sq + GEO::QCOPIES * GEO::QB, near_at, x[i] * down);          // (its rotary channels are not read)
+          if (c < 2 * half) sq_base[r * 2 * half + c] = x[i] * down;
         }
       }
     }
     __syncthreads();
 
+    const int live_n = NT == 1 ? 1 : (n_rows + 7) >> 3;        // 8-row column blocks in use
     float mul[NT][2], m[NT][2], l[NT][2];
     int prow[NT][2];
 #pragma unroll
@@ -341,211 +447,241 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
 
-    for (int k = 0; k < n_pieces; ++k) {
-      {
-        const unsigned on = issue(k + ST - 1, pg_next);
-        pg_next = page_at(k + ST);
+    if (FP4 && warp == W) produce(ST, n_pieces);
+    for (int k = 0; k < n_pieces && warp < W; ++k) {
+      const int first = tile0 + k * GEO::PIECE;
+      unsigned on;
+      uint8_t* st;
+      if constexpr (FP4) {
+        if (!dead && !sm100::mbar_wait(&s_full[warp][stage], phase)) { *R.err = ST_WAIT; dead = true; }
+        dead = __any_sync(0xffffffffu, dead);
+        on = s_on[warp][stage];
+        st = ring + stage * GEO::STAGE;
+      } else {
+        on_ring[ST - 1] = issue(k + ST - 1);
+        on = on_ring[0];
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) on_ring[i] = on_ring[i + 1];        // the masks travel with the ring
         cp_wait<ST - 1>();
         __syncwarp();
-        // the masks travel with the ring
-        const unsigned now = on_ring[0];
-#pragma unroll
-        for (int i = 0; i < ST - 2; ++i) on_ring[i] = on_ring[i + 1];
-        on_ring[ST - 2] = on;
-        on_ring[ST - 1] = now;
+        st = ring + (k % ST) * GEO::STAGE;
       }
-      const unsigned on = on_ring[ST - 1];
-      const int first = tile0 + k * GEO::PIECE;
-      if (on) {
-        const uint8_t* st = ring + (k % ST) * GEO::STAGE;
-        const bool far_any = p.a.cap && p_last - first > p.a.cap;                       // some (row, position) beyond the cap
-        const bool near_any = !p.a.cap || p_first - (first + TILE - 1) <= p.a.cap;      // some within it
+      if (on && !dead) {
+        const bool masked = on != all_on || first < row.start || first + TILE - 1 > p_first;
+        if (FP4 && masked) {
+          // what no row sees may hold anything: its scales become zero, so that its values are zero
+          for (int pos = lane; pos < TILE; pos += 32) {
+            if (!((on >> (pos >> c_shift)) & 1) || first + pos < row.start || first + pos > p_last) {
+#pragma unroll
+              for (int i = 0; i < GEO::S / 4; ++i) *reinterpret_cast<uint32_t*>(st + 2 * GEO::KB + GEO::SB + pos * GEO::S + 4 * i) = 0u;
+            }
+          }
+          sm100::fence_proxy_async();        // before a later bulk copy into the stage
+          __syncwarp();
+        }
         float s[MT][NT][4];
-
-        auto score = [&](bool rotate, const uint8_t* qs, float (&acc)[MT][NT][4]) {
+        // one k16 step of the 16 positions of tile mt against every column block; its queries start at qs, a block's at by bytes further
+        auto step = [&](float (&acc)[NT][4], const uint32_t* a, const uint8_t* qs, int by, int low, bool begin) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (NT > 1 && n >= live_n) continue;
+            const uint2 q1 = *reinterpret_cast<const uint2*>(qs + n * by + lane * 8);
+            if (begin) mma_first<FP4>(acc[n], a, q1.x, q1.y);
+            else mma<FP4>(acc[n], a, q1.x, q1.y);
+            if constexpr (!FP4) {
+              const uint2 q2 = *reinterpret_cast<const uint2*>(qs + low + n * by + lane * 8);
+              mma<FP4>(acc[n], a, q2.x, q2.y);
+            }
+          }
+        };
+        const bool far_any = !CAP || p_last - first > p.a.cap;                     // some (row, position) beyond the cap
+        const bool near_any = CAP && p_first - (first + TILE - 1) <= p.a.cap;      // some within it
+        if (far_any) {
+          // ---- keys as cached: a lane owns 16 consecutive channels of a slice (4 bits: one block)
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[mt][n][e] = 0.f;
-#pragma unroll
-          for (int hs = 0; hs < H; ++hs) {
-            uint32_t x[MT][2][8];                // [tile][row g or g + 8][channel pair]: channels 16 t + 2 i of slice hs
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int hs = 0; hs < H; ++hs) {
+              uint32_t x[2][8];                // [row g or g + 8][channel pair]: channels 16 t + 2 i of slice hs
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int pos = mt * 16 + e * 8 + place<FP4>(g);
                 if constexpr (FP4) {
-                  const uint2 w = *reinterpret_cast<const uint2*>(st + hs * (TILE * 32) + pos * 32 + t * 8);
-                  uint32_t sc = st[2 * GEO::KB + pos * (HD / 16) + hs * 4 + t];
-                  sc = scales_to_f16(sc | (sc << 8));
-                  codes_to_f16(w.x, x[mt][e]);
-                  codes_to_f16(w.y, x[mt][e] + 4);
+                  const uint2 w = *reinterpret_cast<const uint2*>(st + pos * GEO::ROW + hs * 32 + t * 8);
+                  const uint32_t sc = scales_to_f16(st[2 * GEO::KB + pos * GEO::S + hs * 4 + t]);
+                  codes_to_f16(w.x, x[e]);
+                  codes_to_f16(w.y, x[e] + 4);
 #pragma unroll
-                  for (int i = 0; i < 8; ++i) x[mt][e][i] = hmul2(x[mt][e][i], sc);
+                  for (int i = 0; i < 8; ++i) x[e][i] = hmul2_low(x[e][i], sc);
                 } else {
 #pragma unroll
                   for (int c = 0; c < 2; ++c) {
                     const uint4 w = *reinterpret_cast<const uint4*>(st + hs * (TILE * 128) + pos * 128 + (((2 * t + c) ^ (pos & 7)) << 4));
-                    x[mt][e][4 * c] = w.x; x[mt][e][4 * c + 1] = w.y; x[mt][e][4 * c + 2] = w.z; x[mt][e][4 * c + 3] = w.w;
+                    x[e][4 * c] = w.x; x[e][4 * c + 1] = w.y; x[e][4 * c + 2] = w.z; x[e][4 * c + 3] = w.w;
                   }
                 }
               }
-            if (hs == 0 && rotate) {
-              // channel i < half with i + half: both in this lane (half 8), or in the lane half / 16 away
-              const int half = p.a.half;
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
+              for (int ks = 0; ks < 4; ++ks) {
+                const uint32_t a[4] = {x[0][2 * ks], x[1][2 * ks], x[0][2 * ks + 1], x[1][2 * ks + 1]};
+                step(s[mt], a, sq + (hs * 4 + ks) * 256, HD * 16, GEO::QB, hs == 0 && ks == 0);
+              }
+            }
+        }
+        if constexpr (CAP) {
+          if (near_any) {
+            // ---- keys within the cap. R(p) q . R(t) k = R(p - t0) q . R(t - t0) k with t0 the tile's first position: the keys take
+            // one of TILE rotations that stay in shared memory, the queries' rotary channels are rotated once a tile. A lane owns channels
+            // 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16, so that both channels of a rotary pair (half 8, 16 or 32
+            // apart) are its own.
+            const int t0 = max(first, row.start);
+            const int steps = half >> 3, slot_low = NT * steps * 256;          // rotary k16 steps; bytes of the high parts
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int tok = first + mt * 16 + e * 8 + place<FP4>(g);
-                  const int pp = max(0, min(tok - row.start, p.a.n_pos - 1));
-                  const float* co = p.a.cos + static_cast<long>(pp) * half;
-                  const float* si = p.a.sin + static_cast<long>(pp) * half;
-                  uint32_t* y = x[mt][e];
-                  if (half == 8) {
-                    if (t == 0) {
+            for (int n = 0; n < NT; ++n) {
+              if (NT > 1 && n >= live_n) continue;
+              const int r = n * 8 + g;
+              const long d = max(0, min(s_pos[r] - t0, p.a.n_pos - 1));
+              const float* co = p.a.cos + d * half + 2 * t;
+              const float* si = p.a.sin + d * half + 2 * t;
+              const float* qb = sq_base + r * 2 * half + 2 * t;
 #pragma unroll
-                      for (int i = 0; i < 4; ++i) {
-                        const float2 a = unpack<FP4>(y[i]), bb = unpack<FP4>(y[i + 4]);
-                        const float2 c = *reinterpret_cast<const float2*>(co + 2 * i), sn = *reinterpret_cast<const float2*>(si + 2 * i);
-                        y[i] = pack<FP4>(a.x * c.x - bb.x * sn.x, a.y * c.y - bb.y * sn.y);
-                        y[i + 4] = pack<FP4>(bb.x * c.x + a.x * sn.x, bb.y * c.y + a.y * sn.y);
-                      }
-                    }
-                  } else {
-                    const int away = half >> 4;            // 1 or 2 lanes
-                    const int base = (t & (away - 1)) * 16;
-                    const bool lowside = (t & away) == 0, mine = t * 16 < 2 * half;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                      const uint32_t other = __shfl_xor_sync(0xffffffffu, y[i], away);
-                      if (mine) {
-                        const float2 a = unpack<FP4>(y[i]), bb = unpack<FP4>(other);
-                        const float2 c = *reinterpret_cast<const float2*>(co + base + 2 * i), sn = *reinterpret_cast<const float2*>(si + base + 2 * i);
-                        const float sx = lowside ? -sn.x : sn.x, sy = lowside ? -sn.y : sn.y;
-                        y[i] = pack<FP4>(a.x * c.x + bb.x * sx, a.y * c.y + bb.y * sy);
-                      }
-                    }
+              for (int i = 0; i < 4; ++i) {
+                if (i >= steps) break;
+                const float2 c = *reinterpret_cast<const float2*>(co + 8 * i), sn = *reinterpret_cast<const float2*>(si + 8 * i);
+                const float2 u = *reinterpret_cast<const float2*>(qb + 8 * i), v = *reinterpret_cast<const float2*>(qb + half + 8 * i);
+                const float2 a = make_float2(u.x * c.x - v.x * sn.x, u.y * c.y - v.y * sn.y), z = make_float2(v.x * c.x + u.x * sn.x, v.y * c.y + u.y * sn.y);
+                auto put = [&](int eight, float2 x) {         // group of 8 channels -> (step, register) of this lane
+                  uint8_t* to = s_turned + (n * steps + (eight >> 1)) * 256 + lane * 8 + (eight & 1) * 4;
+                  const uint32_t hi = pack<FP4>(x.x, x.y);
+                  *reinterpret_cast<uint32_t*>(to) = hi;
+                  if constexpr (!FP4) {
+                    const float2 f = unpack<FP4>(hi);
+                    *reinterpret_cast<uint32_t*>(to + slot_low) = pack<FP4>(isfinite(x.x) ? x.x - f.x : 0.f, isfinite(x.y) ? x.y - f.y : 0.f);
                   }
-                }
+                };
+                put(i, a);
+                put(steps + i, z);
+              }
             }
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
+            for (int mt = 0; mt < MT; ++mt) {
+              float acc[NT][4];
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const int qi = ((n * (HD / 16) + hs * 4 + ks) * 32 + lane) * 8;
-                const uint2 q1 = *reinterpret_cast<const uint2*>(qs + qi);
+              for (int hs = 0; hs < H; ++hs) {
+                uint32_t x[2][4][2];           // [row][block of the slice][channels 2 t.. or 2 t + 8 ..]
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                  const uint32_t a[4] = {x[mt][0][2 * ks], x[mt][1][2 * ks], x[mt][0][2 * ks + 1], x[mt][1][2 * ks + 1]};
-                  mma<FP4>(acc[mt][n], a, q1.x, q1.y);
-                }
-                if constexpr (!FP4) {
-                  const uint2 q2 = *reinterpret_cast<const uint2*>(qs + GEO::QB + qi);
+                for (int e = 0; e < 2; ++e) {
+                  const int pos = mt * 16 + e * 8 + place<FP4>(g);
+                  if constexpr (FP4) {
+                    const uint32_t scw = *reinterpret_cast<const uint32_t*>(st + 2 * GEO::KB + pos * GEO::S + hs * 4);
+                    const uint32_t sc[2] = {scales_to_f16(scw & 0xffffu), scales_to_f16(scw >> 16)};
 #pragma unroll
-                  for (int mt = 0; mt < MT; ++mt) {
-                    const uint32_t a[4] = {x[mt][0][2 * ks], x[mt][1][2 * ks], x[mt][0][2 * ks + 1], x[mt][1][2 * ks + 1]};
-                    mma<FP4>(acc[mt][n], a, q2.x, q2.y);
+                    for (int bl = 0; bl < 4; ++bl) {
+                      const uint2 w = *reinterpret_cast<const uint2*>(st + pos * GEO::ROW + hs * 32 + bl * 8);
+                      const uint32_t two = prmt(w.x, w.y, t | ((t + 4) << 4));
+                      const uint32_t sb = prmt(sc[bl >> 1], 0u, bl & 1 ? 0x3232 : 0x1010);
+                      code_to_f16(two, x[e][bl][0]);
+                      code_to_f16(two >> 8, x[e][bl][1]);
+                      x[e][bl][0] = hmul2(x[e][bl][0], sb);
+                      x[e][bl][1] = hmul2(x[e][bl][1], sb);
+                    }
+                  } else {
+#pragma unroll
+                    for (int bl = 0; bl < 4; ++bl)
+#pragma unroll
+                      for (int c = 0; c < 2; ++c)
+                        x[e][bl][c] = *reinterpret_cast<const uint32_t*>(st + hs * (TILE * 128) + pos * 128 + (((2 * bl + c) ^ (pos & 7)) << 4) + t * 4);
+                  }
+                  if (hs == 0) {
+                    const float4* tr = s_turn + max(0, first + pos - t0) * (half >> 1) + t;
+                    auto turn = [&](uint32_t& a, uint32_t& bb, int i) {          // pair channels i + 2 t .. of the first half
+                      const float4 cs = tr[i >> 1];
+                      const float2 u = unpack<FP4>(a), v = unpack<FP4>(bb);
+                      a = pack<FP4>(u.x * cs.x - v.x * cs.z, u.y * cs.y - v.y * cs.w);
+                      bb = pack<FP4>(v.x * cs.x + u.x * cs.z, v.y * cs.y + u.y * cs.w);
+                    };
+                    if (half == 8) turn(x[e][0][0], x[e][0][1], 0);
+                    else if (half == 16) { turn(x[e][0][0], x[e][1][0], 0); turn(x[e][0][1], x[e][1][1], 8); }
+                    else { turn(x[e][0][0], x[e][2][0], 0); turn(x[e][0][1], x[e][2][1], 8); turn(x[e][1][0], x[e][3][0], 16); turn(x[e][1][1], x[e][3][1], 24); }
                   }
                 }
-              }
-          }
-        };
-        if (near_any) score(p.a.cap != 0, sq, s);
-        if (far_any) {
-          const uint8_t* qf = sq + GEO::QCOPIES * GEO::QB;
-          if (!near_any) score(false, qf, s);
-          else {
-            float sf[MT][NT][4];
-            score(false, qf, sf);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+                for (int bl = 0; bl < 4; ++bl) {
+                  const uint32_t a[4] = {x[0][bl][0], x[1][bl][0], x[0][bl][1], x[1][bl][1]};
+                  const int ks = hs * 4 + bl;
+                  const bool own = hs == 0 && bl < steps;
+                  step(acc, a, own ? s_turned + ks * 256 : sq + GEO::QCOPIES * GEO::QB + ks * 256, own ? steps * 256 : HD * 16, own ? slot_low : GEO::QB, ks == 0);
+                }
+              }
 #pragma unroll
               for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const int tok = first + mt * 16 + (e >> 1) * 8 + place<FP4>(g);
-                  if (prow[n][e & 1] - tok > p.a.cap) s[mt][n][e] = sf[mt][n][e];
+                  if (!far_any || prow[n][e & 1] - tok <= p.a.cap) s[mt][n][e] = acc[n][e];
                 }
+            }
           }
         }
         // ---- masks, where any (row, position) of the tile is not visible
-        const unsigned whole = TILE == 32 ? 0xffffffffu : 0xffffu;
-        const bool masked = (on & whole) != whole || first + TILE - 1 > p_first;
+        if (masked) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[mt][n][e] *= mul[n][e & 1];
-              if (masked) {
+              for (int e = 0; e < 4; ++e) {
                 const int pos = mt * 16 + (e >> 1) * 8 + place<FP4>(g);
-                if (!((on >> pos) & 1) || first + pos > prow[n][e & 1]) s[mt][n][e] = -INFINITY;
+                if (!((on >> (pos >> c_shift)) & 1) || first + pos < row.start || first + pos > prow[n][e & 1]) s[mt][n][e] = -INFINITY;
               }
-            }
-        // ---- running maximum, probabilities
-        uint32_t pk[MT][NT][2];
-        float alpha[NT][2];
+        }
+        // ---- running maximum (of the raw scores: the factor is positive)
+        float mx[NT][2];
         bool grew = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          if (NT > 1 && n >= live_n) continue;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = s[0][n][e];
+            float x = fmaxf(s[0][n][e], s[0][n][e + 2]);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mx = fmaxf(mx, fmaxf(s[mt][n][e], s[mt][n][e + 2]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float mn = fmaxf(m[n][e], mx);
-            const float ref = mn == -INFINITY ? 0.f : mn;
-            alpha[n][e] = exp2_fast(m[n][e] - ref);
-            grew |= mn != m[n][e];
-            m[n][e] = mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const float pr = exp2_fast(s[mt][n][e + 2 * q] - ref + (FP4 ? PSHIFT : 0.f));
-                s[mt][n][e + 2 * q] = pr;
-                if constexpr (FP4) sum += pr;
-              }
-            if constexpr (FP4) l[n][e] = l[n][e] * alpha[n][e] + sum;
-          }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) pk[mt][n][q] = pack<FP4>(s[mt][n][2 * q], s[mt][n][2 * q + 1]);
-        if constexpr (!FP4) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const float2 f = unpack<FP4>(pk[mt][n][q]);
-                s0 += f.x; s1 += f.y;
-                s[mt][n][2 * q] = f.x; s[mt][n][2 * q + 1] = f.y;
-              }
-            l[n][0] = l[n][0] * alpha[n][0] + s0;
-            l[n][1] = l[n][1] * alpha[n][1] + s1;
+            for (int mt = 1; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][n][e], s[mt][n][e + 2]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            mx[n][e] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * mul[n][e];
+            grew |= mx[n][e] > m[n][e];
           }
         }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-          for (int i = 0; i < H * 4; ++i)
+          for (int n = 0; n < NT; ++n) {
+            if (NT > 1 && n >= live_n) continue;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              o[i][n][0] *= alpha[n][0]; o[i][n][1] *= alpha[n][1];
-              o[i][n][2] *= alpha[n][0]; o[i][n][3] *= alpha[n][1];
+            for (int e = 0; e < 2; ++e) {
+              const float mn = fmaxf(m[n][e], mx[n][e]);
+              const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m[n][e] - mn);
+              m[n][e] = mn;
+              l[n][e] *= alpha;
+#pragma unroll
+              for (int i = 0; i < H * 4; ++i) { o[i][n][e] *= alpha; o[i][n][e + 2] *= alpha; }
+            }
+          }
+        }
+        // ---- probabilities
+        uint32_t pk[MT][NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (NT > 1 && n >= live_n) continue;
+          const float r0 = (m[n][0] == -INFINITY ? 0.f : -m[n][0]) + (FP4 ? PSHIFT : 0.f), r1 = (m[n][1] == -INFINITY ? 0.f : -m[n][1]) + (FP4 ? PSHIFT : 0.f);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              float p0 = exp2_fast(fmaf(s[mt][n][2 * q], mul[n][0], r0)), p1 = exp2_fast(fmaf(s[mt][n][2 * q + 1], mul[n][1], r1));
+              pk[mt][n][q] = pack<FP4>(p0, p1);
+              if constexpr (!FP4) { const float2 f = unpack<FP4>(pk[mt][n][q]); p0 = f.x; p1 = f.y; }     // the sum over what is multiplied
+              s[mt][n][2 * q] = p0; s[mt][n][2 * q + 1] = p1;
+              l[n][0] += p0; l[n][1] += p1;
             }
         }
         // ---- O^T += V^T P^T
@@ -593,43 +729,62 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
           for (int mt = 0; mt < MT; ++mt) {
             uint32_t pb[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) { pb[n][0] = transpose8(pk[mt][n][0]); pb[n][1] = transpose8(pk[mt][n][1]); }
+            for (int n = 0; n < NT; ++n) {
+              if (NT > 1 && n >= live_n) continue;
+              pb[n][0] = transpose8(pk[mt][n][0]); pb[n][1] = transpose8(pk[mt][n][1]);
+            }
             const int u0 = mt * 16 + place<FP4>(2 * t), u1 = mt * 16 + place<FP4>(2 * t + 1);
 #pragma unroll
             for (int hs = 0; hs < H; ++hs) {
-              uint32_t v[4][4];                    // [position u0, u1, u0 + 8, u1 + 8][channel pair 8 g + 2 i]
+              uint32_t a4[4][4];                   // [channel 8 g + 2 i of the slice][operand register]
               uint32_t sc[2];
               if constexpr (FP4) {
-                const uint8_t* vb = st + GEO::KB + hs * (TILE * 32) + g * 4;
-                codes_to_f16(*reinterpret_cast<const uint32_t*>(vb + u0 * 32), v[0]);
-                codes_to_f16(*reinterpret_cast<const uint32_t*>(vb + u1 * 32), v[1]);
-                codes_to_f16(*reinterpret_cast<const uint32_t*>(vb + (u0 + 8) * 32), v[2]);
-                codes_to_f16(*reinterpret_cast<const uint32_t*>(vb + (u1 + 8) * 32), v[3]);
+                // the codes of positions u0, u1 side by side in a byte, even channels and odd ones: one conversion gives the pair
+                const uint8_t* vb = st + GEO::KB + hs * 32 + g * 4;
+                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vb + u0 * GEO::ROW), w1 = *reinterpret_cast<const uint32_t*>(vb + u1 * GEO::ROW);
+                const uint32_t w2 = *reinterpret_cast<const uint32_t*>(vb + (u0 + 8) * GEO::ROW), w3 = *reinterpret_cast<const uint32_t*>(vb + (u1 + 8) * GEO::ROW);
+                uint32_t c0[4], c1[4], c2[4], c3[4];
+                codes_to_f16((w0 & 0x0f0f0f0fu) | ((w1 << 4) & 0xf0f0f0f0u), c0);
+                codes_to_f16(((w0 >> 4) & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u), c1);
+                codes_to_f16((w2 & 0x0f0f0f0fu) | ((w3 << 4) & 0xf0f0f0f0u), c2);
+                codes_to_f16(((w2 >> 4) & 0x0f0f0f0fu) | (w3 & 0xf0f0f0f0u), c3);
                 const uint8_t* sb = st + 2 * GEO::KB + GEO::SB + hs * 4 + (g >> 1);
-                constexpr int S = HD / 16;
+                constexpr int S = GEO::S;
                 sc[0] = scales_to_f16(static_cast<uint32_t>(sb[u0 * S]) | (static_cast<uint32_t>(sb[u1 * S]) << 8));
                 sc[1] = scales_to_f16(static_cast<uint32_t>(sb[(u0 + 8) * S]) | (static_cast<uint32_t>(sb[(u1 + 8) * S]) << 8));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { a4[i][0] = hmul2(c0[i], sc[0]); a4[i][1] = hmul2(c1[i], sc[0]); a4[i][2] = hmul2(c2[i], sc[1]); a4[i][3] = hmul2(c3[i], sc[1]); }
               } else {
                 const uint8_t* vb = st + GEO::KB + hs * (TILE * 128);
+                uint32_t v[4][4];                  // [position u0, u1, u0 + 8, u1 + 8][channel pair 8 g + 2 i]
                 const int us[4] = {u0, u1, u0 + 8, u1 + 8};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                   const uint4 w = *reinterpret_cast<const uint4*>(vb + us[c] * 128 + ((g ^ (us[c] & 7)) << 4));
                   v[c][0] = w.x; v[c][1] = w.y; v[c][2] = w.z; v[c][3] = w.w;
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  a4[i][0] = prmt(v[0][i], v[1][i], 0x5410); a4[i][1] = prmt(v[0][i], v[1][i], 0x7632);
+                  a4[i][2] = prmt(v[2][i], v[3][i], 0x5410); a4[i][3] = prmt(v[2][i], v[3][i], 0x7632);
+                }
               }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t a[4] = {prmt(v[0][i], v[1][i], 0x5410), prmt(v[0][i], v[1][i], 0x7632), prmt(v[2][i], v[3][i], 0x5410), prmt(v[2][i], v[3][i], 0x7632)};
-                if constexpr (FP4) { a[0] = hmul2(a[0], sc[0]); a[1] = hmul2(a[1], sc[0]); a[2] = hmul2(a[2], sc[1]); a[3] = hmul2(a[3], sc[1]); }
+              for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma<FP4>(o[hs * 4 + i][n], a, pb[n][0], pb[n][1]);
-              }
+                for (int n = 0; n < NT; ++n) {
+                  if (NT > 1 && n >= live_n) continue;
+                  mma<FP4>(o[hs * 4 + i][n], a4[i], pb[n][0], pb[n][1]);
+                }
             }
           }
         }
       }
-      __syncwarp();          // the stage is consumed before the next issue refills it
+      __syncwarp();          // the stage is consumed before it is refilled
+      if constexpr (FP4) {
+        if (lane == 0) sm100::mbar_arrive(&s_free[warp][stage]);
+        if (++stage == ST) { stage = 0; phase ^= 1u; }
+      }
     }
     cp_wait<0>();
     __syncthreads();         // every warp is done with its ring: the region takes the partial outputs
@@ -640,6 +795,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        if (warp == W) continue;
         float sum = l[n][e];
         sum += __shfl_xor_sync(0xffffffffu, sum, 4);
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
@@ -678,18 +834,19 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
         if (c == 0) { wo[UR * HD + 2 * r] = mm; wo[UR * HD + 2 * r + 1] = ll; }
       }
     }
-    if (tid == 0 && !(begins && ends)) {
-      int* mt = meta + slot * 4;
-      mt[1] = h; mt[2] = r0; mt[3] = ends ? 1 : 0;
-      mt[0] = b;
+    if (tid == 0 && begins && !ends) {           // the first part: how many CTAs hold the others follows from the shares
+      const long last = at + wk.pieces - 1;      // the unit's last piece
+      meta[1] = h; meta[2] = r0; meta[3] = n_rows; meta[4] = row.q0;
+      meta[0] = static_cast<int>(((last + 1) * use - 1) / total) - cta + 1;
     }
     at += n_pieces;
+    if (FP4) sm100::fence_proxy_async();       // the partial outputs' region takes bulk copies again
     __syncthreads();
   }
 }
 
-// Joins the parts of every unit that CTA borders cut: part one is the last thing its first CTA did (slot 1), the others the first
-// thing the following CTAs did (slot 0). Block (i, r) joins query row r of the unit whose first part CTA i holds. Also the zeros of
+// Joins the parts of every unit that CTA borders cut: part one is the last thing its first CTA did (slot 1), the others are the
+// first thing that the following CTAs did (slot 0). Block (i, r) joins query row r of the unit whose first part CTA i holds. Also the zeros of
 // the packed tokens behind the last row, where the output is this call's own.
 template <int HD, int UR>
 __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_constant__ AttnK p, int n_ctas) {
@@ -705,19 +862,10 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_
       for (long x = (static_cast<long>(i) * gridDim.y + r) * blockDim.x + tid; x < n; x += static_cast<long>(gridDim.x) * gridDim.y * blockDim.x) o[x] = make_uint4(0, 0, 0, 0);
     }
   }
-  const int* head = p.meta + i * 8 + 4;
-  if (head[0] < 0) return;
-  const int b = head[0], h = head[1], r0 = head[2];
-  const Row row = load_row(p.r, b);
-  const int rr = r0 + r;
-  if (rr >= row.nq * p.G) return;
-  int parts = 1;
-  if (head[3] == 0)
-    while (i + parts < n_ctas && p.meta[(i + parts) * 8] >= 0) {
-      const bool end = p.meta[(i + parts) * 8 + 3] != 0;
-      ++parts;
-      if (end) break;
-    }
+  const int* head = p.meta + i * 8;
+  const int parts = head[0];
+  if (parts == 0 || r >= head[3]) return;
+  const int h = head[1], rr = head[2] + r, q0 = head[4];
   auto part = [&](int k) -> const float* { return p.ws + (static_cast<long>(i + k) * 2 + (k == 0 ? 1 : 0)) * UR * (HD + 2); };
   const int grp = tid / LANES, ln = tid % LANES;
   float m = -INFINITY, l = 0.f;
@@ -751,20 +899,25 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_
   }
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
   const __nv_bfloat162 a = __floats2bfloat162_rn(o.x * inv, o.y * inv), c = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.a.out) + ((static_cast<long>(row.q0) + rr / p.G) * p.a.Hq + h * p.G + rr % p.G) * HD + ln * 4;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.a.out) + ((static_cast<long>(q0) + rr / p.G) * p.a.Hq + h * p.G + rr % p.G) * HD + ln * 4;
   *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
 }
 
 namespace {
 
-template <bool FP4, int HD, int NT>
+template <bool FP4, int HD, int NT, bool CAP>
 int launch(const AttnK& k, int ctas, cudaStream_t st) {
   using GEO = Geo<FP4, HD, NT>;
+  const int bytes = GEO::smem(CAP ? k.a.half : 0);
   // (set on every call: the attribute belongs to the device that is current, and costs no launch)
-  if (cudaFuncSetAttribute(paged_attention_kernel<FP4, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEO::SMEM) != cudaSuccess) return 4;
-  paged_attention_kernel<FP4, HD, NT><<<ctas, GEO::THREADS, GEO::SMEM, st>>>(k);
+  if (cudaFuncSetAttribute(paged_attention_kernel<FP4, HD, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return 4;
+  paged_attention_kernel<FP4, HD, NT, CAP><<<ctas, GEO::THREADS, bytes, st>>>(k);
   paged_attention_join_kernel<HD, GEO::UR><<<dim3(ctas, GEO::UR), 256, 0, st>>>(k, ctas);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+template <bool FP4, int HD, int NT>
+int launch(const AttnK& k, int ctas, cudaStream_t st) {
+  return k.a.cap ? launch<FP4, HD, NT, true>(k, ctas, st) : launch<FP4, HD, NT, false>(k, ctas, st);
 }
 
 struct Shape { int ctas, ur, piece; };
@@ -772,7 +925,7 @@ template <bool FP4, int HD, int NT> Shape shape() { using GEO = Geo<FP4, HD, NT>
 
 template <bool FP4>
 bool shape_of(int hd, int nt, Shape* s) {
-  if (hd == 64) { *s = nt == 1 ? shape<FP4, 64, 1>() : nt == 2 ? shape<FP4, 64, 2>() : shape<FP4, 64, 4>(); return true; }
+  if (hd == 64) { *s = nt == 1 ? shape<FP4, 64, 1>() : shape<FP4, 64, 3>(); return nt == 1 || nt == 3; }
   if (hd == 128) { *s = nt == 1 ? shape<FP4, 128, 1>() : shape<FP4, 128, 2>(); return nt <= 2; }
   if (hd == 256) { *s = nt == 1 ? shape<FP4, 256, 1>() : shape<FP4, 256, 2>(); return nt <= 2; }
   return false;
@@ -782,8 +935,7 @@ template <bool FP4>
 int dispatch(const AttnK& k, int hd, const PagedAttnPlan& plan, cudaStream_t st) {
   switch (hd * 8 + plan.nt) {
     case 64 * 8 + 1: return launch<FP4, 64, 1>(k, plan.ctas, st);
-    case 64 * 8 + 2: return launch<FP4, 64, 2>(k, plan.ctas, st);
-    case 64 * 8 + 4: return launch<FP4, 64, 4>(k, plan.ctas, st);
+    case 64 * 8 + 3: return launch<FP4, 64, 3>(k, plan.ctas, st);
     case 128 * 8 + 1: return launch<FP4, 128, 1>(k, plan.ctas, st);
     case 128 * 8 + 2: return launch<FP4, 128, 2>(k, plan.ctas, st);
     case 256 * 8 + 1: return launch<FP4, 256, 1>(k, plan.ctas, st);
@@ -794,14 +946,13 @@ int dispatch(const AttnK& k, int hd, const PagedAttnPlan& plan, cudaStream_t st)
 
 }  // namespace
 
-// How many query rows a unit has (8, 16 or 32: the smallest that holds a row's average, so that cached entries are read once)
-// and how many CTAs run: as many as are resident, fewer where even full tables have fewer pieces.
+// How many query rows a unit has: 8 where that holds the rows' average (a decode step), else 24 (16 for wide heads), of which
+// only the blocks of 8 in use are computed; and how many CTAs run: as many as are resident, fewer where even full
+// tables have fewer pieces.
 int paged_attention_plan(const PagedRows& r, const PagedPool& c, int Hq, int sms, PagedAttnPlan* plan) {
   const int G = Hq / r.Hkv;
   const long per_row = r.B ? static_cast<long>(G) * ((r.n + r.B - 1) / r.B) : 0;
-  const int most = c.hd == 64 ? 4 : 2;
-  int nt = 1;
-  while (nt < most && 8 * nt < per_row) nt *= 2;
+  const int nt = per_row <= 8 ? 1 : c.hd == 64 ? 3 : 2;
   Shape s;
   if (!(c.fp4 ? shape_of<true>(c.hd, nt, &s) : shape_of<false>(c.hd, nt, &s))) return 1;
   const long units = (static_cast<long>(r.n) * G / s.ur + r.B) * r.Hkv;

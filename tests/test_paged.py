@@ -435,6 +435,19 @@ def test_attention_kernels(fmt, hd, group, rot, cap, page, qdt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "fp4"])
+@pytest.mark.parametrize("hd,group,rot", [(64, 6, 16), (64, 7, 64), (128, 4, 32), (128, 3, 64), (256, 4, 64), (256, 3, 16)])
+@pytest.mark.parametrize("cap", [None, 25])
+def test_attention_kernels_many_query_rows(fmt, hd, group, rot, cap):
+    """More query rows than one block of 8: several blocks, partly used ones, several units, rows with different counts."""
+    rows, page = [(30, 9, 0), (100, 1, 70), (64, 2, 0), (0, 4, 1), (3, 14, 0)], 8
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    cache, cpu = _random_cache(n_pages, page, 2, hd, fmt)
+    q = torch.randn(n, 2 * group, hd).bfloat16()
+    _check_attention(q, cache, cpu, rows, pages, q_start, lens, start, _tables(110, rot // 2), cap, page=page)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt,hd,new", [("fp4", 64, 1), ("fp4", 128, 3), ("bf16", 64, 2), ("bf16", 256, 1), ("fp4", 256, 9)])
 def test_attention_kernels_long_rows(fmt, hd, new):
     """Rows long enough to be cut over many CTAs and joined; one of them short, so that borders fall inside units."""
