@@ -18,7 +18,7 @@
 
 namespace ghb {
 
-enum PagedStatus { ST_Q_START = 301, ST_LENS = 302, ST_START = 303, ST_PAGE = 304, ST_ROPE = 305, ST_DRAFTS = 306, ST_TOKEN = 307, ST_WAIT = 310 };
+enum PagedStatus { ST_Q_START = 301, ST_LENS = 302, ST_START = 303, ST_PAGE = 304, ST_ROPE = 305, ST_DRAFTS = 306, ST_TOKEN = 307 };
 
 struct Row { int q0, nq, len, start; };
 

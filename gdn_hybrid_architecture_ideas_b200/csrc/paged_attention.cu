@@ -22,13 +22,12 @@
 // the end of a unit's part. A unit cut by CTA borders leaves partial results (at most two a CTA), joined by a second kernel in
 // the order of the CTAs: no atomics, the same result every time.
 //
-// Loads go into a ring of tiles private to each warp (no block barrier in the loop). 4 bits: one more warp loads for all the others
-// (addresses cost as much as the arithmetic of a tile when every warp forms its own: 418 against NNN instructions for 32
-// positions), one bulk copy for the part of a tile that lies in one page, counted on an mbarrier of the stage (waits are
-// bounded); what no row sees gets scales of zero, so that its values are zero. bfloat16: cp.async, 16 bytes a lane, positions that are not visible filled
-// with zeros.
+// Loads go by cp.async into a ring of tiles private to each warp: no block barrier in the loop, and no warp waits for another. The
+// part of a tile that lies in one page is contiguous, so with pages of a tile or more the addresses are one base and constants.
+// (Bulk copies cost one instruction instead of nine, but about 32 clocks each in the SM's copy engine, which bound
+// the loop; one more warp that loads for all the others ties them to the slowest. Both were measured slower.) What no
+// row sees gets scales of zero (4 bits), so that its values are zero.
 #include "paged.cuh"
-#include "sm100.cuh"
 
 namespace ghb {
 
@@ -38,15 +37,14 @@ struct AttnK {                       // by value to the kernels
   float* ws; int* meta;
 };
 
-// W warps that compute, ST ring stages each, CTAS a SM, MT 16-position tiles a warp takes at once. With the loading warp the
-// block has a multiple of four warps, which is how registers are shared out; blocks of more query rows need more of them, so
-// fewer warps.
+// W warps, ST ring stages each, CTAS a SM, MT 16-position tiles a warp takes at once. Blocks of more query rows need more
+// registers, so fewer warps.
 template <bool FP4, int HD, int NT> struct Cfg;
-template <> struct Cfg<true, 64, 1> { static constexpr int W = 7, ST = 3, CTAS = 2, MT = 4; };
-template <> struct Cfg<true, 64, 3> { static constexpr int W = 11, ST = 4, CTAS = 1, MT = 2; };
-template <> struct Cfg<true, 128, 1> { static constexpr int W = 7, ST = 3, CTAS = 2, MT = 2; };
-template <> struct Cfg<true, 128, 2> { static constexpr int W = 11, ST = 3, CTAS = 1, MT = 2; };
-template <int NT> struct Cfg<true, 256, NT> { static constexpr int W = 7, ST = NT == 1 ? 3 : 2, CTAS = 1, MT = 2; };
+template <> struct Cfg<true, 64, 1> { static constexpr int W = 8, ST = 2, CTAS = 2, MT = 4; };
+template <> struct Cfg<true, 64, 3> { static constexpr int W = 12, ST = 4, CTAS = 1, MT = 2; };
+template <> struct Cfg<true, 128, 1> { static constexpr int W = 8, ST = 2, CTAS = 2, MT = 2; };
+template <> struct Cfg<true, 128, 2> { static constexpr int W = 12, ST = 3, CTAS = 1, MT = 2; };
+template <int NT> struct Cfg<true, 256, NT> { static constexpr int W = 8, ST = 2, CTAS = 1, MT = 2; };
 template <> struct Cfg<false, 64, 1> { static constexpr int W = 8, ST = 3, CTAS = 2, MT = 1; };
 template <> struct Cfg<false, 64, 3> { static constexpr int W = 8, ST = 3, CTAS = 1, MT = 1; };
 template <int NT> struct Cfg<false, 128, NT> { static constexpr int W = 4, ST = 3, CTAS = 2, MT = 1; };
@@ -76,16 +74,11 @@ struct Geo : Cfg<FP4, HD, NT> {
   __host__ __device__ static constexpr int smem(int cap_half) {
     return DATA + q_bytes(cap_half > 0) + UR * 2 * cap_half * 4 + TILE * cap_half * 8 + B::W * turned_bytes(cap_half);
   }
-  static constexpr int THREADS = (B::W + (FP4 ? 1 : 0)) * 32;        // 4 bits: one more warp, which loads for the others
+  static constexpr int THREADS = B::W * 32;
 };
 
 constexpr float PSHIFT = 14.f;
 
-// size bytes (a multiple of 16, both addresses on 16-byte boundaries) into this CTA's shared memory, counted on the barrier
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t size, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(size), "r"(sm100::smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
@@ -137,7 +130,7 @@ __device__ __forceinline__ void code_to_f16(uint32_t byte, uint32_t& h) {       
 // two E4M3 scales (bytes 0 and 1) -> an f16 pair
 __device__ __forceinline__ uint32_t scales_to_f16(uint32_t two) {
   uint32_t h;
-  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(h) : "r"(two));
+  asm("{\n\t.reg .b16 c, d;\n\tmov.b32 {c, d}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(h) : "r"(two));
   return h;
 }
 template <bool FP4>
@@ -192,13 +185,11 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
   using GEO = Geo<FP4, HD, NT>;
   constexpr int H = GEO::H, MT = GEO::MT, TILE = GEO::TILE, UR = GEO::UR, W = GEO::W, ST = GEO::ST;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long s_warp[GEO::THREADS / 32];
+  __shared__ long s_warp[W];
   __shared__ long s_at[2];
   __shared__ float s_mul[UR];                 // a query row's factor on its scores: scale * log2(e) * its power of two
   __shared__ float s_m[W][UR], s_l[W][UR];
   __shared__ int s_pos[UR];                   // a query row's position
-  __shared__ uint64_t s_full[W][ST], s_free[W][ST];      // 4 bits: a warp's ring stage is loaded; is consumed
-  __shared__ unsigned s_on[W][ST];                       // the stage's chunks that were read
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const PagedRows& R = p.r;
   const int n_ctas = gridDim.x, cta = blockIdx.x, Hkv = R.Hkv, G = p.G;
@@ -238,14 +229,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
   long row_at = s_at[1];
   __syncthreads();
 
-  if (FP4) {
-    for (int i = tid; i < W * ST; i += GEO::THREADS) { sm100::mbar_init(&s_full[0][0] + i, 1); sm100::mbar_init(&s_free[0][0] + i, 1); }
-    sm100::mbar_fence_init();
-    __syncthreads();
-  }
-  int stage = 0;                              // 4 bits: of the next tile, through all segments (every piece gives every warp one tile)
-  unsigned phase = 0;
-  bool dead = false;                          // a wait gave up: the status word says so, nothing more is waited for
   uint8_t* ring = smem + warp * (ST * GEO::STAGE);
   const uint32_t ring_u = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   uint8_t* sq = smem + GEO::DATA;
@@ -281,95 +264,72 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     const int n_rows = min(UR, row.nq * G - r0);
     const int pos0 = row.len - row.nq;                              // position of the row's first new token
     const int p_first = pos0 + r0 / G, p_last = row.len ? pos0 + (r0 + n_rows - 1) / G : -1;
-    // ---- loads of one tile: positions tile0 + k PIECE .. + TILE. 4 bits: a tile is one or more chunks, each within a page and so
-    // contiguous per head; a lane of the loading warp copies a chunk (keys, values, their scales) in bulk. bfloat16: lane i owns
-    // position i of its warp's tile.
+    // ---- loads of one tile: positions tile0 + k PIECE .. + TILE. A tile is one or more chunks, each within a page and so contiguous
+    // per head (bfloat16: a chunk is one position); lane i knows the page of chunk i, all lanes copy 16 bytes at a time.
     const int tile0 = wk.base + p0 * GEO::PIECE + warp * TILE;
-    const int c_shift = FP4 ? min(R.page_shift, MT == 4 ? 6 : MT == 2 ? 5 : 4) : 0;
-    const int n_chunks = TILE >> c_shift;
-    const unsigned all_on = n_chunks == 32 ? 0xffffffffu : (1u << n_chunks) - 1u;
-    auto page_of = [&](int tok) -> int {       // page id of a chunk or position, -1: not read
-      if (tok + (1 << c_shift) <= row.start || tok > p_last) return -1;
+    const int c_shift = min(R.page_shift, TILE == 64 ? 6 : TILE == 32 ? 5 : 4);
+    const unsigned all_on = (1u << (TILE >> c_shift)) - 1u;
+    auto page_at = [&](int k) -> int {         // page id of this lane's chunk of tile k, -1: not read
+      const int tok = tile0 + k * GEO::PIECE + (lane << c_shift);
+      if (k >= n_pieces || lane >= (TILE >> c_shift) || tok + (1 << c_shift) <= row.start || tok > p_last) return -1;
       const int pg = R.pages[b * R.pages_stride + (tok >> R.page_shift)];
       if (pg < 0 || pg >= R.n_pages) { *R.err = ST_PAGE; return -1; }
       return pg;
     };
-    const int base = wk.base + p0 * GEO::PIECE, n_all = W * n_chunks;               // chunks of a piece, in rounds of 32 lanes
-    int pg = FP4 && warp == W && lane < n_all ? page_of(base + (lane << c_shift)) : -1;
-    auto produce = [&](int k_from, int k_to) {                                      // the loading warp: pieces k_from .. k_to
-      if constexpr (FP4) {
-        const int lo_shift = __ffs(n_chunks) - 1;
-        for (int k = k_from; k < k_to && !dead; ++k) {
-          for (int i0 = 0; i0 < n_all; i0 += 32) {
-            const int i = i0 + lane;
-            const int tok = base + k * GEO::PIECE + (i << c_shift);
-            // the next round's page ids are on their way while this one waits for its stages
-            const bool more = i0 + 32 < n_all;
-            const int i2 = more ? i + 32 : lane, k2 = more ? k : k + 1;
-            const int pg2 = i2 < n_all && k2 < n_pieces ? page_of(base + k2 * GEO::PIECE + (i2 << c_shift)) : -1;
-            const unsigned on = __ballot_sync(0xffffffffu, pg >= 0);
-            const int w = i >> lo_shift;
-            bool ok = true;
-            if (i < n_all && (i & (n_chunks - 1)) == 0) {
-              ok = sm100::mbar_wait(&s_free[w][stage], phase ^ 1u);
-              const unsigned mine = (on >> lane) & all_on;
-              s_on[w][stage] = mine;
-              if (ok) sm100::mbar_expect_tx(&s_full[w][stage], (__popc(mine) << c_shift) * (2 * GEO::ROW + 2 * GEO::S));
-            }
-            if (__any_sync(0xffffffffu, !ok)) { *R.err = ST_WAIT; dead = true; break; }
-            if (pg >= 0) {
-              const int e = ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1));
-              const int at_c = (i & (n_chunks - 1)) << c_shift;
-              const uint32_t st = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (w * ST + stage) * GEO::STAGE;
-              uint64_t* bar = &s_full[w][stage];
-              bulk_load(st + at_c * GEO::ROW, static_cast<const uint8_t*>(p.c.k) + static_cast<long>(e) * GEO::ROW, GEO::ROW << c_shift, bar);
-              bulk_load(st + GEO::KB + at_c * GEO::ROW, static_cast<const uint8_t*>(p.c.v) + static_cast<long>(e) * GEO::ROW, GEO::ROW << c_shift, bar);
-              bulk_load(st + 2 * GEO::KB + at_c * GEO::S, p.c.k_scale + static_cast<long>(e) * GEO::S, GEO::S << c_shift, bar);
-              bulk_load(st + 2 * GEO::KB + GEO::SB + at_c * GEO::S, p.c.v_scale + static_cast<long>(e) * GEO::S, GEO::S << c_shift, bar);
-            }
-            pg = pg2;
-          }
-          if (++stage == ST) { stage = 0; phase ^= 1u; }
-        }
-      }
-    };
-    // (every stage is free at the start of a unit's part: the first ST pieces wait for nobody, so this may stand before the barrier)
-    if (FP4 && warp == W) produce(0, min(ST, n_pieces));
-    auto issue = [&](int k) -> unsigned {      // bfloat16: returns the mask of positions that are read
-      unsigned on = 0;
-      if constexpr (!FP4) {
-        const int tok = tile0 + k * GEO::PIECE + lane;
-        const int pg = k < n_pieces && lane < TILE ? page_of(tok) : -1;
-        on = __ballot_sync(0xffffffffu, pg >= 0);
-        if (on) {
-          const uint32_t st = ring_u + (k % ST) * GEO::STAGE;
-          const int e = pg >= 0 ? ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1)) : 0;
-          const uint8_t* kb = static_cast<const uint8_t*>(p.c.k);
-          const uint8_t* vb = static_cast<const uint8_t*>(p.c.v);
-          constexpr int CH = GEO::ROW / 16;
+    auto issue = [&](int k, int stage, int pg) -> unsigned {      // returns the mask of chunks that are read
+      const unsigned on = __ballot_sync(0xffffffffu, pg >= 0);
+      if (on) {
+        const uint32_t st = ring_u + stage * GEO::STAGE;
+        const int tok = tile0 + k * GEO::PIECE + (lane << c_shift);
+        const int e = pg >= 0 ? ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1)) : 0;
+        const uint8_t* kb = static_cast<const uint8_t*>(p.c.k);
+        const uint8_t* vb = static_cast<const uint8_t*>(p.c.v);
+        constexpr int CH = GEO::ROW / 16, N = TILE * CH / 32;        // 16-byte parts of a position; copies a lane makes of keys
+        auto place_of = [&](int pos, int sub) -> uint32_t {          // bfloat16: slices of 128-byte rows, swizzled
+          if constexpr (FP4) return pos * GEO::ROW + sub * 16;
+          else return (sub >> 3) * (TILE * 128) + pos * 128 + (((sub & 7) ^ (pos & 7)) << 4);
+        };
+        if ((TILE >> c_shift) == 1) {          // the whole tile lies in one page: one address, fixed distances
+          const long off = static_cast<long>(__shfl_sync(0xffffffffu, e, 0)) * GEO::ROW + lane * 16;
 #pragma unroll
-          for (int i = 0; i < TILE * CH / 32; ++i) {
-            const int idx = i * 32 + lane, pos = idx / CH, sub = idx % CH;
-            const int ee = __shfl_sync(0xffffffffu, e, pos);
-            const bool ok = (on >> pos) & 1;
-            const uint32_t dst = (sub >> 3) * (TILE * 128) + pos * 128 + (((sub & 7) ^ (pos & 7)) << 4);
-            const long off = static_cast<long>(ee) * GEO::ROW + sub * 16;
-            cp16(st + dst, kb + off, ok);
-            cp16(st + GEO::KB + dst, vb + off, ok);
+          for (int i = 0; i < N; ++i) {
+            const uint32_t dst = st + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH);
+            cp16(dst, kb + off + i * 512, true);
+            cp16(dst + GEO::KB, vb + off + i * 512, true);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const int pos = (i * 32 + lane) / CH, sub = (i * 32 + lane) % CH, c = pos >> c_shift;
+            const long off = static_cast<long>(__shfl_sync(0xffffffffu, e, c) + (pos & ((1 << c_shift) - 1))) * GEO::ROW + sub * 16;
+            const bool ok = (on >> c) & 1;
+            const uint32_t dst = st + place_of(pos, sub);
+            cp16(dst, kb + off, ok);
+            cp16(dst + GEO::KB, vb + off, ok);
           }
         }
-        cp_commit();
+        if constexpr (FP4) {                   // scales: TILE S bytes of keys, as many of values
+          constexpr int L = TILE * GEO::S / 16;
+#pragma unroll
+          for (int i = 0; i < (2 * L + 31) / 32; ++i) {
+            const int idx = i * 32 + lane, pos = (idx % L) * (16 / GEO::S), c = pos >> c_shift;
+            const uint8_t* base = idx < L ? p.c.k_scale : p.c.v_scale;
+            const long off = static_cast<long>(__shfl_sync(0xffffffffu, e, c) + (pos & ((1 << c_shift) - 1))) * GEO::S;
+            if (2 * L >= 32 || idx < 2 * L) cp16(st + 2 * GEO::KB + idx * 16, base + off, (on >> c) & 1);
+          }
+        }
       }
+      cp_commit();
       return on;
     };
     unsigned on_ring[ST];
-    if constexpr (!FP4) {
 #pragma unroll
-      for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k);
-    }
+    for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k, k, page_at(k));
+    int pg_next = page_at(ST - 1);
+    int stage = 0;                             // of tile k
 
     // ---- the unit's queries: rotated (near at their positions, far by the cap), brought to about one, in the MMA's order
-    for (int r = warp; r < UR && warp < W; r += W) {
+    for (int r = warp; r < UR; r += W) {
       const bool live = r < n_rows && row.len > 0;
       const int rr = r0 + r;
       const long tok = row.q0 + (live ? rr / G : 0);
@@ -447,26 +407,18 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
 
-    if (FP4 && warp == W) produce(ST, n_pieces);
-    for (int k = 0; k < n_pieces && warp < W; ++k) {
+    for (int k = 0; k < n_pieces; ++k) {
       const int first = tile0 + k * GEO::PIECE;
-      unsigned on;
-      uint8_t* st;
-      if constexpr (FP4) {
-        if (!dead && !sm100::mbar_wait(&s_full[warp][stage], phase)) { *R.err = ST_WAIT; dead = true; }
-        dead = __any_sync(0xffffffffu, dead);
-        on = s_on[warp][stage];
-        st = ring + stage * GEO::STAGE;
-      } else {
-        on_ring[ST - 1] = issue(k + ST - 1);
-        on = on_ring[0];
+      on_ring[ST - 1] = issue(k + ST - 1, stage == 0 ? ST - 1 : stage - 1, pg_next);
+      pg_next = page_at(k + ST);
+      const unsigned on = on_ring[0];
 #pragma unroll
-        for (int i = 0; i < ST - 1; ++i) on_ring[i] = on_ring[i + 1];        // the masks travel with the ring
-        cp_wait<ST - 1>();
-        __syncwarp();
-        st = ring + (k % ST) * GEO::STAGE;
-      }
-      if (on && !dead) {
+      for (int i = 0; i < ST - 1; ++i) on_ring[i] = on_ring[i + 1];        // the masks travel with the ring
+      uint8_t* st = ring + stage * GEO::STAGE;
+      cp_wait<ST - 1>();
+      __syncwarp();
+      stage = stage == ST - 1 ? 0 : stage + 1;
+      if (on) {
         const bool masked = on != all_on || first < row.start || first + TILE - 1 > p_first;
         if (FP4 && masked) {
           // what no row sees may hold anything: its scales become zero, so that its values are zero
@@ -476,7 +428,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
               for (int i = 0; i < GEO::S / 4; ++i) *reinterpret_cast<uint32_t*>(st + 2 * GEO::KB + GEO::SB + pos * GEO::S + 4 * i) = 0u;
             }
           }
-          sm100::fence_proxy_async();        // before a later bulk copy into the stage
           __syncwarp();
         }
         float s[MT][NT][4];
@@ -702,12 +653,12 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
           }
           if (!plain) {
             for (int j = 0; j < TILE; ++j) {
-              if (!((on >> j) & 1)) continue;
+              if (!((on >> (j >> c_shift)) & 1)) continue;
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 const float p0 = __shfl_sync(0xffffffffu, j < 8 ? s[0][n][0] : s[0][n][2], (j & 7) * 4 + t);
                 const float p1 = __shfl_sync(0xffffffffu, j < 8 ? s[0][n][1] : s[0][n][3], (j & 7) * 4 + t);
-                const bool see0 = first + j <= prow[n][0], see1 = first + j <= prow[n][1];
+                const bool in = first + j >= row.start, see0 = in && first + j <= prow[n][0], see1 = in && first + j <= prow[n][1];
 #pragma unroll
                 for (int hs = 0; hs < H; ++hs) {
                   const uint4 w = *reinterpret_cast<const uint4*>(st + GEO::KB + hs * (TILE * 128) + j * 128 + ((g ^ (j & 7)) << 4));
@@ -748,10 +699,11 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
                 codes_to_f16(((w0 >> 4) & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u), c1);
                 codes_to_f16((w2 & 0x0f0f0f0fu) | ((w3 << 4) & 0xf0f0f0f0u), c2);
                 codes_to_f16(((w2 >> 4) & 0x0f0f0f0fu) | (w3 & 0xf0f0f0f0u), c3);
-                const uint8_t* sb = st + 2 * GEO::KB + GEO::SB + hs * 4 + (g >> 1);
-                constexpr int S = GEO::S;
-                sc[0] = scales_to_f16(static_cast<uint32_t>(sb[u0 * S]) | (static_cast<uint32_t>(sb[u1 * S]) << 8));
-                sc[1] = scales_to_f16(static_cast<uint32_t>(sb[(u0 + 8) * S]) | (static_cast<uint32_t>(sb[(u1 + 8) * S]) << 8));
+                const uint8_t* sb = st + 2 * GEO::KB + GEO::SB + hs * 4;
+                auto scale_of = [&](int u) { return *reinterpret_cast<const uint32_t*>(sb + u * GEO::S); };
+                const uint32_t pick = (g >> 1) | ((4 + (g >> 1)) << 4);            // this lane's block of both
+                sc[0] = scales_to_f16(prmt(scale_of(u0), scale_of(u1), pick));
+                sc[1] = scales_to_f16(prmt(scale_of(u0 + 8), scale_of(u1 + 8), pick));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) { a4[i][0] = hmul2(c0[i], sc[0]); a4[i][1] = hmul2(c1[i], sc[0]); a4[i][2] = hmul2(c2[i], sc[1]); a4[i][3] = hmul2(c3[i], sc[1]); }
               } else {
@@ -780,11 +732,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
           }
         }
       }
-      __syncwarp();          // the stage is consumed before it is refilled
-      if constexpr (FP4) {
-        if (lane == 0) sm100::mbar_arrive(&s_free[warp][stage]);
-        if (++stage == ST) { stage = 0; phase ^= 1u; }
-      }
+      __syncwarp();          // the stage is consumed before the next issue refills it
     }
     cp_wait<0>();
     __syncthreads();         // every warp is done with its ring: the region takes the partial outputs
@@ -795,7 +743,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if (warp == W) continue;
         float sum = l[n][e];
         sum += __shfl_xor_sync(0xffffffffu, sum, 4);
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
@@ -840,7 +787,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       meta[0] = static_cast<int>(((last + 1) * use - 1) / total) - cta + 1;
     }
     at += n_pieces;
-    if (FP4) sm100::fence_proxy_async();       // the partial outputs' region takes bulk copies again
     __syncthreads();
   }
 }
