@@ -77,11 +77,17 @@ struct Geo : Cfg<FP4, HD, NT> {
   static constexpr int THREADS = B::W * 32;
 };
 
-constexpr float PSHIFT = 14.f;
+// Probabilities are exp2(score - reference + PSHIFT): the reference trails the running maximum by at most SLACK, so that it moves (and
+// the sums are rescaled, and lanes exchange their maxima) only now and then. f16: up to 2^15, and normal down to 2^-21 of the
+// reference; what a smaller one loses is at most 2^-32 of the reference's weight.
+constexpr float PSHIFT = 7.f, SLACK = 8.f;
+// A condition that is rarely true, kept a branch (as predicated instructions its body would cost every tile).
+__device__ __forceinline__ int opaque(int x) { asm volatile("" : "+r"(x)); return x; }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -269,53 +275,73 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     const int tile0 = wk.base + p0 * GEO::PIECE + warp * TILE;
     const int c_shift = min(R.page_shift, TILE == 64 ? 6 : TILE == 32 ? 5 : 4);
     const unsigned all_on = (1u << (TILE >> c_shift)) - 1u;
-    auto page_at = [&](int k) -> int {         // page id of this lane's chunk of tile k, -1: not read
-      const int tok = tile0 + k * GEO::PIECE + (lane << c_shift);
-      if (k >= n_pieces || lane >= (TILE >> c_shift) || tok + (1 << c_shift) <= row.start || tok > p_last) return -1;
-      const int pg = R.pages[b * R.pages_stride + (tok >> R.page_shift)];
-      if (pg < 0 || pg >= R.n_pages) { *R.err = ST_PAGE; return -1; }
-      return pg;
+    // Page ids are looked up for 32 chunks at a time (32 tiles where a page holds a tile): lane i holds the entry of chunk i of them.
+    const int n_log = TILE == 64 ? 6 - c_shift : TILE == 32 ? 5 - c_shift : 4 - c_shift;          // log2 of a tile's chunks
+    int entry = 0;
+    unsigned batch_on = 0;
+    auto look_up = [&](int k) {                // tiles k .. of this warp
+      const int tok = tile0 + (k + (lane >> n_log)) * GEO::PIECE + ((lane & ((1 << n_log) - 1)) << c_shift);
+      entry = -1;
+      if (k + (lane >> n_log) < n_pieces && tok + (1 << c_shift) > row.start && tok <= p_last) {
+        const int pg = R.pages[b * R.pages_stride + (tok >> R.page_shift)];
+        if (pg < 0 || pg >= R.n_pages) *R.err = ST_PAGE;
+        else entry = ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1));
+      }
+      batch_on = __ballot_sync(0xffffffffu, entry >= 0);
     };
-    auto issue = [&](int k, int stage, int pg) -> unsigned {      // returns the mask of chunks that are read
-      const unsigned on = __ballot_sync(0xffffffffu, pg >= 0);
+    const uint8_t* k_lane = static_cast<const uint8_t*>(p.c.k) + lane * 16;
+    const uint8_t* v_lane = static_cast<const uint8_t*>(p.c.v) + lane * 16;
+    constexpr int L = FP4 ? TILE * GEO::S / 16 : 1;          // 16-byte parts of a tile's key scales; its value scales follow
+    const uint8_t* s_lane = lane % (2 * L) < L ? p.c.k_scale : p.c.v_scale;
+    auto issue = [&](int k, int stage) -> unsigned {         // returns the mask of tile k's chunks that are read
+      if ((k & ((32 >> n_log) - 1)) == 0 && k < n_pieces) look_up(k);
+      const int at_chunk = (k << n_log) & 31;
+      const unsigned on = k < n_pieces ? (batch_on >> at_chunk) & all_on : 0u;
       if (on) {
         const uint32_t st = ring_u + stage * GEO::STAGE;
-        const int tok = tile0 + k * GEO::PIECE + (lane << c_shift);
-        const int e = pg >= 0 ? ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1)) : 0;
-        const uint8_t* kb = static_cast<const uint8_t*>(p.c.k);
-        const uint8_t* vb = static_cast<const uint8_t*>(p.c.v);
         constexpr int CH = GEO::ROW / 16, N = TILE * CH / 32;        // 16-byte parts of a position; copies a lane makes of keys
         auto place_of = [&](int pos, int sub) -> uint32_t {          // bfloat16: slices of 128-byte rows, swizzled
           if constexpr (FP4) return pos * GEO::ROW + sub * 16;
           else return (sub >> 3) * (TILE * 128) + pos * 128 + (((sub & 7) ^ (pos & 7)) << 4);
         };
-        if ((TILE >> c_shift) == 1) {          // the whole tile lies in one page: one address, fixed distances
-          const long off = static_cast<long>(__shfl_sync(0xffffffffu, e, 0)) * GEO::ROW + lane * 16;
+        if (n_log == 0) {                      // the whole tile lies in one page: one address, fixed distances
+          const int e = __shfl_sync(0xffffffffu, entry, at_chunk);
+          const long off = static_cast<long>(e) * GEO::ROW;
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             const uint32_t dst = st + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH);
-            cp16(dst, kb + off + i * 512, true);
-            cp16(dst + GEO::KB, vb + off + i * 512, true);
+            cp16(dst, k_lane + off + i * 512);
+            cp16(dst + GEO::KB, v_lane + off + i * 512);
+          }
+          if constexpr (FP4) {
+            const long soff = static_cast<long>(e) * GEO::S + (lane % L) * 16;
+            if constexpr (2 * L > 32) {        // (wide heads: one copy for the keys', one for the values')
+              cp16(st + 2 * GEO::KB + lane * 16, p.c.k_scale + soff);
+              cp16(st + 2 * GEO::KB + GEO::SB + lane * 16, p.c.v_scale + soff);
+            } else if (2 * L == 32 || lane < 2 * L) {
+              cp16(st + 2 * GEO::KB + lane * 16, s_lane + soff);
+            }
           }
         } else {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             const int pos = (i * 32 + lane) / CH, sub = (i * 32 + lane) % CH, c = pos >> c_shift;
-            const long off = static_cast<long>(__shfl_sync(0xffffffffu, e, c) + (pos & ((1 << c_shift) - 1))) * GEO::ROW + sub * 16;
+            const int e = __shfl_sync(0xffffffffu, entry, at_chunk + c) + (pos & ((1 << c_shift) - 1));
+            const long off = static_cast<long>(e) * GEO::ROW + sub * 16;
             const bool ok = (on >> c) & 1;
             const uint32_t dst = st + place_of(pos, sub);
-            cp16(dst, kb + off, ok);
-            cp16(dst + GEO::KB, vb + off, ok);
+            cp16(dst, static_cast<const uint8_t*>(p.c.k) + (ok ? off : 0), ok);
+            cp16(dst + GEO::KB, static_cast<const uint8_t*>(p.c.v) + (ok ? off : 0), ok);
           }
-        }
-        if constexpr (FP4) {                   // scales: TILE S bytes of keys, as many of values
-          constexpr int L = TILE * GEO::S / 16;
+          if constexpr (FP4) {
 #pragma unroll
-          for (int i = 0; i < (2 * L + 31) / 32; ++i) {
-            const int idx = i * 32 + lane, pos = (idx % L) * (16 / GEO::S), c = pos >> c_shift;
-            const uint8_t* base = idx < L ? p.c.k_scale : p.c.v_scale;
-            const long off = static_cast<long>(__shfl_sync(0xffffffffu, e, c) + (pos & ((1 << c_shift) - 1))) * GEO::S;
-            if (2 * L >= 32 || idx < 2 * L) cp16(st + 2 * GEO::KB + idx * 16, base + off, (on >> c) & 1);
+            for (int i = 0; i < (2 * L + 31) / 32; ++i) {
+              const int idx = i * 32 + lane, pos = (idx % L) * (16 / GEO::S), c = pos >> c_shift;
+              const int e = __shfl_sync(0xffffffffu, entry, at_chunk + c) + (pos & ((1 << c_shift) - 1));
+              const bool ok = (on >> c) & 1;
+              const uint8_t* base = idx % (2 * L) < L ? p.c.k_scale : p.c.v_scale;
+              if (2 * L >= 32 || idx < 2 * L) cp16(st + 2 * GEO::KB + idx * 16, base + (ok ? static_cast<long>(e) * GEO::S : 0), ok);
+            }
           }
         }
       }
@@ -324,8 +350,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     };
     unsigned on_ring[ST];
 #pragma unroll
-    for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k, k, page_at(k));
-    int pg_next = page_at(ST - 1);
+    for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k, k);
     int stage = 0;                             // of tile k
 
     // ---- the unit's queries: rotated (near at their positions, far by the cap), brought to about one, in the MMA's order
@@ -388,7 +413,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     __syncthreads();
 
     const int live_n = NT == 1 ? 1 : (n_rows + 7) >> 3;        // 8-row column blocks in use
-    float mul[NT][2], m[NT][2], l[NT][2];
+    float mul[NT][2], m[NT][2], l[NT][4];       // l: the sums of the probabilities, as a product with ones (every row the same)
     int prow[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -397,7 +422,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
         const int r = n * 8 + 2 * t + e;
         mul[n][e] = s_mul[r];
         prow[n][e] = r < n_rows && row.len > 0 ? pos0 + (r0 + r) / G : -1;
-        m[n][e] = -INFINITY; l[n][e] = 0.f;
+        m[n][e] = -INFINITY; l[n][e] = l[n][e + 2] = 0.f;
       }
     float o[H * 4][NT][4];
 #pragma unroll
@@ -409,8 +434,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 
     for (int k = 0; k < n_pieces; ++k) {
       const int first = tile0 + k * GEO::PIECE;
-      on_ring[ST - 1] = issue(k + ST - 1, stage == 0 ? ST - 1 : stage - 1, pg_next);
-      pg_next = page_at(k + ST);
+      on_ring[ST - 1] = issue(k + ST - 1, stage == 0 ? ST - 1 : stage - 1);
       const unsigned on = on_ring[0];
 #pragma unroll
       for (int i = 0; i < ST - 1; ++i) on_ring[i] = on_ring[i + 1];        // the masks travel with the ring
@@ -575,7 +599,8 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
           }
         }
         // ---- masks, where any (row, position) of the tile is not visible
-        if (masked) {
+#pragma unroll 1
+        for (int again = opaque(masked); again > 0; again = opaque(0)) {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -586,7 +611,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
                 if (!((on >> (pos >> c_shift)) & 1) || first + pos < row.start || first + pos > prow[n][e & 1]) s[mt][n][e] = -INFINITY;
               }
         }
-        // ---- running maximum (of the raw scores: the factor is positive)
+        // ---- the reference of the exponents, where a score leaves the slack (raw scores: the factor is positive)
         float mx[NT][2];
         bool grew = false;
 #pragma unroll
@@ -597,10 +622,8 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             float x = fmaxf(s[0][n][e], s[0][n][e + 2]);
 #pragma unroll
             for (int mt = 1; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][n][e], s[mt][n][e + 2]));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            mx[n][e] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * mul[n][e];
-            grew |= mx[n][e] > m[n][e];
+            mx[n][e] = x * mul[n][e];
+            grew |= mx[n][e] > m[n][e] + SLACK;
           }
         }
         if (__any_sync(0xffffffffu, grew)) {
@@ -609,10 +632,14 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             if (NT > 1 && n >= live_n) continue;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float mn = fmaxf(m[n][e], mx[n][e]);
+              float x = mx[n][e];
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              const float mn = fmaxf(m[n][e], x);
               const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m[n][e] - mn);
               m[n][e] = mn;
-              l[n][e] *= alpha;
+              l[n][e] *= alpha; l[n][e + 2] *= alpha;
 #pragma unroll
               for (int i = 0; i < H * 4; ++i) { o[i][n][e] *= alpha; o[i][n][e + 2] *= alpha; }
             }
@@ -627,13 +654,8 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              float p0 = exp2_fast(fmaf(s[mt][n][2 * q], mul[n][0], r0)), p1 = exp2_fast(fmaf(s[mt][n][2 * q + 1], mul[n][1], r1));
-              pk[mt][n][q] = pack<FP4>(p0, p1);
-              if constexpr (!FP4) { const float2 f = unpack<FP4>(pk[mt][n][q]); p0 = f.x; p1 = f.y; }     // the sum over what is multiplied
-              s[mt][n][2 * q] = p0; s[mt][n][2 * q + 1] = p1;
-              l[n][0] += p0; l[n][1] += p1;
-            }
+            for (int q = 0; q < 2; ++q)
+              pk[mt][n][q] = pack<FP4>(exp2_fast(fmaf(s[mt][n][2 * q], mul[n][0], r0)), exp2_fast(fmaf(s[mt][n][2 * q + 1], mul[n][1], r1)));
         }
         // ---- O^T += V^T P^T
         bool plain = true;
@@ -652,13 +674,16 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             plain = !__any_sync(0xffffffffu, odd);
           }
           if (!plain) {
+            auto see = [&](int j, int n, int e) { return first + j >= row.start && first + j <= prow[n][e]; };
             for (int j = 0; j < TILE; ++j) {
               if (!((on >> (j >> c_shift)) & 1)) continue;
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                const float p0 = __shfl_sync(0xffffffffu, j < 8 ? s[0][n][0] : s[0][n][2], (j & 7) * 4 + t);
-                const float p1 = __shfl_sync(0xffffffffu, j < 8 ? s[0][n][1] : s[0][n][3], (j & 7) * 4 + t);
-                const bool in = first + j >= row.start, see0 = in && first + j <= prow[n][0], see1 = in && first + j <= prow[n][1];
+                const float2 pp = unpack<FP4>(__shfl_sync(0xffffffffu, j < 8 ? pk[0][n][0] : pk[0][n][1], (j & 7) * 4 + t));
+                const float p0 = pp.x, p1 = pp.y;
+                if (see(j, n, 0)) { l[n][0] += p0; l[n][2] += p0; }
+                if (see(j, n, 1)) { l[n][1] += p1; l[n][3] += p1; }
+                const bool see0 = see(j, n, 0), see1 = see(j, n, 1);
 #pragma unroll
                 for (int hs = 0; hs < H; ++hs) {
                   const uint4 w = *reinterpret_cast<const uint4*>(st + GEO::KB + hs * (TILE * 128) + j * 128 + ((g ^ (j & 7)) << 4));
@@ -683,6 +708,8 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             for (int n = 0; n < NT; ++n) {
               if (NT > 1 && n >= live_n) continue;
               pb[n][0] = transpose8(pk[mt][n][0]); pb[n][1] = transpose8(pk[mt][n][1]);
+              const uint32_t ones[4] = {FP4 ? 0x3c003c00u : 0x3f803f80u, FP4 ? 0x3c003c00u : 0x3f803f80u, FP4 ? 0x3c003c00u : 0x3f803f80u, FP4 ? 0x3c003c00u : 0x3f803f80u};
+              mma<FP4>(l[n], ones, pb[n][0], pb[n][1]);
             }
             const int u0 = mt * 16 + place<FP4>(2 * t), u1 = mt * 16 + place<FP4>(2 * t + 1);
 #pragma unroll
@@ -743,12 +770,8 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float sum = l[n][e];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int r = n * 8 + 2 * t + e;
-        if (g == 0) { s_m[warp][r] = m[n][e]; s_l[warp][r] = sum; }
+        if (g == 0) { s_m[warp][r] = m[n][e]; s_l[warp][r] = l[n][e]; }
         float* dst = so + (static_cast<long>(warp) * UR + r) * HD + 8 * g;
 #pragma unroll
         for (int i = 0; i < H * 4; ++i)
