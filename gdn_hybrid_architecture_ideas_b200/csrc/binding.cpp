@@ -4,6 +4,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
+
 #include "kernels.h"
 
 namespace {
@@ -411,33 +413,46 @@ Tensor whole_heads(const Tensor& t) {
   const bool ok = t.stride(2) == 1 && t.stride(1) % per == 0 && t.stride(0) % per == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   return ok ? t : t.contiguous().clone(at::MemoryFormat::Contiguous);
 }
-ghb::PagedPool pool_of(const Tensor& k, const Tensor& v, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const char* what) {
+// The cache's tensors, checked once; what the calls need of them.
+struct PagedCache {
+  Tensor k, v;
+  c10::optional<Tensor> ks, vs;
+  int hd, heads, n_pages, page_shift;
+  ghb::PagedPool pool() const {
+    return {k.data_ptr(), v.data_ptr(), ks.has_value() ? static_cast<uint8_t*>(ks->data_ptr()) : nullptr, vs.has_value() ? static_cast<uint8_t*>(vs->data_ptr()) : nullptr, hd, ks.has_value()};
+  }
+};
+PagedCache paged_cache(const Tensor& k, const Tensor& v, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs) {
   const bool fp4 = k.scalar_type() == torch::kUInt8;
-  TORCH_CHECK(k.is_cuda() && (fp4 || is_bf16(k)) && k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && k.is_contiguous() && v.is_contiguous(), what,
-              ": the cache on a GPU is bfloat16, or uint8 codes with scales");
-  const int hd = static_cast<int>(k.size(3)) * (fp4 ? 2 : 1);
-  TORCH_CHECK(hd == 64 || hd == 128 || hd == 256, what, ": head dimension ", hd, " (64, 128 or 256 on a GPU)");
-  TORCH_CHECK(fp4 == ks.has_value() && fp4 == vs.has_value(), what, ": 4-bit codes come with scales");
+  TORCH_CHECK_VALUE(k.is_cuda() && k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
+                    "PagedKV: k and v are [pages, kv heads, page size, channels] of one type on one device, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(fp4 || is_bf16(k), "PagedKV: the cache on a GPU is bfloat16, or uint8 codes with scales");
+  TORCH_CHECK_VALUE(k.is_contiguous() && v.is_contiguous(), "PagedKV: k and v are contiguous");
+  const int64_t hd = k.size(3) * (fp4 ? 2 : 1), page = k.size(2);
+  TORCH_CHECK_VALUE(page >= 8 && (page & (page - 1)) == 0, "PagedKV: the page size is a power of two from 8 on, got ", page);
+  TORCH_CHECK_VALUE(hd == 64 || hd == 128 || hd == 256, "PagedKV: head dimension ", hd, " (64, 128 or 256 on a GPU)");
+  TORCH_CHECK_VALUE(fp4 == ks.has_value() && fp4 == vs.has_value(), "PagedKV: uint8 codes, and they alone, come with k_scale and v_scale");
   if (fp4) for (const Tensor* s : {&*ks, &*vs})
-    TORCH_CHECK(s->is_contiguous() && s->element_size() == 1 && s->numel() == k.numel() / 8 && s->device() == k.device() && reinterpret_cast<uintptr_t>(s->data_ptr()) % 16 == 0, what,
-                ": scales of the codes, starting on a 16-byte boundary");
-  TORCH_CHECK(v.device() == k.device(), what, ": one device");
-  for (const Tensor* t : {&k, &v}) TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, what, ": the cache starts on a 16-byte boundary");
-  return {k.data_ptr(), v.data_ptr(), fp4 ? static_cast<uint8_t*>(ks->data_ptr()) : nullptr, fp4 ? static_cast<uint8_t*>(vs->data_ptr()) : nullptr, hd, fp4};
+    TORCH_CHECK_VALUE(s->scalar_type() == torch::kFloat8_e4m3fn && s->is_contiguous() && s->dim() == 4 && s->size(0) == k.size(0) && s->size(1) == k.size(1) && s->size(2) == page &&
+                      s->size(3) == hd / 16 && s->device() == k.device(), "PagedKV: scales are contiguous float8_e4m3fn [pages, kv heads, page size, channels / 16] beside the codes");
+  for (const Tensor* t : {&k, &v, fp4 ? &*ks : &k, fp4 ? &*vs : &v})
+    TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "PagedKV: the tensors start on 16-byte boundaries");
+  TORCH_CHECK_VALUE(k.size(0) <= 0x7fffffff && k.size(1) <= 0x7fffffff && page <= (1 << 30), "PagedKV: sizes");
+  return {k, v, ks, vs, static_cast<int>(hd), static_cast<int>(k.size(1)), static_cast<int>(k.size(0)), __builtin_ctzll(page)};
 }
-ghb::PagedRows rows_of(const Tensor& k, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start, int64_t n, Tensor& err, const char* what) {
+ghb::PagedRows rows_of(const PagedCache& c, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start, int64_t n, Tensor& err, const char* what) {
   TORCH_CHECK(pages.dim() == 2 && q_start.dim() == 1 && lens.dim() == 1 && q_start.numel() == lens.numel() + 1 && pages.size(0) == lens.numel(), what,
               ": pages [B, width], q_start [B + 1], lens [B] of one batch");
-  for (const Tensor* t : {&pages, &q_start, &lens}) TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->device() == k.device(), what, ": pages, q_start and lens are int32 on the cache's device");
+  for (const Tensor* t : {&pages, &q_start, &lens}) TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->device() == c.k.device(), what, ": pages, q_start and lens are int32 on the cache's device");
   TORCH_CHECK((pages.size(1) <= 1 || pages.stride(1) == 1) && q_start.is_contiguous() && lens.is_contiguous(), what, ": tables with unit inner stride");
-  if (start.has_value()) TORCH_CHECK(start->scalar_type() == torch::kInt32 && start->device() == k.device() && start->sizes() == lens.sizes() && start->is_contiguous(), what, ": start int32 [B]");
-  TORCH_CHECK(n <= 0x7fffffff && k.size(0) <= 0x7fffffff && lens.numel() < 0x7fffffff, what, ": sizes");
-  const int64_t page = k.size(2);
-  TORCH_CHECK(page >= 8 && (page & (page - 1)) == 0, what, ": the page size is a power of two from 8 on");
-  TORCH_CHECK(pages.size(1) <= 0x7fffffff / page, what, ": a row's table holds more positions than 32 bits count");
+  if (start.has_value()) TORCH_CHECK(start->scalar_type() == torch::kInt32 && start->device() == c.k.device() && start->sizes() == lens.sizes() && start->is_contiguous(), what, ": start int32 [B]");
+  TORCH_CHECK(n >= 0 && n <= 0x7fffffff && lens.numel() < 0x7fffffff && pages.size(1) <= (0x7fffffffll >> c.page_shift), what, ": a row's table holds more positions than 32 bits count");
   return {pages.data_ptr<int>(), static_cast<long>(pages.stride(0)), static_cast<int>(pages.size(1)), q_start.data_ptr<int>(), lens.data_ptr<int>(),
-          start.has_value() ? start->data_ptr<int>() : nullptr, static_cast<int>(lens.numel()), static_cast<int>(n), static_cast<int>(k.size(1)),
-          static_cast<int>(k.size(0)), __builtin_ctzll(page), err.data_ptr<int>()};
+          start.has_value() ? start->data_ptr<int>() : nullptr, static_cast<int>(lens.numel()), static_cast<int>(n), c.heads, c.n_pages, c.page_shift, err.data_ptr<int>()};
+}
+// These ops have no backward: an input that a gradient would be asked of is refused, not silently cut off.
+void no_grad(const Tensor& t, const char* what) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), what, ": forward only, call it under torch.no_grad() or with detached inputs");
 }
 struct Rope { const float* cos; const float* sin; int half, n_pos; };
 Rope rope_of(const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, int hd, const Tensor& like, const char* what) {
@@ -449,55 +464,64 @@ Rope rope_of(const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin,
   for (const Tensor* t : {&*cos, &*sin}) TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, what, ": rope tables start on a 16-byte boundary");
   return {cos->data_ptr<float>(), sin->data_ptr<float>(), static_cast<int>(half), static_cast<int>(std::min<int64_t>(cos->size(0), 0x7fffffff))};
 }
-void paged_append(Tensor& kc, Tensor& vc, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const Tensor& k_, const Tensor& v_, const Tensor& pages,
-                  const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start, const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, Tensor& err) {
-  const c10::cuda::CUDAGuard guard(kc.device());
-  const ghb::PagedPool pool = pool_of(kc, vc, ks, vs, "paged_append");
-  TORCH_CHECK(k_.dim() == 3 && v_.sizes() == k_.sizes() && k_.size(1) == kc.size(1) && k_.size(2) == pool.hd && k_.device() == kc.device() && v_.device() == kc.device(),
-              "paged_append: k, v [n, ", kc.size(1), ", ", pool.hd, "] on the cache's device, got ", k_.sizes(), " and ", v_.sizes());
+void paged_append(const PagedCache& c, const Tensor& k_, const Tensor& v_, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start,
+                  const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, Tensor& err) {
+  const c10::cuda::CUDAGuard guard(c.k.device());
+  TORCH_CHECK(k_.dim() == 3 && v_.sizes() == k_.sizes() && k_.size(1) == c.heads && k_.size(2) == c.hd && k_.device() == c.k.device() && v_.device() == c.k.device(),
+              "paged_append: k, v [n, ", c.heads, ", ", c.hd, "] on the cache's device, got ", k_.sizes(), " and ", v_.sizes());
   TORCH_CHECK((is_bf16(k_) || is_f32(k_)) && k_.scalar_type() == v_.scalar_type(), "paged_append: k, v bfloat16 or float32");
-  const ghb::PagedRows r = rows_of(kc, pages, q_start, lens, start, k_.size(0), err, "paged_append");
-  const Rope rope = rope_of(cos, sin, pool.hd, kc, "paged_append");
+  no_grad(k_, "paged_append"); no_grad(v_, "paged_append");
+  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, start, k_.size(0), err, "paged_append");
+  const Rope rope = rope_of(cos, sin, c.hd, c.k, "paged_append");
   const Tensor k = whole_heads(k_), v = whole_heads(v_);
-  check(ghb::paged_append(r, pool, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), is_f32(k), rope.cos, rope.sin, rope.half, rope.n_pos, stream()),
+  check(ghb::paged_append(r, c.pool(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), is_f32(k), rope.cos, rope.sin, rope.half, rope.n_pos, stream()),
         "paged_append");
 }
-void paged_read(const Tensor& kc, const Tensor& vc, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const Tensor& pages, const Tensor& q_start, const Tensor& lens,
-                Tensor& ko, Tensor& vo, bool fill, Tensor& err) {
-  const c10::cuda::CUDAGuard guard(kc.device());
-  const ghb::PagedPool pool = pool_of(kc, vc, ks, vs, "paged_read");
+std::tuple<Tensor, Tensor> paged_read(const PagedCache& c, const Tensor& pages, const Tensor& q_start, const Tensor& lens, int64_t n, const c10::optional<Tensor>& k_out,
+                                      const c10::optional<Tensor>& v_out, Tensor& err) {
+  const c10::cuda::CUDAGuard guard(c.k.device());
+  const bool fill = !k_out.has_value();
+  TORCH_CHECK(n >= 0 && fill == !v_out.has_value(), "paged_read: n >= 0, out two tensors or none");
+  TORCH_CHECK(fill || (k_out->dim() == 3 && k_out->size(0) == n), "paged_read: out holds ", k_out->dim() ? k_out->size(0) : 0, " tokens, n is ", n);
+  const auto opts = c.k.options().dtype(torch::kBFloat16);
+  Tensor ko = fill ? at::empty({n, c.heads, c.hd}, opts) : *k_out, vo = fill ? at::empty({n, c.heads, c.hd}, opts) : *v_out;
   for (const Tensor* o : {&ko, &vo})
-    TORCH_CHECK(o->dim() == 3 && is_bf16(*o) && o->is_contiguous() && o->size(1) == kc.size(1) && o->size(2) == pool.hd && o->size(0) == ko.size(0) && o->device() == kc.device() &&
-                reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0, "paged_read: out is two contiguous bfloat16 tensors [n, ", kc.size(1), ", ", pool.hd, "]");
-  const ghb::PagedRows r = rows_of(kc, pages, q_start, lens, c10::nullopt, ko.size(0), err, "paged_read");
-  check(ghb::paged_read(r, pool, ko.data_ptr(), vo.data_ptr(), fill, stream()), "paged_read");
+    TORCH_CHECK(o->dim() == 3 && is_bf16(*o) && o->is_contiguous() && o->size(0) == n && o->size(1) == c.heads && o->size(2) == c.hd && o->device() == c.k.device() &&
+                reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0, "paged_read: out is two contiguous bfloat16 tensors [", n, ", ", c.heads, ", ", c.hd, "], got ", o->sizes());
+  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, c10::nullopt, n, err, "paged_read");
+  check(ghb::paged_read(r, c.pool(), ko.data_ptr(), vo.data_ptr(), fill, stream()), "paged_read");
+  return {ko, vo};
 }
-void paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const Tensor& pages, const Tensor& q_start,
-                     const Tensor& lens, const c10::optional<Tensor>& start, const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, int64_t cap, double scale, Tensor& out,
-                     bool fill, Tensor& err) {
-  const c10::cuda::CUDAGuard guard(kc.device());
-  const ghb::PagedPool pool = pool_of(kc, vc, ks, vs, "paged_attention");
-  TORCH_CHECK(q.dim() == 3 && (is_bf16(q) || is_f32(q)) && q.device() == kc.device() && q.size(2) == pool.hd && q.size(1) > 0 && q.size(1) % kc.size(1) == 0 && q.size(2) == pool.hd,
-              "paged_attention: q bfloat16 or float32 [n, a multiple of ", kc.size(1), ", ", pool.hd, "] on the cache's device, got ", q.sizes());
+Tensor paged_attention(const Tensor& q, const PagedCache& c, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start,
+                       const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, int64_t cap, const c10::optional<double>& scale, const c10::optional<Tensor>& out_, Tensor& err) {
+  const c10::cuda::CUDAGuard guard(c.k.device());
+  TORCH_CHECK(q.dim() == 3 && (is_bf16(q) || is_f32(q)) && q.device() == c.k.device() && q.size(2) == c.hd && q.size(1) > 0 && q.size(1) % c.heads == 0,
+              "paged_attention: q bfloat16 or float32 [n, a multiple of ", c.heads, ", ", c.hd, "] on the cache's device, got ", q.sizes());
   TORCH_CHECK(q.stride(2) == 1, "paged_attention: q with unit inner stride");
-  TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.sizes() == q.sizes() && out.device() == kc.device() && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+  no_grad(q, "paged_attention");
+  const bool fill = !out_.has_value();
+  Tensor out = fill ? at::empty(q.sizes(), q.options().dtype(torch::kBFloat16)) : *out_;
+  TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.sizes() == q.sizes() && out.device() == c.k.device() && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
               "paged_attention: out is a contiguous bfloat16 tensor of q's shape");
-  const ghb::PagedRows r = rows_of(kc, pages, q_start, lens, start, q.size(0), err, "paged_attention");
-  TORCH_CHECK(kc.size(0) * kc.size(1) * kc.size(2) <= 0x7fffffff, "paged_attention: the cache has more than 2^31 entries of a head");
-  const Rope rope = rope_of(cos, sin, pool.hd, kc, "paged_attention");
+  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, start, q.size(0), err, "paged_attention");
+  TORCH_CHECK((static_cast<int64_t>(c.n_pages) * c.heads << c.page_shift) <= 0x7fffffff, "paged_attention: the cache has more than 2^31 entries of a head");
+  const Rope rope = rope_of(cos, sin, c.hd, c.k, "paged_attention");
   TORCH_CHECK(cap == 0 || (rope.half > 0 && cap > 0 && cap < rope.n_pos), "paged_attention: a rotary distance cap is >= 1 and inside the rope table");
   TORCH_CHECK(cap == 0 || rope.half == 8 || rope.half == 16 || rope.half == 32, "paged_attention: under a cap 16, 32 or 64 rotary channels on a GPU, got ", 2 * rope.half);
-  if (q.size(0) == 0) return;
+  const float sc = scale.has_value() ? static_cast<float>(*scale) : 1.0f / std::sqrt(static_cast<float>(c.hd));
+  TORCH_CHECK(sc > 0.f && std::isfinite(sc), "paged_attention: scale > 0");
+  if (q.size(0) == 0) return out;
   const ghb::PagedAttn a{q.data_ptr(), static_cast<long>(q.stride(0)), static_cast<long>(q.stride(1)), is_f32(q), out.data_ptr(), rope.cos, rope.sin, rope.half, rope.n_pos,
-                         static_cast<int>(cap), static_cast<int>(q.size(1)), static_cast<float>(scale), fill};
+                         static_cast<int>(cap), static_cast<int>(q.size(1)), sc, fill};
   ghb::PagedAttnPlan plan;
-  check(ghb::paged_attention_plan(r, pool, a.Hq, sm_count(), &plan), "paged_attention");
+  check(ghb::paged_attention_plan(r, c.pool(), a.Hq, sm_count(), &plan), "paged_attention");
   // this call's own work space (a captured call's comes from its graph's pool)
-  const Tensor ws = torch::empty({plan.ws_floats + plan.ws_ints}, q.options().dtype(torch::kFloat32));
-  check(ghb::paged_attention(r, pool, a, plan, ws.data_ptr<float>(), reinterpret_cast<int*>(ws.data_ptr<float>() + plan.ws_floats), stream()), "paged_attention");
+  const Tensor ws = at::empty({plan.ws_floats + plan.ws_ints}, q.options().dtype(torch::kFloat32));
+  check(ghb::paged_attention(r, c.pool(), a, plan, ws.data_ptr<float>(), reinterpret_cast<int*>(ws.data_ptr<float>() + plan.ws_floats), stream()), "paged_attention");
+  return out;
 }
-void verify_drafts(const Tensor& target, const c10::optional<Tensor>& draft, const Tensor& drafts, const Tensor& u_accept, const Tensor& u_sample, const c10::optional<Tensor>& n_drafts,
-                   Tensor& tokens, Tensor& kept, Tensor& err) {
+std::tuple<Tensor, Tensor> verify_drafts(const Tensor& target, const c10::optional<Tensor>& draft, const Tensor& drafts, const Tensor& u_accept, const Tensor& u_sample,
+                                         const c10::optional<Tensor>& n_drafts, Tensor& err) {
   const c10::cuda::CUDAGuard guard(target.device());
   TORCH_CHECK(target.is_cuda() && target.dim() == 3 && (is_bf16(target) || is_f32(target)) && target.size(1) >= 1 && target.size(2) >= 1 && target.stride(2) == 1,
               "verify_drafts: target bfloat16 or float32 [B, N + 1, V] with unit inner stride");
@@ -511,13 +535,14 @@ void verify_drafts(const Tensor& target, const c10::optional<Tensor>& draft, con
               "verify_drafts: drafts int64 [B, N], u_accept float32 [B, N], u_sample float32 [B]");
   for (const Tensor* t : {&drafts, &u_accept, &u_sample}) TORCH_CHECK(t->device() == target.device(), "verify_drafts: one device");
   if (n_drafts.has_value()) TORCH_CHECK(n_drafts->scalar_type() == torch::kInt32 && n_drafts->sizes() == u_sample.sizes() && n_drafts->is_contiguous() && n_drafts->device() == target.device(), "verify_drafts: n_drafts int32 [B]");
-  TORCH_CHECK(tokens.scalar_type() == torch::kInt64 && tokens.sizes() == at::IntArrayRef({B, N + 1}) && tokens.is_contiguous() && kept.scalar_type() == torch::kInt64 && kept.numel() == B, "verify_drafts: outputs");
+  const Tensor tokens = at::empty({B, N + 1}, drafts.options()), kept = at::empty({B}, drafts.options());
   const ghb::VerifyArgs a{target.data_ptr(), static_cast<long>(target.stride(0)), static_cast<long>(target.stride(1)), draft.has_value() ? draft->data_ptr() : nullptr,
                           draft.has_value() ? static_cast<long>(draft->stride(0)) : 0, draft.has_value() ? static_cast<long>(draft->stride(1)) : 0, is_bf16(target),
                           reinterpret_cast<const long*>(drafts.data_ptr<int64_t>()), u_accept.data_ptr<float>(), u_sample.data_ptr<float>(),
                           n_drafts.has_value() ? n_drafts->data_ptr<int>() : nullptr, reinterpret_cast<long*>(tokens.data_ptr<int64_t>()),
                           reinterpret_cast<long*>(kept.data_ptr<int64_t>()), static_cast<int>(B), static_cast<int>(N), static_cast<int>(V), err.data_ptr<int>()};
   check(ghb::verify_drafts(a, stream()), "verify_drafts");
+  return {tokens, kept};
 }
 
 // ---- fused data-parallel step over peer memory. `peers` is a CPU uint8 tensor holding the pointer table.
@@ -675,6 +700,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_bwd", &embedding_bwd);
   m.def("decode_attention", &decode_attention);
   m.def("decode_attention_grid", &decode_attention_grid);
+  py::class_<PagedCache>(m, "PagedCache");
+  m.def("paged_cache", &paged_cache);
   m.def("paged_append", &paged_append);
   m.def("paged_read", &paged_read);
   m.def("paged_attention", &paged_attention);

@@ -12,9 +12,9 @@
 //
 // 4 bits: a lane's 16 channels of a key are one block with one scale. Codes become f16 pairs (cvt.f16x2.e2m1x2), times the
 // scale: exact in f16 (2 + 4 significant bits, 2^-10 .. 2688). Queries are rounded to f16 once (2^-12 relative), after a
-// power of two per query row has brought them to about one, probabilities to f16 scaled by 2^14, so that one of 2^-28 of the
-// maximum is still normal. bfloat16 cache: queries as the sum of two bfloat16 (2^-17), keys as they are, probabilities to
-// bfloat16 (2^-9) with the sum taken over the rounded ones. All sums are float32 in the accumulators.
+// power of two per query row has brought them to about one, probabilities to f16 (2^-12, scaled up: PSHIFT below). bfloat16 cache:
+// queries as the sum of two bfloat16 (2^-17), keys as they are, probabilities to bfloat16 (2^-9). The sum of the probabilities is
+// taken over the rounded ones. All sums are float32 in the accumulators.
 //
 // Work: the pieces (one tile of positions for each warp) of all (row, KV head, block of query rows) units form one sequence,
 // and every CTA takes an equal share of it, so that rows of any lengths load the SMs evenly. Each CTA finds its share by
@@ -27,6 +27,8 @@
 // (Bulk copies cost one instruction instead of nine, but about 32 clocks each in the SM's copy engine, which bound
 // the loop; one more warp that loads for all the others ties them to the slowest. Both were measured slower.) What no
 // row sees gets scales of zero (4 bits), so that its values are zero.
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace ghb {
@@ -65,7 +67,10 @@ struct Geo : Cfg<FP4, HD, NT> {
   static constexpr int PIECE = B::W * TILE;
   static constexpr int RING = B::W * ST * STAGE;
   static constexpr int MERGE = B::W * UR * HD * 4;
-  static constexpr int DATA = RING > MERGE ? RING : MERGE;
+  // Partial outputs beside the ring, where both fit twice on an SM: the next unit's first tiles are then on their way while the
+  // warps of this one join. Else over it.
+  static constexpr bool BESIDE = FP4 && NT == 1 && HD == 64;
+  static constexpr int DATA = BESIDE ? RING + MERGE : RING > MERGE ? RING : MERGE;
   static constexpr int QCOPIES = FP4 ? 1 : 2;        // bfloat16: high and low part
   static constexpr int QB = UR * HD * 2;             // bytes of one copy of the queries
   // under a cap: near and far queries, the near ones' rotary channels in float32 and as each warp rotated them, a tile of rotations
@@ -148,6 +153,12 @@ template <bool FP4>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   if constexpr (FP4) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
   else { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+}
+// a byte's low half of a, its high half of b
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, 0x0f0f0f0f, 0xe4;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
@@ -250,9 +261,11 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     }
   }
 
+  // ---- the part of a unit that this CTA does next
+  struct Part { int b, q0, start, h, r0, n_rows, p0, n_pieces, pieces, pos0, p_first, p_last, tile0; };
   long at = lo;
-  while (at < hi) {
-    // ---- the unit that piece `at` belongs to
+  Part sg;
+  auto locate = [&]() {
     Row row = load_row(R, b);
     RowWork wk = row_work<GEO>(row, G);
     long count = static_cast<long>(wk.units) * wk.pieces * Hkv;
@@ -264,100 +277,111 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       count = static_cast<long>(wk.units) * wk.pieces * Hkv;
     }
     const long in_row = at - row_at;
-    const int unit = static_cast<int>(in_row / wk.pieces), p0 = static_cast<int>(in_row % wk.pieces);
-    const int n_pieces = static_cast<int>(min(static_cast<long>(wk.pieces - p0), hi - at));
-    const int h = unit / wk.units, r0 = (unit % wk.units) * UR;
-    const int n_rows = min(UR, row.nq * G - r0);
-    const int pos0 = row.len - row.nq;                              // position of the row's first new token
-    const int p_first = pos0 + r0 / G, p_last = row.len ? pos0 + (r0 + n_rows - 1) / G : -1;
-    // ---- loads of one tile: positions tile0 + k PIECE .. + TILE. A tile is one or more chunks, each within a page and so contiguous
-    // per head (bfloat16: a chunk is one position); lane i knows the page of chunk i, all lanes copy 16 bytes at a time.
-    const int tile0 = wk.base + p0 * GEO::PIECE + warp * TILE;
-    const int c_shift = min(R.page_shift, TILE == 64 ? 6 : TILE == 32 ? 5 : 4);
-    const unsigned all_on = (1u << (TILE >> c_shift)) - 1u;
-    // Page ids are looked up for 32 chunks at a time (32 tiles where a page holds a tile): lane i holds the entry of chunk i of them.
-    const int n_log = TILE == 64 ? 6 - c_shift : TILE == 32 ? 5 - c_shift : 4 - c_shift;          // log2 of a tile's chunks
-    int entry = 0;
-    unsigned batch_on = 0;
-    auto look_up = [&](int k) {                // tiles k .. of this warp
-      const int tok = tile0 + (k + (lane >> n_log)) * GEO::PIECE + ((lane & ((1 << n_log) - 1)) << c_shift);
-      entry = -1;
-      if (k + (lane >> n_log) < n_pieces && tok + (1 << c_shift) > row.start && tok <= p_last) {
-        const int pg = R.pages[b * R.pages_stride + (tok >> R.page_shift)];
-        if (pg < 0 || pg >= R.n_pages) *R.err = ST_PAGE;
-        else entry = ((pg * Hkv + h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1));
-      }
-      batch_on = __ballot_sync(0xffffffffu, entry >= 0);
-    };
-    const uint8_t* k_lane = static_cast<const uint8_t*>(p.c.k) + lane * 16;
-    const uint8_t* v_lane = static_cast<const uint8_t*>(p.c.v) + lane * 16;
-    constexpr int L = FP4 ? TILE * GEO::S / 16 : 1;          // 16-byte parts of a tile's key scales; its value scales follow
-    const uint8_t* s_lane = lane % (2 * L) < L ? p.c.k_scale : p.c.v_scale;
-    auto issue = [&](int k, int stage) -> unsigned {         // returns the mask of tile k's chunks that are read
-      if ((k & ((32 >> n_log) - 1)) == 0 && k < n_pieces) look_up(k);
-      const int at_chunk = (k << n_log) & 31;
-      const unsigned on = k < n_pieces ? (batch_on >> at_chunk) & all_on : 0u;
-      if (on) {
-        const uint32_t st = ring_u + stage * GEO::STAGE;
-        constexpr int CH = GEO::ROW / 16, N = TILE * CH / 32;        // 16-byte parts of a position; copies a lane makes of keys
-        auto place_of = [&](int pos, int sub) -> uint32_t {          // bfloat16: slices of 128-byte rows, swizzled
-          if constexpr (FP4) return pos * GEO::ROW + sub * 16;
-          else return (sub >> 3) * (TILE * 128) + pos * 128 + (((sub & 7) ^ (pos & 7)) << 4);
-        };
-        if (n_log == 0) {                      // the whole tile lies in one page: one address, fixed distances
-          const int e = __shfl_sync(0xffffffffu, entry, at_chunk);
-          const long off = static_cast<long>(e) * GEO::ROW;
+    const int unit = static_cast<int>(in_row / wk.pieces);
+    sg.b = b; sg.q0 = row.q0; sg.start = row.start; sg.pieces = wk.pieces;
+    sg.p0 = static_cast<int>(in_row % wk.pieces);
+    sg.n_pieces = static_cast<int>(min(static_cast<long>(wk.pieces - sg.p0), hi - at));
+    sg.h = unit / wk.units; sg.r0 = (unit % wk.units) * UR;
+    sg.n_rows = min(UR, row.nq * G - sg.r0);
+    sg.pos0 = row.len - row.nq;                              // position of the row's first new token
+    sg.p_first = sg.pos0 + sg.r0 / G;
+    sg.p_last = row.len ? sg.pos0 + (sg.r0 + sg.n_rows - 1) / G : -1;
+    sg.tile0 = wk.base + sg.p0 * GEO::PIECE + warp * TILE;
+  };
+  // ---- loads of one tile: positions tile0 + k PIECE .. + TILE. A tile is one or more chunks, each within a page and so contiguous
+  // per head; all lanes copy 16 bytes at a time. Page ids are looked up for 32 chunks at once (32 tiles where a page holds a
+  // tile): lane i holds the entry of chunk i of them.
+  const int c_shift = min(R.page_shift, TILE == 64 ? 6 : TILE == 32 ? 5 : 4);
+  const unsigned all_on = (1u << (TILE >> c_shift)) - 1u;
+  const int n_log = TILE == 64 ? 6 - c_shift : TILE == 32 ? 5 - c_shift : 4 - c_shift;          // log2 of a tile's chunks
+  int entry = 0;
+  unsigned batch_on = 0;
+  auto look_up = [&](int k) {                // tiles k .. of this warp
+    const int tok = sg.tile0 + (k + (lane >> n_log)) * GEO::PIECE + ((lane & ((1 << n_log) - 1)) << c_shift);
+    entry = -1;
+    if (k + (lane >> n_log) < sg.n_pieces && tok + (1 << c_shift) > sg.start && tok <= sg.p_last) {
+      const int pg = R.pages[sg.b * R.pages_stride + (tok >> R.page_shift)];
+      if (pg < 0 || pg >= R.n_pages) *R.err = ST_PAGE;
+      else entry = ((pg * Hkv + sg.h) << R.page_shift) + (tok & ((1 << R.page_shift) - 1));
+    }
+    batch_on = __ballot_sync(0xffffffffu, entry >= 0);
+  };
+  const uint8_t* k_lane = static_cast<const uint8_t*>(p.c.k) + lane * 16;
+  const uint8_t* v_lane = static_cast<const uint8_t*>(p.c.v) + lane * 16;
+  constexpr int L = FP4 ? TILE * GEO::S / 16 : 1;          // 16-byte parts of a tile's key scales; its value scales follow
+  const uint8_t* s_lane = lane % (2 * L) < L ? p.c.k_scale : p.c.v_scale;
+  auto issue = [&](int k, int stage) -> unsigned {         // returns the mask of tile k's chunks that are read
+    if ((k & ((32 >> n_log) - 1)) == 0 && k < sg.n_pieces) look_up(k);
+    const int at_chunk = (k << n_log) & 31;
+    const unsigned on = k < sg.n_pieces ? (batch_on >> at_chunk) & all_on : 0u;
+    if (on) {
+      const uint32_t st = ring_u + stage * GEO::STAGE;
+      constexpr int CH = GEO::ROW / 16, N = TILE * CH / 32;        // 16-byte parts of a position; copies a lane makes of keys
+      auto place_of = [&](int pos, int sub) -> uint32_t {          // bfloat16: slices of 128-byte rows, swizzled
+        if constexpr (FP4) return pos * GEO::ROW + sub * 16;
+        else return (sub >> 3) * (TILE * 128) + pos * 128 + (((sub & 7) ^ (pos & 7)) << 4);
+      };
+      if (n_log == 0) {                      // the whole tile lies in one page: one address, fixed distances
+        const int e = __shfl_sync(0xffffffffu, entry, at_chunk);
+        const long off = static_cast<long>(e) * GEO::ROW;
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const uint32_t dst = st + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH);
-            cp16(dst, k_lane + off + i * 512);
-            cp16(dst + GEO::KB, v_lane + off + i * 512);
+        for (int i = 0; i < N; ++i) {
+          const uint32_t dst = st + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH);
+          cp16(dst, k_lane + off + i * 512);
+          cp16(dst + GEO::KB, v_lane + off + i * 512);
+        }
+        if constexpr (FP4) {
+          const long soff = static_cast<long>(e) * GEO::S + (lane % L) * 16;
+          if constexpr (2 * L > 32) {        // (wide heads: one copy for the keys', one for the values')
+            cp16(st + 2 * GEO::KB + lane * 16, p.c.k_scale + soff);
+            cp16(st + 2 * GEO::KB + GEO::SB + lane * 16, p.c.v_scale + soff);
+          } else if (2 * L == 32 || lane < 2 * L) {
+            cp16(st + 2 * GEO::KB + lane * 16, s_lane + soff);
           }
-          if constexpr (FP4) {
-            const long soff = static_cast<long>(e) * GEO::S + (lane % L) * 16;
-            if constexpr (2 * L > 32) {        // (wide heads: one copy for the keys', one for the values')
-              cp16(st + 2 * GEO::KB + lane * 16, p.c.k_scale + soff);
-              cp16(st + 2 * GEO::KB + GEO::SB + lane * 16, p.c.v_scale + soff);
-            } else if (2 * L == 32 || lane < 2 * L) {
-              cp16(st + 2 * GEO::KB + lane * 16, s_lane + soff);
-            }
-          }
-        } else {
+        }
+      } else {
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const int pos = (i * 32 + lane) / CH, sub = (i * 32 + lane) % CH, c = pos >> c_shift;
+        for (int i = 0; i < N; ++i) {
+          const int pos = (i * 32 + lane) / CH, sub = (i * 32 + lane) % CH, c = pos >> c_shift;
+          const int e = __shfl_sync(0xffffffffu, entry, at_chunk + c) + (pos & ((1 << c_shift) - 1));
+          const long off = static_cast<long>(e) * GEO::ROW + sub * 16;
+          const bool ok = (on >> c) & 1;
+          const uint32_t dst = st + place_of(pos, sub);
+          cp16(dst, static_cast<const uint8_t*>(p.c.k) + (ok ? off : 0), ok);
+          cp16(dst + GEO::KB, static_cast<const uint8_t*>(p.c.v) + (ok ? off : 0), ok);
+        }
+        if constexpr (FP4) {
+#pragma unroll
+          for (int i = 0; i < (2 * L + 31) / 32; ++i) {
+            const int idx = i * 32 + lane, pos = (idx % L) * (16 / GEO::S), c = pos >> c_shift;
             const int e = __shfl_sync(0xffffffffu, entry, at_chunk + c) + (pos & ((1 << c_shift) - 1));
-            const long off = static_cast<long>(e) * GEO::ROW + sub * 16;
             const bool ok = (on >> c) & 1;
-            const uint32_t dst = st + place_of(pos, sub);
-            cp16(dst, static_cast<const uint8_t*>(p.c.k) + (ok ? off : 0), ok);
-            cp16(dst + GEO::KB, static_cast<const uint8_t*>(p.c.v) + (ok ? off : 0), ok);
-          }
-          if constexpr (FP4) {
-#pragma unroll
-            for (int i = 0; i < (2 * L + 31) / 32; ++i) {
-              const int idx = i * 32 + lane, pos = (idx % L) * (16 / GEO::S), c = pos >> c_shift;
-              const int e = __shfl_sync(0xffffffffu, entry, at_chunk + c) + (pos & ((1 << c_shift) - 1));
-              const bool ok = (on >> c) & 1;
-              const uint8_t* base = idx % (2 * L) < L ? p.c.k_scale : p.c.v_scale;
-              if (2 * L >= 32 || idx < 2 * L) cp16(st + 2 * GEO::KB + idx * 16, base + (ok ? static_cast<long>(e) * GEO::S : 0), ok);
-            }
+            const uint8_t* base = idx % (2 * L) < L ? p.c.k_scale : p.c.v_scale;
+            if (2 * L >= 32 || idx < 2 * L) cp16(st + 2 * GEO::KB + idx * 16, base + (ok ? static_cast<long>(e) * GEO::S : 0), ok);
           }
         }
       }
-      cp_commit();
-      return on;
-    };
-    unsigned on_ring[ST];
+    }
+    cp_commit();
+    return on;
+  };
+  unsigned on_ring[ST];
+  auto begin = [&]() {
 #pragma unroll
     for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k, k);
+  };
+  locate();
+  begin();
+  while (true) {
+    const int h = sg.h, r0 = sg.r0, n_rows = sg.n_rows, n_pieces = sg.n_pieces, pos0 = sg.pos0, p_first = sg.p_first, p_last = sg.p_last, tile0 = sg.tile0;
+    const int q0 = sg.q0, start = sg.start, p0 = sg.p0, pieces = sg.pieces;
     int stage = 0;                             // of tile k
 
     // ---- the unit's queries: rotated (near at their positions, far by the cap), brought to about one, in the MMA's order
     for (int r = warp; r < UR; r += W) {
-      const bool live = r < n_rows && row.len > 0;
+      const bool live = r < n_rows && p_last >= 0;
       const int rr = r0 + r;
-      const long tok = row.q0 + (live ? rr / G : 0);
+      const long tok = q0 + (live ? rr / G : 0);
       const int head = h * G + (live ? rr % G : 0);
       const long off = tok * p.a.q_ts + head * p.a.q_hs;
       auto qv = [&](int c) -> float {
@@ -375,7 +399,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       const float down = exp2f(static_cast<float>(-ex));
       if (lane == 0) s_mul[r] = p.a.scale * 1.44269504088896340736f * exp2f(static_cast<float>(ex));
       if (lane == 0) s_pos[r] = live ? pos0 + rr / G : -1;
-      int qpos = pos0 + rr / G - row.start;
+      int qpos = pos0 + rr / G - start;
       if (live && half > 0 && qpos >= p.a.n_pos) { *R.err = ST_ROPE; qpos = p.a.n_pos - 1; }
       qpos = CAP ? p.a.cap : max(qpos, 0);
 #pragma unroll
@@ -421,7 +445,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       for (int e = 0; e < 2; ++e) {
         const int r = n * 8 + 2 * t + e;
         mul[n][e] = s_mul[r];
-        prow[n][e] = r < n_rows && row.len > 0 ? pos0 + (r0 + r) / G : -1;
+        prow[n][e] = r < n_rows && p_last >= 0 ? pos0 + (r0 + r) / G : -1;
         m[n][e] = -INFINITY; l[n][e] = l[n][e + 2] = 0.f;
       }
     float o[H * 4][NT][4];
@@ -443,11 +467,11 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       __syncwarp();
       stage = stage == ST - 1 ? 0 : stage + 1;
       if (on) {
-        const bool masked = on != all_on || first < row.start || first + TILE - 1 > p_first;
+        const bool masked = on != all_on || first < start || first + TILE - 1 > p_first;
         if (FP4 && masked) {
           // what no row sees may hold anything: its scales become zero, so that its values are zero
           for (int pos = lane; pos < TILE; pos += 32) {
-            if (!((on >> (pos >> c_shift)) & 1) || first + pos < row.start || first + pos > p_last) {
+            if (!((on >> (pos >> c_shift)) & 1) || first + pos < start || first + pos > p_last) {
 #pragma unroll
               for (int i = 0; i < GEO::S / 4; ++i) *reinterpret_cast<uint32_t*>(st + 2 * GEO::KB + GEO::SB + pos * GEO::S + 4 * i) = 0u;
             }
@@ -509,7 +533,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             // one of TILE rotations that stay in shared memory, the queries' rotary channels are rotated once a tile. A lane owns channels
             // 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16, so that both channels of a rotary pair (half 8, 16 or 32
             // apart) are its own.
-            const int t0 = max(first, row.start);
+            const int t0 = max(first, start);
             const int steps = half >> 3, slot_low = NT * steps * 256;          // rotary k16 steps; bytes of the high parts
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -608,7 +632,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int pos = mt * 16 + (e >> 1) * 8 + place<FP4>(g);
-                if (!((on >> (pos >> c_shift)) & 1) || first + pos < row.start || first + pos > prow[n][e & 1]) s[mt][n][e] = -INFINITY;
+                if (!((on >> (pos >> c_shift)) & 1) || first + pos < start || first + pos > prow[n][e & 1]) s[mt][n][e] = -INFINITY;
               }
         }
         // ---- the reference of the exponents, where a score leaves the slack (raw scores: the factor is positive)
@@ -674,7 +698,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             plain = !__any_sync(0xffffffffu, odd);
           }
           if (!plain) {
-            auto see = [&](int j, int n, int e) { return first + j >= row.start && first + j <= prow[n][e]; };
+            auto see = [&](int j, int n, int e) { return first + j >= start && first + j <= prow[n][e]; };
             for (int j = 0; j < TILE; ++j) {
               if (!((on >> (j >> c_shift)) & 1)) continue;
 #pragma unroll
@@ -722,10 +746,10 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
                 const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vb + u0 * GEO::ROW), w1 = *reinterpret_cast<const uint32_t*>(vb + u1 * GEO::ROW);
                 const uint32_t w2 = *reinterpret_cast<const uint32_t*>(vb + (u0 + 8) * GEO::ROW), w3 = *reinterpret_cast<const uint32_t*>(vb + (u1 + 8) * GEO::ROW);
                 uint32_t c0[4], c1[4], c2[4], c3[4];
-                codes_to_f16((w0 & 0x0f0f0f0fu) | ((w1 << 4) & 0xf0f0f0f0u), c0);
-                codes_to_f16(((w0 >> 4) & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u), c1);
-                codes_to_f16((w2 & 0x0f0f0f0fu) | ((w3 << 4) & 0xf0f0f0f0u), c2);
-                codes_to_f16(((w2 >> 4) & 0x0f0f0f0fu) | (w3 & 0xf0f0f0f0u), c3);
+                codes_to_f16(low_nibbles(w0, w1 << 4), c0);
+                codes_to_f16(low_nibbles(w0 >> 4, w1), c1);
+                codes_to_f16(low_nibbles(w2, w3 << 4), c2);
+                codes_to_f16(low_nibbles(w2 >> 4, w3), c3);
                 const uint8_t* sb = st + 2 * GEO::KB + GEO::SB + hs * 4;
                 auto scale_of = [&](int u) { return *reinterpret_cast<const uint32_t*>(sb + u * GEO::S); };
                 const uint32_t pick = (g >> 1) | ((4 + (g >> 1)) << 4);            // this lane's block of both
@@ -762,10 +786,10 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       __syncwarp();          // the stage is consumed before the next issue refills it
     }
     cp_wait<0>();
-    __syncthreads();         // every warp is done with its ring: the region takes the partial outputs
+    if constexpr (!GEO::BESIDE) __syncthreads();         // every warp is done with its ring: the region takes the partial outputs
 
     // ---- join the warps
-    float* so = reinterpret_cast<float*>(smem);
+    float* so = reinterpret_cast<float*>(smem + (GEO::BESIDE ? GEO::RING : 0));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -777,8 +801,13 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
         for (int i = 0; i < H * 4; ++i)
           *reinterpret_cast<float2*>(dst + (i >> 2) * 64 + (i & 3) * 2) = make_float2(o[i][n][e], o[i][n][e + 2]);
       }
+    const long first_piece = at;
+    at += n_pieces;
+    const bool more = at < hi;
+    if (!more) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if constexpr (GEO::BESIDE) { if (more) { locate(); begin(); } }
     __syncthreads();
-    const bool begins = p0 == 0, ends = p0 + n_pieces == wk.pieces;
+    const bool begins = p0 == 0, ends = p0 + n_pieces == pieces;
     const int slot = begins ? 1 : 0;
     float* wo = p.ws + (static_cast<long>(cta) * 2 + slot) * UR * (HD + 2);
     for (int idx = tid; idx < n_rows * HD; idx += GEO::THREADS) {
@@ -798,19 +827,23 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       if (begins && ends) {
         const int rr = r0 + r;
         // a row of scores without one above -inf has no weights: zeros
-        static_cast<__nv_bfloat16*>(p.a.out)[((static_cast<long>(row.q0) + rr / G) * p.a.Hq + h * G + rr % G) * HD + c] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
+        static_cast<__nv_bfloat16*>(p.a.out)[((static_cast<long>(q0) + rr / G) * p.a.Hq + h * G + rr % G) * HD + c] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
       } else {
         wo[r * HD + c] = oo;
         if (c == 0) { wo[UR * HD + 2 * r] = mm; wo[UR * HD + 2 * r + 1] = ll; }
       }
     }
     if (tid == 0 && begins && !ends) {           // the first part: how many CTAs hold the others follows from the shares
-      const long last = at + wk.pieces - 1;      // the unit's last piece
-      meta[1] = h; meta[2] = r0; meta[3] = n_rows; meta[4] = row.q0;
+      const long last = first_piece + pieces - 1;      // the unit's last piece
+      meta[1] = h; meta[2] = r0; meta[3] = n_rows; meta[4] = q0;
       meta[0] = static_cast<int>(((last + 1) * use - 1) / total) - cta + 1;
     }
-    at += n_pieces;
-    __syncthreads();
+    if (!more) break;
+    if constexpr (!GEO::BESIDE) {
+      __syncthreads();
+      locate();
+      begin();
+    }
   }
 }
 
@@ -823,6 +856,7 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_
   __shared__ float4 s_o[GROUPS][LANES];
   __shared__ float s_m[GROUPS], s_l[GROUPS];
   const int i = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");          // launched while the first kernel ends; from here on that is complete
   if (p.a.fill) {
     const int q_end = p.r.B ? p.r.q_start[p.r.B] : 0;
     if (q_end >= 0) {
@@ -878,10 +912,25 @@ template <bool FP4, int HD, int NT, bool CAP>
 int launch(const AttnK& k, int ctas, cudaStream_t st) {
   using GEO = Geo<FP4, HD, NT>;
   const int bytes = GEO::smem(CAP ? k.a.half : 0);
-  // (set on every call: the attribute belongs to the device that is current, and costs no launch)
-  if (cudaFuncSetAttribute(paged_attention_kernel<FP4, HD, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return 4;
+  // (the largest size this kernel can ask for, set once per device)
+  static std::atomic<uint64_t> ready[4];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 4;
+  if (dev > 255 || !(ready[dev >> 6].load(std::memory_order_acquire) >> (dev & 63) & 1)) {
+    if (cudaFuncSetAttribute(paged_attention_kernel<FP4, HD, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEO::smem(CAP ? 32 : 0)) != cudaSuccess) return 4;
+    if (dev <= 255) ready[dev >> 6].fetch_or(uint64_t(1) << (dev & 63), std::memory_order_release);
+  }
   paged_attention_kernel<FP4, HD, NT, CAP><<<ctas, GEO::THREADS, bytes, st>>>(k);
-  paged_attention_join_kernel<HD, GEO::UR><<<dim3(ctas, GEO::UR), 256, 0, st>>>(k, ctas);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, GEO::UR);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<HD, GEO::UR>, k, ctas) != cudaSuccess) return 4;
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 template <bool FP4, int HD, int NT>

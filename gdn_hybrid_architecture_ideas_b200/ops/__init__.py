@@ -34,9 +34,21 @@ def use_native(x: torch.Tensor) -> bool:
     return x.is_cuda and _MODE == "native"
 
 
+_native_module = None
+
+
 def _native():
-    from . import native
-    return native
+    global _native_module
+    if _native_module is None:
+        from . import native
+        _native_module = native
+    return _native_module
+
+
+def native_cache(cache) -> None:
+    """Checks a PagedKV on a GPU (in the binding, once); nothing to do in reference mode."""
+    if _MODE == "native":
+        _native()._cache(cache)
 
 
 def rmsnorm(x, weight, eps, out_dtype=None):

@@ -697,41 +697,39 @@ def attention(q, k, v, doc, q_far, k_far, cap, pos=None, single_doc=False):
 
 # ------------------------------------------------------------------------------------------------------------ paged cache, drafts
 
+def _cache(cache):
+    """The binding's checked form of a PagedKV's tensors, made on first use."""
+    c = cache.native
+    if c is None:
+        c = cache.native = ext().paged_cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
+    return c
+
+
 def paged_append(cache, k, v, pages, q_start, lens, start, rope):
-    cos, sin = (None, None) if rope is None else rope
-    ext().paged_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, pages, q_start, lens, start, cos, sin, err_flag(cache.k.device))
+    cos, sin = rope or (None, None)
+    ext().paged_append(_cache(cache), k, v, pages, q_start, lens, start, cos, sin, err_flag(cache.k.device))
     _count()
 
 
 def paged_read(cache, pages, q_start, lens, n, out):
-    fill = out is None
-    if fill:
-        shape = (n, cache.n_kv_heads, cache.head_dim)
-        out = (torch.empty(shape, dtype=BF16, device=cache.k.device), torch.empty(shape, dtype=BF16, device=cache.k.device))
-    elif out[0].shape[0] != n:
-        raise ValueError(f"paged_read: out holds {out[0].shape[0]} tokens, n is {n}")
-    ext().paged_read(cache.k, cache.v, cache.k_scale, cache.v_scale, pages, q_start, lens, out[0], out[1], fill, err_flag(cache.k.device))
+    ko, vo = out or (None, None)
+    r = ext().paged_read(_cache(cache), pages, q_start, lens, n, ko, vo, err_flag(cache.k.device))
     _count()
-    return out
+    return r
 
 
 def paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out):
-    cos, sin = (None, None) if rope is None else rope
-    if cap is not None and (rope is None or cap < 1):
+    cos, sin = rope or (None, None)
+    if cap is None:
+        cap = 0
+    elif rope is None or cap < 1:
         raise ValueError("paged_attention: a rotary distance cap is an integer >= 1 beside a rope table")
-    fill = out is None
-    if fill:
-        out = torch.empty(q.shape, dtype=BF16, device=q.device)
-    ext().paged_attention(q.detach(), cache.k, cache.v, cache.k_scale, cache.v_scale, pages, q_start, lens, start, cos, sin, cap or 0,
-                          q.shape[-1] ** -0.5 if scale is None else scale, out, fill, err_flag(cache.k.device))
+    out = ext().paged_attention(q, _cache(cache), pages, q_start, lens, start, cos, sin, cap, scale, out, err_flag(cache.k.device))
     _count(2)
     return out
 
 
 def verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts):
-    B, N1 = target.shape[:2]
-    tokens = torch.empty(B, N1, dtype=torch.long, device=target.device)
-    kept = torch.empty(B, dtype=torch.long, device=target.device)
-    ext().verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts, tokens, kept, err_flag(target.device))
+    r = ext().verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts, err_flag(target.device))
     _count()
-    return tokens, kept
+    return r

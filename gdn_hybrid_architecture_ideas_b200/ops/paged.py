@@ -37,9 +37,16 @@ LARGEST = 6.0 * 448.0
 class PagedKV:
     """The cache's tensors (see the module's head for the layout). `PagedKV.zeros` allocates an empty one."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale")
+    __slots__ = ("_k", "_v", "_ks", "_vs", "native")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
+        self._k, self._v, self._ks, self._vs = k, v, k_scale, v_scale          # (fixed: the binding holds them too)
+        self.native = None              # the CUDA binding's form of these tensors (ops/native.py)
+        if k.is_cuda:
+            from . import native_cache
+
+            native_cache(self)          # checks in the binding
+            return
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise ValueError(f"PagedKV: k and v are [pages, kv heads, page size, channels] of one type on one device, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
         if not (k.is_contiguous() and v.is_contiguous()):
@@ -56,7 +63,6 @@ class PagedKV:
         page = k.shape[2]
         if page < 8 or page & (page - 1):
             raise ValueError(f"PagedKV: the page size is a power of two from 8 on, got {page}")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
 
     @classmethod
     def zeros(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, fmt: str = "bf16", device="cpu", make=None) -> "PagedKV":
@@ -74,6 +80,11 @@ class PagedKV:
         if fmt not in dtypes:
             raise ValueError(f"PagedKV: fmt {fmt!r}: 'bf16', 'fp4' (on the CPU also 'fp32', 'fp64')")
         return cls(*(make(n, (*lead, head_dim), dtypes[fmt]) for n in ("k", "v")))
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scale = property(lambda self: self._ks)
+    v_scale = property(lambda self: self._vs)
 
     @property
     def fp4(self) -> bool:
