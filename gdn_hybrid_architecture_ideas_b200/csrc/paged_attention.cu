@@ -479,26 +479,38 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
           __syncwarp();
         }
         float s[MT][NT][4];
+        // Products that add into one accumulator wait for one another: wide heads take two by turns of their slices, bfloat16 two more
+        // for the low parts, summed at the end (a head of 256 is 32 products otherwise in one chain).
+        constexpr int CHAINS = (H > 1 ? 2 : 1) * GEO::QCOPIES;
         // one k16 step of the 16 positions of tile mt against every column block; its queries start at qs, a block's at by bytes further
-        auto step = [&](float (&acc)[NT][4], const uint32_t* a, const uint8_t* qs, int by, int low, bool begin) {
+        auto step = [&](float (&acc)[CHAINS][NT][4], const uint32_t* a, const uint8_t* qs, int by, int low, int hs, bool begin) {
+          const int c = (H > 1 ? hs & 1 : 0) * GEO::QCOPIES;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             if (NT > 1 && n >= live_n) continue;
             const uint2 q1 = *reinterpret_cast<const uint2*>(qs + n * by + lane * 8);
-            if (begin) mma_first<FP4>(acc[n], a, q1.x, q1.y);
-            else mma<FP4>(acc[n], a, q1.x, q1.y);
+            if (begin) mma_first<FP4>(acc[c][n], a, q1.x, q1.y);
+            else mma<FP4>(acc[c][n], a, q1.x, q1.y);
             if constexpr (!FP4) {
               const uint2 q2 = *reinterpret_cast<const uint2*>(qs + low + n * by + lane * 8);
-              mma<FP4>(acc[n], a, q2.x, q2.y);
+              if (begin) mma_first<FP4>(acc[c + 1][n], a, q2.x, q2.y);
+              else mma<FP4>(acc[c + 1][n], a, q2.x, q2.y);
             }
           }
+        };
+        auto joined = [&](float (&acc)[CHAINS][NT][4], int n, int e) -> float {
+          float x = acc[0][n][e];
+#pragma unroll
+          for (int c = 1; c < CHAINS; ++c) x += acc[c][n][e];
+          return x;
         };
         const bool far_any = !CAP || p_last - first > p.a.cap;                     // some (row, position) beyond the cap
         const bool near_any = CAP && p_first - (first + TILE - 1) <= p.a.cap;      // some within it
         if (far_any) {
           // ---- keys as cached: a lane owns 16 consecutive channels of a slice (4 bits: one block)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int mt = 0; mt < MT; ++mt) {
+            float acc[CHAINS][NT][4];
 #pragma unroll
             for (int hs = 0; hs < H; ++hs) {
               uint32_t x[2][8];                // [row g or g + 8][channel pair]: channels 16 t + 2 i of slice hs
@@ -523,9 +535,14 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
               for (int ks = 0; ks < 4; ++ks) {
                 const uint32_t a[4] = {x[0][2 * ks], x[1][2 * ks], x[0][2 * ks + 1], x[1][2 * ks + 1]};
-                step(s[mt], a, sq + (hs * 4 + ks) * 256, HD * 16, GEO::QB, hs == 0 && ks == 0);
+                step(acc, a, sq + (hs * 4 + ks) * 256, HD * 16, GEO::QB, hs, hs < 2 && (hs == 0 || H > 1) && ks == 0);
               }
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[mt][n][e] = joined(acc, n, e);
+          }
         }
         if constexpr (CAP) {
           if (near_any) {
@@ -564,7 +581,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             }
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              float acc[NT][4];
+              float acc[CHAINS][NT][4];
 #pragma unroll
               for (int hs = 0; hs < H; ++hs) {
                 uint32_t x[2][4][2];           // [row][block of the slice][channels 2 t.. or 2 t + 8 ..]
@@ -609,7 +626,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
                   const uint32_t a[4] = {x[0][bl][0], x[1][bl][0], x[0][bl][1], x[1][bl][1]};
                   const int ks = hs * 4 + bl;
                   const bool own = hs == 0 && bl < steps;
-                  step(acc, a, own ? s_turned + ks * 256 : sq + GEO::QCOPIES * GEO::QB + ks * 256, own ? steps * 256 : HD * 16, own ? slot_low : GEO::QB, ks == 0);
+                  step(acc, a, own ? s_turned + ks * 256 : sq + GEO::QCOPIES * GEO::QB + ks * 256, own ? steps * 256 : HD * 16, own ? slot_low : GEO::QB, hs, hs < 2 && bl == 0);
                 }
               }
 #pragma unroll
@@ -617,7 +634,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const int tok = first + mt * 16 + (e >> 1) * 8 + place<FP4>(g);
-                  if (!far_any || prow[n][e & 1] - tok <= p.a.cap) s[mt][n][e] = acc[n][e];
+                  if (!far_any || prow[n][e & 1] - tok <= p.a.cap) s[mt][n][e] = joined(acc, n, e);
                 }
             }
           }

@@ -66,11 +66,15 @@ template <typename T>
 __device__ __forceinline__ double range_sum(const Weights<T>& w, int lo, int hi, int lane) {
   double s0 = 0.0, s1 = 0.0;
   int j = lo + lane * 4;
-  for (; j + 128 + 3 < hi; j += 256) {       // two independent groups in flight
-    double a[4], b[4];
-    w.four(j, a); w.four(j + 128, b);
-    s0 += (a[0] + a[1]) + (a[2] + a[3]);
-    s1 += (b[0] + b[1]) + (b[2] + b[3]);
+  for (; j + 3 * 128 + 3 < hi; j += 4 * 128) {       // four independent groups in flight
+    double a[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.four(j + 128 * i, a[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      s0 += (a[i][0] + a[i][1]) + (a[i][2] + a[i][3]);
+      s1 += (a[i + 1][0] + a[i + 1][1]) + (a[i + 1][2] + a[i + 1][3]);
+    }
   }
   for (; j < hi; j += 128) {
     if (j + 3 < hi) { double a[4]; w.four(j, a); s0 += (a[0] + a[1]) + (a[2] + a[3]); }
@@ -157,29 +161,47 @@ __global__ void __launch_bounds__(VWARPS * 32) verify_drafts_kernel(VerifyArgs a
   const int ranges = CL * VWARPS, mine = rank * VWARPS + warp;
   const int per = ((a.V + ranges - 1) / ranges + 3) & ~3;
   const int lo = min(a.V, mine * per), hi = min(a.V, lo + per);
-  double total = 0.0;
+  double total = 0.0, t4[4], ahead = 0.0;
   int phase = 0;
   for (; phase < 2; ++phase) {
     const double s = range_sum(w, lo, hi, lane);
     if (phase == 0) cluster.barrier_wait();
     if (lane < CL) *cluster.map_shared_rank(&totals[phase][mine], lane) = s;
     cluster.sync();
-    total = 0.0;
-    for (int i = 0; i < ranges; ++i) total += totals[phase][i];
+    // four ranges a lane (there are at most 128): their sums, and by a scan over the lanes what lies before them
+    double mine4 = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { t4[i] = 4 * lane + i < ranges ? totals[phase][4 * lane + i] : 0.0; mine4 += t4[i]; }
+    double upto = mine4;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const double up = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += up; }
+    ahead = __shfl_up_sync(0xffffffffu, upto, 1);
+    if (lane == 0) ahead = 0.0;
+    total = __shfl_sync(0xffffffffu, upto, 31);
     if (total > 0.0 || !refused) break;
     w.q = nullptr; w.x = -1;             // the residual is zero everywhere: the target itself (every CTA sees the same totals)
   }
-  phase = min(phase, 1);
+  // the first range at whose end the running sum exceeds the threshold (every warp finds the same); the last one of positive weight
+  // where rounding leaves none
   const double thr = static_cast<double>(a.u_sample[b]) * total;
-  int owner = -1, last = -1;
-  double run = 0.0, before = 0.0, before_last = 0.0;
-  for (int i = 0; i < ranges; ++i) {
-    const double t = totals[phase][i];
-    if (t > 0.0) { last = i; before_last = run; }
-    if (owner < 0 && run + t > thr) { owner = i; before = run; }
-    run += t;
+  int owner = ranges, last = -1;
+  double before = 0.0, before_last = 0.0, run = ahead;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (t4[i] > 0.0) { last = 4 * lane + i; before_last = run; }
+    if (owner == ranges && run + t4[i] > thr) { owner = 4 * lane + i; before = run; }
+    run += t4[i];
   }
-  if (owner < 0) { owner = last; before = before_last; }
+  const unsigned hits = __ballot_sync(0xffffffffu, owner < ranges), lives = __ballot_sync(0xffffffffu, last >= 0);
+  if (hits) {
+    owner = __shfl_sync(0xffffffffu, owner, __ffs(hits) - 1);
+    before = __shfl_sync(0xffffffffu, before, __ffs(hits) - 1);
+  } else if (lives) {
+    owner = __shfl_sync(0xffffffffu, last, 31 - __clz(lives));
+    before = __shfl_sync(0xffffffffu, before_last, 31 - __clz(lives));
+  } else {
+    owner = -1;
+  }
   long* out = a.tokens + static_cast<long>(b) * (a.N + 1);
   if (owner == mine) {
     const int pick = range_pick(w, lo, hi, before, thr, lane);
@@ -198,7 +220,9 @@ __global__ void __launch_bounds__(VWARPS * 32) verify_drafts_kernel(VerifyArgs a
 int verify_drafts(const VerifyArgs& a, cudaStream_t st) {
   if (a.B == 0) return 0;
   if (a.V < 1 || a.N < 0 || a.B > 0x7fffffff / VMAXCL) return 1;
-  const int cl = a.V >= 8192 ? VMAXCL : 1;
+  // CTAs a row: as many as keep the grid within two an SM (one wave), each with some hundreds of probabilities a warp
+  int cl = 1;
+  while (cl < VMAXCL && a.V >= 2 * cl * 4096 && static_cast<long>(a.B) * cl * 2 <= 296) cl *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.B * cl);
   cfg.blockDim = dim3(VWARPS * 32);
