@@ -141,7 +141,7 @@ struct PagedAttn {
   int Hq; float scale; bool fill;
 };
 // Work space of one call: floats of partial results and ints of their descriptions (both may be 0 long).
-struct PagedAttnPlan { int nt, ctas; long ws_floats, ws_ints; };
+struct PagedAttnPlan { int ctas; long ws_floats, ws_ints; };
 int paged_attention_plan(const PagedRows& r, const PagedPool& c, int Hq, int sms, PagedAttnPlan* plan);
 int paged_attention(const PagedRows& r, const PagedPool& c, const PagedAttn& a, const PagedAttnPlan& plan, float* ws, int* meta, cudaStream_t st);
 struct VerifyArgs {

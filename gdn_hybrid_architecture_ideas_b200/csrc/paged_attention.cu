@@ -39,22 +39,20 @@ struct AttnK {                       // by value to the kernels
   float* ws; int* meta;
 };
 
-// W warps, ST ring stages each, CTAS a SM, MT 16-position tiles a warp takes at once. Blocks of more query rows need more
-// registers, so fewer warps.
-template <bool FP4, int HD, int NT> struct Cfg;
-template <> struct Cfg<true, 64, 1> { static constexpr int W = 8, ST = 2, CTAS = 2, MT = 4; };
-template <> struct Cfg<true, 64, 3> { static constexpr int W = 12, ST = 4, CTAS = 1, MT = 2; };
-template <> struct Cfg<true, 128, 1> { static constexpr int W = 8, ST = 2, CTAS = 2, MT = 2; };
-template <> struct Cfg<true, 128, 2> { static constexpr int W = 12, ST = 3, CTAS = 1, MT = 2; };
-template <int NT> struct Cfg<true, 256, NT> { static constexpr int W = 8, ST = 2, CTAS = 1, MT = 2; };
-template <> struct Cfg<false, 64, 1> { static constexpr int W = 8, ST = 3, CTAS = 2, MT = 1; };
-template <> struct Cfg<false, 64, 3> { static constexpr int W = 8, ST = 3, CTAS = 1, MT = 1; };
-template <int NT> struct Cfg<false, 128, NT> { static constexpr int W = 4, ST = 3, CTAS = 2, MT = 1; };
-template <int NT> struct Cfg<false, 256, NT> { static constexpr int W = NT == 1 ? 6 : 4, ST = 2, CTAS = 1, MT = 1; };
+// W warps, ST ring stages each, CTAS a SM, MT 16-position tiles a warp takes at once.
+template <bool FP4, int HD> struct Cfg;
+template <> struct Cfg<true, 64> { static constexpr int W = 8, ST = 2, CTAS = 2, MT = 4; };
+template <> struct Cfg<true, 128> { static constexpr int W = 8, ST = 2, CTAS = 2, MT = 2; };
+template <> struct Cfg<true, 256> { static constexpr int W = 8, ST = 2, CTAS = 1, MT = 2; };
+template <> struct Cfg<false, 64> { static constexpr int W = 8, ST = 3, CTAS = 2, MT = 1; };
+template <> struct Cfg<false, 128> { static constexpr int W = 4, ST = 3, CTAS = 2, MT = 1; };
+template <> struct Cfg<false, 256> { static constexpr int W = 6, ST = 2, CTAS = 1, MT = 1; };
 
-template <bool FP4, int HD, int NT>
-struct Geo : Cfg<FP4, HD, NT> {
-  using B = Cfg<FP4, HD, NT>;
+constexpr int UNIT_ROWS = 8;         // query rows of a unit: the products' columns
+
+template <bool FP4, int HD>
+struct Geo : Cfg<FP4, HD> {
+  using B = Cfg<FP4, HD>;
   static constexpr int MT = B::MT, ST = B::ST;
   static constexpr int TILE = 16 * MT;
   static constexpr int H = HD / 64;                  // 64-channel slices
@@ -63,19 +61,19 @@ struct Geo : Cfg<FP4, HD, NT> {
   static constexpr int KB = TILE * ROW;              // bytes of a tile's keys (values the same)
   static constexpr int SB = FP4 ? TILE * S : 0;      // bytes of its scales
   static constexpr int STAGE = 2 * KB + 2 * SB;
-  static constexpr int UR = 8 * NT;                  // query rows of a unit
+  static constexpr int UR = UNIT_ROWS;
   static constexpr int PIECE = B::W * TILE;
   static constexpr int RING = B::W * ST * STAGE;
   static constexpr int MERGE = B::W * UR * HD * 4;
   // Partial outputs beside the ring, where both fit twice on an SM: the next unit's first tiles are then on their way while the
   // warps of this one join. Else over it.
-  static constexpr bool BESIDE = FP4 && NT == 1 && HD == 64;
+  static constexpr bool BESIDE = FP4 && HD == 64;
   static constexpr int DATA = BESIDE ? RING + MERGE : RING > MERGE ? RING : MERGE;
   static constexpr int QCOPIES = FP4 ? 1 : 2;        // bfloat16: high and low part
   static constexpr int QB = UR * HD * 2;             // bytes of one copy of the queries
   // under a cap: near and far queries, the near ones' rotary channels in float32 and as each warp rotated them, a tile of rotations
   __host__ __device__ static constexpr int q_bytes(bool cap) { return (cap ? 2 : 1) * QCOPIES * QB; }
-  __host__ __device__ static constexpr int turned_bytes(int half) { return NT * (half / 8) * 256 * QCOPIES; }      // of a warp
+  __host__ __device__ static constexpr int turned_bytes(int half) { return (half / 8) * 256 * QCOPIES; }      // of a warp
   __host__ __device__ static constexpr int smem(int cap_half) {
     return DATA + q_bytes(cap_half > 0) + UR * 2 * cap_half * 4 + TILE * cap_half * 8 + B::W * turned_bytes(cap_half);
   }
@@ -169,15 +167,32 @@ template <bool FP4> __device__ __forceinline__ int place(int rho) {
   return FP4 ? (rho & 4) | (((rho ^ (rho >> 2)) & 1) << 1) | ((rho >> 1) & 1) : rho;
 }
 
-// The units of a row: how many for a head, and how many pieces each.
-struct RowWork { int units, pieces, base; };
-template <typename GEO>
-__device__ __forceinline__ RowWork row_work(const Row& row, int G) {
-  RowWork w;
+// The units of a row: how many for a head, how many pieces each, and what a unit costs. Under a cap, pieces with keys to rotate count
+// 3 where the others, which come first, count 2 (618 against 408 instructions for 32 positions).
+template <bool CAP>
+struct RowWork {
+  static constexpr int FAR = CAP ? 2 : 1, NEAR = CAP ? 3 : 1;
+  int units, pieces, base, far;              // far: leading pieces that lie beyond the cap for every new token
+  __device__ __forceinline__ long cost() const { return static_cast<long>(far) * FAR + static_cast<long>(pieces - far) * NEAR; }
+  __device__ __forceinline__ long cost_at(int piece) const { return piece < far ? static_cast<long>(piece) * FAR : static_cast<long>(far) * FAR + static_cast<long>(piece - far) * NEAR; }
+  // the first piece that starts at a cost of c or more
+  __device__ __forceinline__ int piece_at(long c) const {
+    const long f = static_cast<long>(far) * FAR;
+    return static_cast<int>(c <= f ? (c + FAR - 1) / FAR : far + (c - f + NEAR - 1) / NEAR);
+  }
+};
+template <typename GEO, bool CAP>
+__device__ __forceinline__ RowWork<CAP> row_work(const Row& row, int G, int cap) {
+  RowWork<CAP> w;
   w.units = (row.nq * G + GEO::UR - 1) / GEO::UR;
   w.base = row.start & ~(GEO::TILE - 1);
   const int span = row.len - w.base;
   w.pieces = span > 0 ? (span + GEO::PIECE - 1) / GEO::PIECE : 1;      // a row that sees nothing still owes zeros
+  w.far = 0;
+  if (CAP) {
+    const int beyond = row.len - row.nq - cap - w.base;                // positions beyond the cap of the first new token
+    w.far = beyond > 0 ? min(beyond / GEO::PIECE, w.pieces) : 0;
+  }
   return w;
 }
 
@@ -197,9 +212,9 @@ __device__ __forceinline__ long block_scan(long x, long* s_warp, long* total) {
   return before + inc - x;      // exclusive
 }
 
-template <bool FP4, int HD, int NT, bool CAP>
-__global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::CTAS) paged_attention_kernel(const __grid_constant__ AttnK p) {
-  using GEO = Geo<FP4, HD, NT>;
+template <bool FP4, int HD, bool CAP>
+__global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) paged_attention_kernel(const __grid_constant__ AttnK p) {
+  using GEO = Geo<FP4, HD>;
   constexpr int H = GEO::H, MT = GEO::MT, TILE = GEO::TILE, UR = GEO::UR, W = GEO::W, ST = GEO::ST;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long s_warp[W];
@@ -214,8 +229,8 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
   // ---- this CTA's share of the pieces
   auto pieces_of = [&](int i) -> long {
     if (i >= R.B) return 0;
-    const RowWork w = row_work<GEO>(load_row(R, i), G);
-    return static_cast<long>(w.units) * w.pieces * Hkv;
+    const RowWork<CAP> w = row_work<GEO, CAP>(load_row(R, i), G, p.a.cap);
+    return w.units * w.cost() * Hkv;
   };
   long total = 0, mine = 0, ex = 0;
   for (int b0 = 0; b0 < R.B; b0 += GEO::THREADS) {
@@ -224,7 +239,9 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     ex = total + block_scan<GEO::THREADS>(mine, s_warp, &all);
     total += all;
   }
-  const long use = total < n_ctas ? total : n_ctas;      // CTAs with work: at least one piece each
+  // CTAs with work: their shares are at least a piece's cost, so that each holds the start of one
+  const long most = total / RowWork<CAP>::NEAR;
+  const long use = most < 1 ? (total > 0) : most < n_ctas ? most : n_ctas;
   int* meta = p.meta + cta * 8;
   if (tid == 0) meta[0] = 0;                  // parts of the unit that this CTA begins and others end
   if (cta >= use) return;
@@ -262,31 +279,38 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
   }
 
   // ---- the part of a unit that this CTA does next
-  struct Part { int b, q0, start, h, r0, n_rows, p0, n_pieces, pieces, pos0, p_first, p_last, tile0; };
+  struct Part { int b, q0, start, h, r0, n_rows, p0, n_pieces, pieces, pos0, p_first, p_last, tile0; long last_cost; };
   long at = lo;
   Part sg;
-  auto locate = [&]() {
-    Row row = load_row(R, b);
-    RowWork wk = row_work<GEO>(row, G);
-    long count = static_cast<long>(wk.units) * wk.pieces * Hkv;
-    while (at >= row_at + count) {            // rows without tokens have no pieces
-      row_at += count;
-      ++b;
-      row = load_row(R, b);
-      wk = row_work<GEO>(row, G);
-      count = static_cast<long>(wk.units) * wk.pieces * Hkv;
+  // (at: where the part starts, in costs; its pieces are those that start in at .. hi. Moves at to the part's end; false: none left.)
+  auto locate = [&]() -> bool {
+    while (at < hi) {
+      const Row row = load_row(R, b);
+      const RowWork<CAP> wk = row_work<GEO, CAP>(row, G, p.a.cap);
+      const long each = wk.cost(), count = wk.units * each * Hkv;
+      if (at >= row_at + count) {             // (rows without tokens have no pieces)
+        row_at += count;
+        ++b;
+        continue;
+      }
+      const int unit = static_cast<int>((at - row_at) / each);
+      const long unit_at = row_at + unit * each;
+      sg.p0 = wk.piece_at(at - unit_at);
+      const int p1 = hi - unit_at >= each ? wk.pieces : wk.piece_at(hi - unit_at);
+      at = min(hi, unit_at + each);
+      if (p1 <= sg.p0) continue;
+      sg.b = b; sg.q0 = row.q0; sg.start = row.start; sg.pieces = wk.pieces;
+      sg.n_pieces = p1 - sg.p0;
+      sg.last_cost = unit_at + wk.cost_at(wk.pieces - 1);
+      sg.h = unit / wk.units; sg.r0 = (unit % wk.units) * UR;
+      sg.n_rows = min(UR, row.nq * G - sg.r0);
+      sg.pos0 = row.len - row.nq;                            // position of the row's first new token
+      sg.p_first = sg.pos0 + sg.r0 / G;
+      sg.p_last = row.len ? sg.pos0 + (sg.r0 + sg.n_rows - 1) / G : -1;
+      sg.tile0 = wk.base + sg.p0 * GEO::PIECE + warp * TILE;
+      return true;
     }
-    const long in_row = at - row_at;
-    const int unit = static_cast<int>(in_row / wk.pieces);
-    sg.b = b; sg.q0 = row.q0; sg.start = row.start; sg.pieces = wk.pieces;
-    sg.p0 = static_cast<int>(in_row % wk.pieces);
-    sg.n_pieces = static_cast<int>(min(static_cast<long>(wk.pieces - sg.p0), hi - at));
-    sg.h = unit / wk.units; sg.r0 = (unit % wk.units) * UR;
-    sg.n_rows = min(UR, row.nq * G - sg.r0);
-    sg.pos0 = row.len - row.nq;                              // position of the row's first new token
-    sg.p_first = sg.pos0 + sg.r0 / G;
-    sg.p_last = row.len ? sg.pos0 + (sg.r0 + sg.n_rows - 1) / G : -1;
-    sg.tile0 = wk.base + sg.p0 * GEO::PIECE + warp * TILE;
+    return false;
   };
   // ---- loads of one tile: positions tile0 + k PIECE .. + TILE. A tile is one or more chunks, each within a page and so contiguous
   // per head; all lanes copy 16 bytes at a time. Page ids are looked up for 32 chunks at once (32 tiles where a page holds a
@@ -370,7 +394,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
     for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k, k);
   };
-  locate();
+  if (!locate()) return;
   begin();
   while (true) {
     const int h = sg.h, r0 = sg.r0, n_rows = sg.n_rows, n_pieces = sg.n_pieces, pos0 = sg.pos0, p_first = sg.p_first, p_last = sg.p_last, tile0 = sg.tile0;
@@ -415,8 +439,8 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
         // the order of the plain products (a lane owns the 16 channels 16 t .. of each slice), and of the rotating ones (its
         // channels are 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16)
         const int cc = c & 63;
-        const int plain_at = ((((r >> 3) * (HD / 16) + (c >> 6) * 4 + ((cc & 15) >> 2)) * 32 + (r & 7) * 4 + (cc >> 4)) << 2) + (cc & 3);
-        const int near_at = ((((r >> 3) * (HD / 16) + (c >> 4)) * 32 + (r & 7) * 4 + ((c & 7) >> 1)) << 2) + ((c >> 2) & 2) + (c & 1);
+        const int plain_at = ((((c >> 6) * 4 + ((cc & 15) >> 2)) * 32 + r * 4 + (cc >> 4)) << 2) + (cc & 3);
+        const int near_at = (((c >> 4) * 32 + r * 4 + ((c & 7) >> 1)) << 2) + ((c >> 2) & 2) + (c & 1);
         auto put = [&](uint8_t* to, int idx, float v) {
           if constexpr (FP4) {
             reinterpret_cast<__half*>(to)[idx] = __float2half_rn(v);
@@ -436,25 +460,20 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     }
     __syncthreads();
 
-    const int live_n = NT == 1 ? 1 : (n_rows + 7) >> 3;        // 8-row column blocks in use
-    float mul[NT][2], m[NT][2], l[NT][4];       // l: the sums of the probabilities, as a product with ones (every row the same)
-    int prow[NT][2];
+    float mul[2], m[2], l[4];       // l: the sums of the probabilities, as a product with ones (every row the same)
+    int prow[2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = n * 8 + 2 * t + e;
-        mul[n][e] = s_mul[r];
-        prow[n][e] = r < n_rows && p_last >= 0 ? pos0 + (r0 + r) / G : -1;
-        m[n][e] = -INFINITY; l[n][e] = l[n][e + 2] = 0.f;
-      }
-    float o[H * 4][NT][4];
+    for (int e = 0; e < 2; ++e) {
+      const int r = 2 * t + e;
+      mul[e] = s_mul[r];
+      prow[e] = r < n_rows && p_last >= 0 ? pos0 + (r0 + r) / G : -1;
+      m[e] = -INFINITY; l[e] = l[e + 2] = 0.f;
+    }
+    float o[H * 4][4];
 #pragma unroll
     for (int i = 0; i < H * 4; ++i)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
     for (int k = 0; k < n_pieces; ++k) {
       const int first = tile0 + k * GEO::PIECE;
@@ -478,30 +497,26 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
           }
           __syncwarp();
         }
-        float s[MT][NT][4];
+        float s[MT][4];
         // Products that add into one accumulator wait for one another: wide heads take two by turns of their slices, bfloat16 two more
         // for the low parts, summed at the end (a head of 256 is 32 products otherwise in one chain).
         constexpr int CHAINS = (H > 1 ? 2 : 1) * GEO::QCOPIES;
-        // one k16 step of the 16 positions of tile mt against every column block; its queries start at qs, a block's at by bytes further
-        auto step = [&](float (&acc)[CHAINS][NT][4], const uint32_t* a, const uint8_t* qs, int by, int low, int hs, bool begin) {
+        // one k16 step of the 16 positions of tile mt against the queries' operand at qs (the low parts' `low` bytes further)
+        auto step = [&](float (&acc)[CHAINS][4], const uint32_t* a, const uint8_t* qs, int low, int hs, bool begin) {
           const int c = (H > 1 ? hs & 1 : 0) * GEO::QCOPIES;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (NT > 1 && n >= live_n) continue;
-            const uint2 q1 = *reinterpret_cast<const uint2*>(qs + n * by + lane * 8);
-            if (begin) mma_first<FP4>(acc[c][n], a, q1.x, q1.y);
-            else mma<FP4>(acc[c][n], a, q1.x, q1.y);
-            if constexpr (!FP4) {
-              const uint2 q2 = *reinterpret_cast<const uint2*>(qs + low + n * by + lane * 8);
-              if (begin) mma_first<FP4>(acc[c + 1][n], a, q2.x, q2.y);
-              else mma<FP4>(acc[c + 1][n], a, q2.x, q2.y);
-            }
+          const uint2 q1 = *reinterpret_cast<const uint2*>(qs + lane * 8);
+          if (begin) mma_first<FP4>(acc[c], a, q1.x, q1.y);
+          else mma<FP4>(acc[c], a, q1.x, q1.y);
+          if constexpr (!FP4) {
+            const uint2 q2 = *reinterpret_cast<const uint2*>(qs + low + lane * 8);
+            if (begin) mma_first<FP4>(acc[c + 1], a, q2.x, q2.y);
+            else mma<FP4>(acc[c + 1], a, q2.x, q2.y);
           }
         };
-        auto joined = [&](float (&acc)[CHAINS][NT][4], int n, int e) -> float {
-          float x = acc[0][n][e];
+        auto joined = [&](float (&acc)[CHAINS][4], int e) -> float {
+          float x = acc[0][e];
 #pragma unroll
-          for (int c = 1; c < CHAINS; ++c) x += acc[c][n][e];
+          for (int c = 1; c < CHAINS; ++c) x += acc[c][e];
           return x;
         };
         const bool far_any = !CAP || p_last - first > p.a.cap;                     // some (row, position) beyond the cap
@@ -510,7 +525,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
           // ---- keys as cached: a lane owns 16 consecutive channels of a slice (4 bits: one block)
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            float acc[CHAINS][NT][4];
+            float acc[CHAINS][4];
 #pragma unroll
             for (int hs = 0; hs < H; ++hs) {
               uint32_t x[2][8];                // [row g or g + 8][channel pair]: channels 16 t + 2 i of slice hs
@@ -535,13 +550,11 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
               for (int ks = 0; ks < 4; ++ks) {
                 const uint32_t a[4] = {x[0][2 * ks], x[1][2 * ks], x[0][2 * ks + 1], x[1][2 * ks + 1]};
-                step(acc, a, sq + (hs * 4 + ks) * 256, HD * 16, GEO::QB, hs, hs < 2 && (hs == 0 || H > 1) && ks == 0);
+                step(acc, a, sq + (hs * 4 + ks) * 256, GEO::QB, hs, hs < 2 && ks == 0);
               }
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[mt][n][e] = joined(acc, n, e);
+            for (int e = 0; e < 4; ++e) s[mt][e] = joined(acc, e);
           }
         }
         if constexpr (CAP) {
@@ -551,15 +564,12 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             // 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16, so that both channels of a rotary pair (half 8, 16 or 32
             // apart) are its own.
             const int t0 = max(first, start);
-            const int steps = half >> 3, slot_low = NT * steps * 256;          // rotary k16 steps; bytes of the high parts
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              if (NT > 1 && n >= live_n) continue;
-              const int r = n * 8 + g;
-              const long d = max(0, min(s_pos[r] - t0, p.a.n_pos - 1));
+            const int steps = half >> 3, slot_low = steps * 256;          // rotary k16 steps; bytes of the high parts
+            {
+              const long d = max(0, min(s_pos[g] - t0, p.a.n_pos - 1));
               const float* co = p.a.cos + d * half + 2 * t;
               const float* si = p.a.sin + d * half + 2 * t;
-              const float* qb = sq_base + r * 2 * half + 2 * t;
+              const float* qb = sq_base + g * 2 * half + 2 * t;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 if (i >= steps) break;
@@ -567,7 +577,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
                 const float2 u = *reinterpret_cast<const float2*>(qb + 8 * i), v = *reinterpret_cast<const float2*>(qb + half + 8 * i);
                 const float2 a = make_float2(u.x * c.x - v.x * sn.x, u.y * c.y - v.y * sn.y), z = make_float2(v.x * c.x + u.x * sn.x, v.y * c.y + u.y * sn.y);
                 auto put = [&](int eight, float2 x) {         // group of 8 channels -> (step, register) of this lane
-                  uint8_t* to = s_turned + (n * steps + (eight >> 1)) * 256 + lane * 8 + (eight & 1) * 4;
+                  uint8_t* to = s_turned + (eight >> 1) * 256 + lane * 8 + (eight & 1) * 4;
                   const uint32_t hi = pack<FP4>(x.x, x.y);
                   *reinterpret_cast<uint32_t*>(to) = hi;
                   if constexpr (!FP4) {
@@ -581,7 +591,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             }
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              float acc[CHAINS][NT][4];
+              float acc[CHAINS][4];
 #pragma unroll
               for (int hs = 0; hs < H; ++hs) {
                 uint32_t x[2][4][2];           // [row][block of the slice][channels 2 t.. or 2 t + 8 ..]
@@ -626,16 +636,14 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
                   const uint32_t a[4] = {x[0][bl][0], x[1][bl][0], x[0][bl][1], x[1][bl][1]};
                   const int ks = hs * 4 + bl;
                   const bool own = hs == 0 && bl < steps;
-                  step(acc, a, own ? s_turned + ks * 256 : sq + GEO::QCOPIES * GEO::QB + ks * 256, own ? steps * 256 : HD * 16, own ? slot_low : GEO::QB, hs, hs < 2 && bl == 0);
+                  step(acc, a, own ? s_turned + ks * 256 : sq + GEO::QCOPIES * GEO::QB + ks * 256, own ? slot_low : GEO::QB, hs, hs < 2 && bl == 0);
                 }
               }
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int tok = first + mt * 16 + (e >> 1) * 8 + place<FP4>(g);
-                  if (!far_any || prow[n][e & 1] - tok <= p.a.cap) s[mt][n][e] = joined(acc, n, e);
-                }
+              for (int e = 0; e < 4; ++e) {
+                const int tok = first + mt * 16 + (e >> 1) * 8 + place<FP4>(g);
+                if (!far_any || prow[e & 1] - tok <= p.a.cap) s[mt][e] = joined(acc, e);
+              }
             }
           }
         }
@@ -645,59 +653,45 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int pos = mt * 16 + (e >> 1) * 8 + place<FP4>(g);
-                if (!((on >> (pos >> c_shift)) & 1) || first + pos < start || first + pos > prow[n][e & 1]) s[mt][n][e] = -INFINITY;
-              }
+            for (int e = 0; e < 4; ++e) {
+              const int pos = mt * 16 + (e >> 1) * 8 + place<FP4>(g);
+              if (!((on >> (pos >> c_shift)) & 1) || first + pos < start || first + pos > prow[e & 1]) s[mt][e] = -INFINITY;
+            }
         }
         // ---- the reference of the exponents, where a score leaves the slack (raw scores: the factor is positive)
-        float mx[NT][2];
+        float mx[2];
         bool grew = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (NT > 1 && n >= live_n) continue;
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(s[0][e], s[0][e + 2]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(s[0][n][e], s[0][n][e + 2]);
-#pragma unroll
-            for (int mt = 1; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][n][e], s[mt][n][e + 2]));
-            mx[n][e] = x * mul[n][e];
-            grew |= mx[n][e] > m[n][e] + SLACK;
-          }
+          for (int mt = 1; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][e], s[mt][e + 2]));
+          mx[e] = x * mul[e];
+          grew |= mx[e] > m[e] + SLACK;
         }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (NT > 1 && n >= live_n) continue;
+          for (int e = 0; e < 2; ++e) {
+            float x = mx[e];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float mn = fmaxf(m[e], x);
+            const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m[e] - mn);
+            m[e] = mn;
+            l[e] *= alpha; l[e + 2] *= alpha;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = mx[n][e];
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-              const float mn = fmaxf(m[n][e], x);
-              const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m[n][e] - mn);
-              m[n][e] = mn;
-              l[n][e] *= alpha; l[n][e + 2] *= alpha;
-#pragma unroll
-              for (int i = 0; i < H * 4; ++i) { o[i][n][e] *= alpha; o[i][n][e + 2] *= alpha; }
-            }
+            for (int i = 0; i < H * 4; ++i) { o[i][e] *= alpha; o[i][e + 2] *= alpha; }
           }
         }
         // ---- probabilities
-        uint32_t pk[MT][NT][2];
+        uint32_t pk[MT][2];
+        const float ref0 = (m[0] == -INFINITY ? 0.f : -m[0]) + (FP4 ? PSHIFT : 0.f), ref1 = (m[1] == -INFINITY ? 0.f : -m[1]) + (FP4 ? PSHIFT : 0.f);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (NT > 1 && n >= live_n) continue;
-          const float r0 = (m[n][0] == -INFINITY ? 0.f : -m[n][0]) + (FP4 ? PSHIFT : 0.f), r1 = (m[n][1] == -INFINITY ? 0.f : -m[n][1]) + (FP4 ? PSHIFT : 0.f);
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-              pk[mt][n][q] = pack<FP4>(exp2_fast(fmaf(s[mt][n][2 * q], mul[n][0], r0)), exp2_fast(fmaf(s[mt][n][2 * q + 1], mul[n][1], r1)));
-        }
+          for (int q = 0; q < 2; ++q)
+            pk[mt][q] = pack<FP4>(exp2_fast(fmaf(s[mt][2 * q], mul[0], ref0)), exp2_fast(fmaf(s[mt][2 * q + 1], mul[1], ref1)));
         // ---- O^T += V^T P^T
         bool plain = true;
         if constexpr (!FP4) {
@@ -715,27 +709,22 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
             plain = !__any_sync(0xffffffffu, odd);
           }
           if (!plain) {
-            auto see = [&](int j, int n, int e) { return first + j >= start && first + j <= prow[n][e]; };
             for (int j = 0; j < TILE; ++j) {
-              if (!((on >> (j >> c_shift)) & 1)) continue;
+              if (!((on >> (j >> c_shift)) & 1) || first + j < start) continue;
+              const float2 pp = unpack<FP4>(__shfl_sync(0xffffffffu, j < 8 ? pk[0][0] : pk[0][1], (j & 7) * 4 + t));
+              const bool see0 = first + j <= prow[0], see1 = first + j <= prow[1];
+              if (see0) { l[0] += pp.x; l[2] += pp.x; }
+              if (see1) { l[1] += pp.y; l[3] += pp.y; }
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const float2 pp = unpack<FP4>(__shfl_sync(0xffffffffu, j < 8 ? pk[0][n][0] : pk[0][n][1], (j & 7) * 4 + t));
-                const float p0 = pp.x, p1 = pp.y;
-                if (see(j, n, 0)) { l[n][0] += p0; l[n][2] += p0; }
-                if (see(j, n, 1)) { l[n][1] += p1; l[n][3] += p1; }
-                const bool see0 = see(j, n, 0), see1 = see(j, n, 1);
+              for (int hs = 0; hs < H; ++hs) {
+                const uint4 w = *reinterpret_cast<const uint4*>(st + GEO::KB + hs * (TILE * 128) + j * 128 + ((g ^ (j & 7)) << 4));
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int hs = 0; hs < H; ++hs) {
-                  const uint4 w = *reinterpret_cast<const uint4*>(st + GEO::KB + hs * (TILE * 128) + j * 128 + ((g ^ (j & 7)) << 4));
-                  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const float2 v = unpack<FP4>(ws[i]);
-                    float* oo = o[hs * 4 + i][n];
-                    if (see0) { oo[0] += p0 * v.x; oo[2] += p0 * v.y; }
-                    if (see1) { oo[1] += p1 * v.x; oo[3] += p1 * v.y; }
-                  }
+                for (int i = 0; i < 4; ++i) {
+                  const float2 v = unpack<FP4>(ws[i]);
+                  float* oo = o[hs * 4 + i];
+                  if (see0) { oo[0] += pp.x * v.x; oo[2] += pp.x * v.y; }
+                  if (see1) { oo[1] += pp.y * v.x; oo[3] += pp.y * v.y; }
                 }
               }
             }
@@ -744,14 +733,10 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
         if (plain) {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            uint32_t pb[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              if (NT > 1 && n >= live_n) continue;
-              pb[n][0] = transpose8(pk[mt][n][0]); pb[n][1] = transpose8(pk[mt][n][1]);
-              const uint32_t ones[4] = {FP4 ? 0x3c003c00u : 0x3f803f80u, FP4 ? 0x3c003c00u : 0x3f803f80u, FP4 ? 0x3c003c00u : 0x3f803f80u, FP4 ? 0x3c003c00u : 0x3f803f80u};
-              mma<FP4>(l[n], ones, pb[n][0], pb[n][1]);
-            }
+            const uint32_t pb[2] = {transpose8(pk[mt][0]), transpose8(pk[mt][1])};
+            constexpr uint32_t ONE2 = FP4 ? 0x3c003c00u : 0x3f803f80u;
+            const uint32_t ones[4] = {ONE2, ONE2, ONE2, ONE2};
+            mma<FP4>(l, ones, pb[0], pb[1]);
             const int u0 = mt * 16 + place<FP4>(2 * t), u1 = mt * 16 + place<FP4>(2 * t + 1);
 #pragma unroll
             for (int hs = 0; hs < H; ++hs) {
@@ -790,12 +775,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
                 }
               }
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  if (NT > 1 && n >= live_n) continue;
-                  mma<FP4>(o[hs * 4 + i][n], a4[i], pb[n][0], pb[n][1]);
-                }
+              for (int i = 0; i < 4; ++i) mma<FP4>(o[hs * 4 + i], a4[i], pb[0], pb[1]);
             }
           }
         }
@@ -808,21 +788,18 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
     // ---- join the warps
     float* so = reinterpret_cast<float*>(smem + (GEO::BESIDE ? GEO::RING : 0));
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int e = 0; e < 2; ++e) {
+      const int r = 2 * t + e;
+      if (g == 0) { s_m[warp][r] = m[e]; s_l[warp][r] = l[e]; }
+      float* dst = so + (static_cast<long>(warp) * UR + r) * HD + 8 * g;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = n * 8 + 2 * t + e;
-        if (g == 0) { s_m[warp][r] = m[n][e]; s_l[warp][r] = l[n][e]; }
-        float* dst = so + (static_cast<long>(warp) * UR + r) * HD + 8 * g;
-#pragma unroll
-        for (int i = 0; i < H * 4; ++i)
-          *reinterpret_cast<float2*>(dst + (i >> 2) * 64 + (i & 3) * 2) = make_float2(o[i][n][e], o[i][n][e + 2]);
-      }
-    const long first_piece = at;
-    at += n_pieces;
-    const bool more = at < hi;
+      for (int i = 0; i < H * 4; ++i)
+        *reinterpret_cast<float2*>(dst + (i >> 2) * 64 + (i & 3) * 2) = make_float2(o[i][e], o[i][e + 2]);
+    }
+    const long last_cost = sg.last_cost;
+    const bool more = locate();                // (the next part, from here on)
     if (!more) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if constexpr (GEO::BESIDE) { if (more) { locate(); begin(); } }
+    if (GEO::BESIDE && more) begin();
     __syncthreads();
     const bool begins = p0 == 0, ends = p0 + n_pieces == pieces;
     const int slot = begins ? 1 : 0;
@@ -851,14 +828,12 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
       }
     }
     if (tid == 0 && begins && !ends) {           // the first part: how many CTAs hold the others follows from the shares
-      const long last = first_piece + pieces - 1;      // the unit's last piece
       meta[1] = h; meta[2] = r0; meta[3] = n_rows; meta[4] = q0;
-      meta[0] = static_cast<int>(((last + 1) * use - 1) / total) - cta + 1;
+      meta[0] = static_cast<int>(((last_cost + 1) * use - 1) / total) - cta + 1;
     }
     if (!more) break;
     if constexpr (!GEO::BESIDE) {
       __syncthreads();
-      locate();
       begin();
     }
   }
@@ -867,9 +842,9 @@ __global__ void __launch_bounds__(Geo<FP4, HD, NT>::THREADS, Geo<FP4, HD, NT>::C
 // Joins the parts of every unit that CTA borders cut: part one is the last thing its first CTA did (slot 1), the others are the
 // first thing that the following CTAs did (slot 0). Block (i, r) joins query row r of the unit whose first part CTA i holds. Also the zeros of
 // the packed tokens behind the last row, where the output is this call's own.
-template <int HD, int UR>
+template <int HD>
 __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_constant__ AttnK p, int n_ctas) {
-  constexpr int LANES = HD / 4, GROUPS = 256 / LANES;
+  constexpr int LANES = HD / 4, GROUPS = 256 / LANES, UR = UNIT_ROWS;
   __shared__ float4 s_o[GROUPS][LANES];
   __shared__ float s_m[GROUPS], s_l[GROUPS];
   const int i = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
@@ -925,19 +900,19 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_
 
 namespace {
 
-template <bool FP4, int HD, int NT, bool CAP>
+template <bool FP4, int HD, bool CAP>
 int launch(const AttnK& k, int ctas, cudaStream_t st) {
-  using GEO = Geo<FP4, HD, NT>;
+  using GEO = Geo<FP4, HD>;
   const int bytes = GEO::smem(CAP ? k.a.half : 0);
   // (the largest size this kernel can ask for, set once per device)
   static std::atomic<uint64_t> ready[4];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 4;
   if (dev > 255 || !(ready[dev >> 6].load(std::memory_order_acquire) >> (dev & 63) & 1)) {
-    if (cudaFuncSetAttribute(paged_attention_kernel<FP4, HD, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEO::smem(CAP ? 32 : 0)) != cudaSuccess) return 4;
+    if (cudaFuncSetAttribute(paged_attention_kernel<FP4, HD, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEO::smem(CAP ? 32 : 0)) != cudaSuccess) return 4;
     if (dev <= 255) ready[dev >> 6].fetch_or(uint64_t(1) << (dev & 63), std::memory_order_release);
   }
-  paged_attention_kernel<FP4, HD, NT, CAP><<<ctas, GEO::THREADS, bytes, st>>>(k);
+  paged_attention_kernel<FP4, HD, CAP><<<ctas, GEO::THREADS, bytes, st>>>(k);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, GEO::UR);
   cfg.blockDim = dim3(256);
@@ -947,56 +922,41 @@ int launch(const AttnK& k, int ctas, cudaStream_t st) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<HD, GEO::UR>, k, ctas) != cudaSuccess) return 4;
+  if (cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<HD>, k, ctas) != cudaSuccess) return 4;
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
-template <bool FP4, int HD, int NT>
-int launch(const AttnK& k, int ctas, cudaStream_t st) {
-  return k.a.cap ? launch<FP4, HD, NT, true>(k, ctas, st) : launch<FP4, HD, NT, false>(k, ctas, st);
-}
-
-struct Shape { int ctas, ur, piece; };
-template <bool FP4, int HD, int NT> Shape shape() { using GEO = Geo<FP4, HD, NT>; return {GEO::CTAS, GEO::UR, GEO::PIECE}; }
+template <bool FP4, int HD>
+int launch(const AttnK& k, int ctas, cudaStream_t st) { return k.a.cap ? launch<FP4, HD, true>(k, ctas, st) : launch<FP4, HD, false>(k, ctas, st); }
 
 template <bool FP4>
-bool shape_of(int hd, int nt, Shape* s) {
-  if (hd == 64) { *s = nt == 1 ? shape<FP4, 64, 1>() : shape<FP4, 64, 3>(); return nt == 1 || nt == 3; }
-  if (hd == 128) { *s = nt == 1 ? shape<FP4, 128, 1>() : shape<FP4, 128, 2>(); return nt <= 2; }
-  if (hd == 256) { *s = nt == 1 ? shape<FP4, 256, 1>() : shape<FP4, 256, 2>(); return nt <= 2; }
-  return false;
-}
-
-template <bool FP4>
-int dispatch(const AttnK& k, int hd, const PagedAttnPlan& plan, cudaStream_t st) {
-  switch (hd * 8 + plan.nt) {
-    case 64 * 8 + 1: return launch<FP4, 64, 1>(k, plan.ctas, st);
-    case 64 * 8 + 3: return launch<FP4, 64, 3>(k, plan.ctas, st);
-    case 128 * 8 + 1: return launch<FP4, 128, 1>(k, plan.ctas, st);
-    case 128 * 8 + 2: return launch<FP4, 128, 2>(k, plan.ctas, st);
-    case 256 * 8 + 1: return launch<FP4, 256, 1>(k, plan.ctas, st);
-    case 256 * 8 + 2: return launch<FP4, 256, 2>(k, plan.ctas, st);
+int dispatch(const AttnK& k, int hd, int ctas, cudaStream_t st) {
+  switch (hd) {
+    case 64: return launch<FP4, 64>(k, ctas, st);
+    case 128: return launch<FP4, 128>(k, ctas, st);
+    case 256: return launch<FP4, 256>(k, ctas, st);
   }
   return 1;
 }
 
+struct Shape { int ctas, piece; };
+template <bool FP4, int HD> Shape shape() { using GEO = Geo<FP4, HD>; return {GEO::CTAS, GEO::PIECE}; }
+template <bool FP4> Shape shape_of(int hd) { return hd == 64 ? shape<FP4, 64>() : hd == 128 ? shape<FP4, 128>() : shape<FP4, 256>(); }
+
 }  // namespace
 
-// How many query rows a unit has: 8 where that holds the rows' average (a decode step), else 24 (16 for wide heads), of which
-// only the blocks of 8 in use are computed; and how many CTAs run: as many as are resident, fewer where even full
-// tables have fewer pieces.
+// How many CTAs run: as many as are resident, fewer where even full tables have fewer pieces. A unit is always 8 query rows: units of
+// 16 and 24, which convert each entry once for more rows, were measured and are slower (24 rows of up to 5 drafts, 32 heads over 8:
+// 94 us against 65; of up to 16: 212 against 162), because their accumulators leave room for fewer warps and shorter tiles.
 int paged_attention_plan(const PagedRows& r, const PagedPool& c, int Hq, int sms, PagedAttnPlan* plan) {
+  if (c.hd != 64 && c.hd != 128 && c.hd != 256) return 1;
   const int G = Hq / r.Hkv;
-  const long per_row = r.B ? static_cast<long>(G) * ((r.n + r.B - 1) / r.B) : 0;
-  const int nt = per_row <= 8 ? 1 : c.hd == 64 ? 3 : 2;
-  Shape s;
-  if (!(c.fp4 ? shape_of<true>(c.hd, nt, &s) : shape_of<false>(c.hd, nt, &s))) return 1;
-  const long units = (static_cast<long>(r.n) * G / s.ur + r.B) * r.Hkv;
+  const Shape s = c.fp4 ? shape_of<true>(c.hd) : shape_of<false>(c.hd);
+  const long units = (static_cast<long>(r.n) * G / UNIT_ROWS + r.B) * r.Hkv;
   const long pieces = ((static_cast<long>(r.width) << r.page_shift) / s.piece + 2) * units;
   long ctas = static_cast<long>(sms) * s.ctas;
   if (pieces < ctas) ctas = pieces;
-  plan->nt = nt;
   plan->ctas = ctas < 1 ? 1 : static_cast<int>(ctas);
-  plan->ws_floats = static_cast<long>(plan->ctas) * 2 * s.ur * (c.hd + 2);
+  plan->ws_floats = static_cast<long>(plan->ctas) * 2 * UNIT_ROWS * (c.hd + 2);
   plan->ws_ints = static_cast<long>(plan->ctas) * 8;
   return 0;
 }
@@ -1007,7 +967,7 @@ int paged_attention(const PagedRows& r, const PagedPool& c, const PagedAttn& a, 
   // rotating cached keys: pairs within the first 64 channels, whole lanes apart
   if (a.cap && a.half != 8 && a.half != 16 && a.half != 32) return 1;
   AttnK k{r, c, a, a.Hq / r.Hkv, ws, meta};
-  return c.fp4 ? dispatch<true>(k, c.hd, plan, st) : dispatch<false>(k, c.hd, plan, st);
+  return c.fp4 ? dispatch<true>(k, c.hd, plan.ctas, st) : dispatch<false>(k, c.hd, plan.ctas, st);
 }
 
 }  // namespace ghb
