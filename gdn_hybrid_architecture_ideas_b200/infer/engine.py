@@ -11,6 +11,9 @@ batch size with fixed-shape state:
   cache, ced/model/attention.py:943-1030: a 4 x 4 grid of 32-channel components holds 256 channels per token, the
   same bytes as 4 grouped KV heads); the key norm over the assembled head and the rotation are applied while scoring,
   on the GPU inside the grid decode kernel.
+* `kv_cache` "paged" or "paged_fp4": the grouped-KV layers' keys and values live in pages (`ops.paged`), in bfloat16 or in 4 bits
+  (0.28 of the bytes), written by `ops.paged_append` and read by `ops.paged_attention`. Keys are rotated as they are
+  appended where the layer has no distance cap, and stay unrotated under one.
 * GDN layers: the recurrent state S [B, Hv, dk, dv] (fp32) and the K-1 conv inputs, updated in place.
 * one decode step (embedding -> all layers -> final norm -> head -> argmax) is captured in a CUDA graph on static
   input/output buffers; per-row lengths live on the device and advance inside the graph.
@@ -33,13 +36,17 @@ from ..models.sequence import SeqContext
 
 
 class DecodeEngine:
-    def __init__(self, model, batch: int, max_len: int, device=None, splits: int | None = None, use_graph: bool = True):
+    def __init__(self, model, batch: int, max_len: int, device=None, splits: int | None = None, use_graph: bool = True, kv_cache: str = "static",
+                 page_size: int = 64):
+        if kv_cache not in ("static", "paged", "paged_fp4"):
+            raise ValueError(f"kv_cache {kv_cache!r}: 'static', 'paged' or 'paged_fp4'")
+        self.paged = kv_cache != "static"
         self.model = model.eval()
         self.cfg = model.cfg
         self.B, self.T = batch, max_len
         self.device = torch.device(device) if device is not None else next(model.parameters()).device
         self.native = self.device.type == "cuda" and ops.mode() == "native"
-        self.use_graph = use_graph and self.device.type == "cuda"
+        self.use_graph = use_graph and self.device.type == "cuda" and (self.native or not self.paged)     # (the paged statements read their tables on the host)
         dev, B, T = self.device, batch, max_len
         # every static buffer sits between guard bands (infer/arena.py); `check_guards()` after a run finds a write past an end
         self.buffers = GuardedBuffers(dev)
@@ -80,6 +87,15 @@ class DecodeEngine:
             raise ValueError("the decode engine does not keep a Canon layer's input history (model.encoder.canon_kernel): "
                              "generate through the model's cached forward (eval.generate)")
         kv_dtype = torch.bfloat16 if dev.type == "cuda" else torch.float32
+        if self.paged:
+            if any(l.kind == "attention" and l.mixer.grid is not None for l in model.encoder.layers):
+                raise ValueError("kv_cache 'paged' holds grouped heads; grid KV layers cache raw components, whose key norm is applied while scoring: "
+                                 "kv_cache 'static'")
+            width = -(-T // page_size)         # every row owns its pages; the tables are the ops', so that rows may hold any of them
+            self.pages = z("pages", (B, width), torch.int32)
+            self.pages.copy_(torch.arange(B * width, device=dev, dtype=torch.int32).view(B, width))
+            self.q_start = z("q_start", B + 1, torch.int32)
+            self.q_start.copy_(torch.arange(B + 1, device=dev))
         for li, layer in enumerate(model.encoder.layers):
             m = layer.mixer
             if layer.kind == "attention":
@@ -87,8 +103,14 @@ class DecodeEngine:
                 heads, width = (1, m.grid.width) if m.grid is not None else (c.n_kv_heads, c.head_dim)
                 rot = rotary_dims(c.head_dim, c.rope_fraction)
                 n_ang = (m.cap + 1) if m.cap is not None else max_len
-                st = {"k": z(f"layer{li}.k", (B, T, heads, width), kv_dtype),
-                      "v": z(f"layer{li}.v", (B, T, heads, width), kv_dtype), "rot": rot, "heads": heads}
+                if self.paged:
+                    n_ang = max(n_ang, max_len)          # the paged ops index the rotations by position
+                    fmt = "fp4" if kv_cache == "paged_fp4" else "bf16" if dev.type == "cuda" else "fp32"
+                    st = {"rot": rot, "heads": heads, "paged": ops.PagedKV.zeros(self.pages.numel(), page_size, heads, width, fmt, dev,
+                                                                                make=lambda name, shape, dtype, li=li: z(f"layer{li}.{name}", shape, dtype))}
+                else:
+                    st = {"k": z(f"layer{li}.k", (B, T, heads, width), kv_dtype),
+                          "v": z(f"layer{li}.v", (B, T, heads, width), kv_dtype), "rot": rot, "heads": heads}
                 if rot:
                     inv = c.rope_theta ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=dev) / rot)
                     ang = torch.arange(n_ang, dtype=torch.float64, device=dev)[:, None] * inv
@@ -121,6 +143,7 @@ class DecodeEngine:
         n = 0
         for st in self.layers:
             n += sum(t.numel() * t.element_size() for t in st.values() if isinstance(t, torch.Tensor))
+            n += st["paged"].bytes() if "paged" in st else 0
         return n
 
     # ------------------------------------------------------------------ prefill
@@ -143,6 +166,11 @@ class DecodeEngine:
             for st, layer, cache in zip(self.layers, self.model.encoder.layers, out.cache.encoder):
                 if layer.kind == "attention":
                     m = layer.mixer
+                    if self.paged:              # as the step appends them: unrotated under a cap, rotated without
+                        kn, n = cache.k if m.cap is None else cache.k_far, hi - lo
+                        ends = torch.arange(n + 1, device=kn.device, dtype=torch.int32) * P
+                        ops.paged_append(st["paged"], kn.flatten(0, 1), cache.v.flatten(0, 1), self.pages[lo:hi], ends, ends[1:] - ends[:-1])
+                        continue
                     if m.grid is not None:      # raw components, as the model's own cache holds them
                         kn, v = cache.k, cache.v
                     else:
@@ -190,6 +218,11 @@ class DecodeEngine:
         else:
             k_new = m.k_norm(m.k_proj(h).view(B, 1, c.n_kv_heads, hd)) if hasattr(m.k_norm, "weight") else m.k_proj(h).view(B, 1, c.n_kv_heads, hd)
             v_new = m.v_proj(h).view(B, 1, c.n_kv_heads, hd)
+        if self.paged:
+            lens, rope = self.lens + 1, (st["cos"], st["sin"]) if st["rot"] else None
+            ops.paged_append(st["paged"], k_new[:, 0], v_new[:, 0], self.pages, self.q_start, lens, start=self.doc_start, rope=rope if m.cap is None else None)
+            o = ops.paged_attention(qn[:, 0], st["paged"], self.pages, self.q_start, lens, start=self.doc_start, rope=rope, cap=m.cap).unsqueeze(1)
+            return m.output(o.to(h.dtype if gate is None else gate.dtype), gate)
         rows = torch.arange(B, device=h.device)
         at = self.lens.long()
         st["k"][rows, at] = k_new[:, 0].to(st["k"].dtype)

@@ -785,3 +785,161 @@ def test_the_operators_together(fmt):
         for a, b in zip(_values(cpu), _values(gpu)):
             assert torch.equal(a, b)
     _status_clean()
+
+
+# ------------------------------------------------------------------------------------------------------------ callers: the decode engine, LoopSpec
+
+def _engine_cfg(kind):
+    from gdn_hybrid_architecture_ideas_b200 import config as C
+
+    cfg = C.tiny_full_config() if kind == "full" else C.tiny_control_config()
+    cfg.encoder.attention.head_dim = 16
+    return cfg
+
+
+@pytest.mark.parametrize("kind", ["full", "plain"])
+def test_engine_over_pages_matches_prefill_and_extend_cpu(kind):
+    """The decode engine on paged keys and values equals the model's own cached forward (with the distance cap, position-free
+    layers, a document that starts inside a row; and rotated keys without a cap)."""
+    from gdn_hybrid_architecture_ideas_b200.infer.engine import DecodeEngine
+    from tests.helpers import make_model
+    from tests.test_decode_engine import _oracle
+
+    model = make_model(_engine_cfg(kind), dtype=torch.float32).eval()
+    B, P, steps = 3, 40, 6
+    g = torch.Generator().manual_seed(0)
+    prompts = torch.randint(0, 256, (B, P), generator=g)
+    docs = torch.zeros(B, P, dtype=torch.long)
+    docs[1, 11:] = 1
+    want = _oracle(model, prompts, docs, steps)
+    eng = DecodeEngine(model, B, P + steps + 2, device="cpu", use_graph=False, kv_cache="paged", page_size=8)
+    assert torch.equal(eng.prefill(prompts, docs, rows_per_pass=2), want[:, 0].argmax(-1))
+    for i in range(1, steps):
+        eng.step()
+        assert (eng.logits - want[:, i]).abs().max() < 2e-4
+    eng.check_guards()
+
+
+def test_engine_over_4_bit_pages_cpu():
+    """The first attention layer's pages hold the static engine's keys and values in 4 bits; steps run, no guard is touched,
+    the cache takes 4.5 / 32 of the float32 bytes."""
+    from gdn_hybrid_architecture_ideas_b200.infer.engine import DecodeEngine
+    from tests.helpers import make_model
+
+    model = make_model(_engine_cfg("full"), dtype=torch.float32).eval()
+    prompts = torch.randint(0, 256, (2, 30), generator=torch.Generator().manual_seed(1))
+    kw = dict(device="cpu", use_graph=False)
+    eng, static = DecodeEngine(model, 2, 48, kv_cache="paged_fp4", page_size=16, **kw), DecodeEngine(model, 2, 48, **kw)
+    eng.prefill(prompts), static.prefill(prompts)
+    li = next(i for i, st in enumerate(eng.layers) if "paged" in st)
+    c = eng.layers[li]["paged"]
+    q_start = torch.tensor([0, 30, 60], dtype=torch.int32)
+    k, v = ops.paged_read(c, eng.pages, q_start, eng.lens, 60)
+    for got, name in ((k, "k"), (v, "v")):
+        x = static.layers[li][name][:, :30].flatten(0, 1)
+        assert torch.equal(got, pg.fp4_values(*pg.fp4_quantize(x)).bfloat16())
+    for _ in range(4):
+        eng.step()
+    assert torch.isfinite(eng.logits).all()
+    eng.check_guards()
+    attn = lambda e: sum(st["paged"].bytes() if "paged" in st else st["k"].numel() * 8 for st in e.layers if "paged" in st or "k" in st)       # noqa: E731
+    assert attn(eng) * 32 == attn(static) * 4.5
+
+
+def test_engine_refuses_paged_grid_and_unknown_caches():
+    from gdn_hybrid_architecture_ideas_b200.infer.engine import DecodeEngine
+    from tests.helpers import make_model
+    from tests.test_decode_engine import _cfg
+
+    with pytest.raises(ValueError, match="grid"):
+        DecodeEngine(make_model(_cfg("grid"), dtype=torch.float32), 1, 16, device="cpu", use_graph=False, kv_cache="paged")
+    with pytest.raises(ValueError, match="kv_cache"):
+        DecodeEngine(make_model(_cfg("full"), dtype=torch.float32), 1, 16, device="cpu", use_graph=False, kv_cache="fp8")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_cache", ["paged", "paged_fp4"])
+@pytest.mark.parametrize("cap", [96, None])
+def test_engine_over_pages_gpu(kv_cache, cap):
+    """The captured step equals the eager one token for token; with bfloat16 pages the logits agree with the static cache's
+    (the same cached values, rotated and scored by another kernel: bfloat16 noise), with 4 bits they stay near."""
+    from gdn_hybrid_architecture_ideas_b200 import config as C
+    from gdn_hybrid_architecture_ideas_b200.infer.engine import DecodeEngine
+    from gdn_hybrid_architecture_ideas_b200.models import build_model
+
+    torch.manual_seed(0)
+    cfg = C.hybrid_model_config("60m", full=True)
+    cfg.encoder.n_layers, cfg.encoder.nope_global_layers, cfg.vocab_size = 8, (1,), 2048
+    cfg.encoder.attention.rope_max_distance = cap
+    model = build_model(cfg).cuda().eval()
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(torch.randn_like(p) * 0.02)
+    B, P, steps = 4, 256, 8
+    prompts = torch.randint(0, 2048, (B, P), device="cuda")
+    mk = lambda graph, kv: DecodeEngine(model, B, P + steps + 4, use_graph=graph, kv_cache=kv)          # noqa: E731
+    graph, eager, static = mk(True, kv_cache), mk(False, kv_cache), mk(False, "static")
+    assert torch.equal(graph.generate(prompts, steps), eager.generate(prompts, steps))
+    _status_clean()
+    graph.check_guards(), eager.check_guards()
+    eager.prefill(prompts), static.prefill(prompts)
+    eager.tokens.copy_(static.tokens)
+    eager.step(), static.step()
+    rel = float((eager.logits - static.logits).norm() / static.logits.norm())
+    assert rel < (0.05 if kv_cache == "paged" else 0.5), rel
+
+
+def _looped():
+    from gdn_hybrid_architecture_ideas_b200 import config as C
+    from gdn_hybrid_architecture_ideas_b200.models import build_model
+
+    torch.manual_seed(0)
+    cfg = C.tiny_looped_config()
+    model = build_model(cfg).double().eval()
+    g = torch.Generator().manual_seed(2)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(torch.randn(p.shape, generator=g, dtype=p.dtype) * 0.05)
+    prompt = torch.randint(0, cfg.vocab_size, (1, 14), generator=g)
+    doc, dec = torch.zeros_like(prompt), torch.zeros_like(prompt, dtype=torch.bool)
+    dec[0, 9:] = True
+    return model, prompt, doc, dec
+
+
+def test_loopspec_samples_by_the_acceptance_rule(monkeypatch):
+    """Every step's decision is the rule's on the distributions of the model's own forwards at that prefix: the target's of two
+    passes, the draft head's of one; a draft head equal to the target is always kept."""
+    from gdn_hybrid_architecture_ideas_b200.infer import loopspec
+
+    model, prompt, doc, dec = _looped()
+    seen = []
+    real = ops.verify_drafts
+    monkeypatch.setattr(loopspec.ops, "verify_drafts", lambda *a, **k: seen.append((a, real(*a, **k))) or seen[-1][1])
+    toks, stats = loopspec.LoopSpec(model).generate(prompt, doc, dec, 10, greedy=False, generator=torch.Generator().manual_seed(7))
+    assert len(toks) == 10 and stats.steps == len(seen) == 9 and stats.flags == [bool(k[0]) for _, (_, k) in seen] and len(set(stats.flags)) == 2
+    for i, ((target, draft, drafted, ua, us), (tokens, kept)) in enumerate(seen):
+        prefix = torch.cat([prompt, torch.tensor([toks[:i + 1]])], 1)
+        mask = torch.cat([dec, torch.ones(1, i + 1, dtype=torch.bool)], 1)
+        with torch.no_grad():
+            two = model(prefix, torch.zeros_like(prefix), mask, T=2, capacity=int(mask.sum())).logits[0, prefix.shape[1] - 1]
+        p = torch.softmax(two.float(), -1)
+        assert (target[0, 0] - p).abs().max() < 1e-6
+        x, q = int(drafted), draft[0, 0].double()
+        keep = float(ua) * float(q[x]) < float(target[0, 0, x])
+        assert bool(kept[0]) == keep and toks[i + 1] == int(tokens[0, 0])
+        if keep:
+            assert toks[i + 1] == x
+        else:
+            w = (target[0, 0].double() - q).clamp(min=0)
+            assert toks[i + 1] == int((w.cumsum(0) > float(us) * w.sum()).nonzero()[0])
+    again, _ = loopspec.LoopSpec(model).generate(prompt, doc, dec, 10, greedy=False, generator=torch.Generator().manual_seed(7))
+    assert again == toks
+    with torch.no_grad():                    # a second pass that changes nothing
+        model.readout_norms[0].weight.copy_(model.decoder_norm.weight)
+        for layer in model.decoder_layers:
+            layer.residual_scale = 0.0
+        model.injection.A_log.fill_(-30.0)
+        model.injection.B.zero_()
+        model.loop_embedding.zero_()
+    _, stats = loopspec.LoopSpec(model).generate(prompt, doc, dec, 8, greedy=False, generator=torch.Generator().manual_seed(3))
+    assert stats.acceptance == 1.0
