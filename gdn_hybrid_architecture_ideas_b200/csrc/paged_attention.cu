@@ -54,6 +54,7 @@ template <bool FP4, int HD>
 struct Geo : Cfg<FP4, HD> {
   using B = Cfg<FP4, HD>;
   static constexpr int MT = B::MT, ST = B::ST;
+  static constexpr bool SPLIT = ST == 1;             // one stage: the values arrive while the scores are formed
   static constexpr int TILE = 16 * MT;
   static constexpr int H = HD / 64;                  // 64-channel slices
   static constexpr int ROW = FP4 ? HD / 2 : HD * 2;  // bytes of a position
@@ -349,11 +350,10 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
         const int e = __shfl_sync(0xffffffffu, entry, at_chunk);
         const long off = static_cast<long>(e) * GEO::ROW;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t dst = st + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH);
-          cp16(dst, k_lane + off + i * 512);
-          cp16(dst + GEO::KB, v_lane + off + i * 512);
-        }
+        for (int i = 0; i < N; ++i) cp16(st + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH), k_lane + off + i * 512);
+        if constexpr (GEO::SPLIT) cp_commit();
+#pragma unroll
+        for (int i = 0; i < N; ++i) cp16(st + GEO::KB + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH), v_lane + off + i * 512);
         if constexpr (FP4) {
           const long soff = static_cast<long>(e) * GEO::S + (lane % L) * 16;
           if constexpr (2 * L > 32) {        // (wide heads: one copy for the keys', one for the values')
@@ -364,16 +364,18 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
           }
         }
       } else {
+        auto copy = [&](uint32_t to, const void* from) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int pos = (i * 32 + lane) / CH, sub = (i * 32 + lane) % CH, c = pos >> c_shift;
-          const int e = __shfl_sync(0xffffffffu, entry, at_chunk + c) + (pos & ((1 << c_shift) - 1));
-          const long off = static_cast<long>(e) * GEO::ROW + sub * 16;
-          const bool ok = (on >> c) & 1;
-          const uint32_t dst = st + place_of(pos, sub);
-          cp16(dst, static_cast<const uint8_t*>(p.c.k) + (ok ? off : 0), ok);
-          cp16(dst + GEO::KB, static_cast<const uint8_t*>(p.c.v) + (ok ? off : 0), ok);
-        }
+          for (int i = 0; i < N; ++i) {
+            const int pos = (i * 32 + lane) / CH, sub = (i * 32 + lane) % CH, c = pos >> c_shift;
+            const int e = __shfl_sync(0xffffffffu, entry, at_chunk + c) + (pos & ((1 << c_shift) - 1));
+            const bool ok = (on >> c) & 1;
+            cp16(to + place_of(pos, sub), static_cast<const uint8_t*>(from) + (ok ? static_cast<long>(e) * GEO::ROW + sub * 16 : 0), ok);
+          }
+        };
+        copy(st, p.c.k);
+        if constexpr (GEO::SPLIT) cp_commit();
+        copy(st + GEO::KB, p.c.v);
         if constexpr (FP4) {
 #pragma unroll
           for (int i = 0; i < (2 * L + 31) / 32; ++i) {
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
 #pragma unroll
       for (int i = 0; i < ST - 1; ++i) on_ring[i] = on_ring[i + 1];        // the masks travel with the ring
       uint8_t* st = ring + stage * GEO::STAGE;
-      cp_wait<ST - 1>();
+      cp_wait<GEO::SPLIT ? 1 : ST - 1>();
       __syncwarp();
       stage = stage == ST - 1 ? 0 : stage + 1;
       if (on) {
@@ -693,6 +695,10 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
           for (int q = 0; q < 2; ++q)
             pk[mt][q] = pack<FP4>(exp2_fast(fmaf(s[mt][2 * q], mul[0], ref0)), exp2_fast(fmaf(s[mt][2 * q + 1], mul[1], ref1)));
         // ---- O^T += V^T P^T
+        if constexpr (GEO::SPLIT) {
+          cp_wait<0>();
+          __syncwarp();
+        }
         bool plain = true;
         if constexpr (!FP4) {
           // A masked position's value may be infinite or NaN, and 0 times it would reach rows that do not see it: such a
