@@ -197,6 +197,11 @@ __device__ __forceinline__ RowWork<CAP> row_work(const Row& row, int G, int cap)
   return w;
 }
 
+// a / b for a >= 0, b > 0: costs fit 32 bits but for enormous batches
+__device__ __forceinline__ long quot(long a, long b) {
+  return ((a | b) >> 32) == 0 ? static_cast<long>(static_cast<unsigned>(a) / static_cast<unsigned>(b)) : a / b;
+}
+
 template <int THREADS>
 __device__ __forceinline__ long block_scan(long x, long* s_warp, long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -220,6 +225,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long s_warp[W];
   __shared__ long s_at[2];
+  __shared__ Row s_row;
   __shared__ float s_mul[UR];                 // a query row's factor on its scores: scale * log2(e) * its power of two
   __shared__ float s_m[W][UR], s_l[W][UR];
   __shared__ int s_pos[UR];                   // a query row's position
@@ -228,9 +234,11 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
   const int n_ctas = gridDim.x, cta = blockIdx.x, Hkv = R.Hkv, G = p.G;
 
   // ---- this CTA's share of the pieces
+  Row own = {0, 0, 0, 0};
   auto pieces_of = [&](int i) -> long {
     if (i >= R.B) return 0;
-    const RowWork<CAP> w = row_work<GEO, CAP>(load_row(R, i), G, p.a.cap);
+    own = load_row(R, i);
+    const RowWork<CAP> w = row_work<GEO, CAP>(own, G, p.a.cap);
     return w.units * w.cost() * Hkv;
   };
   long total = 0, mine = 0, ex = 0;
@@ -240,29 +248,32 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
     ex = total + block_scan<GEO::THREADS>(mine, s_warp, &all);
     total += all;
   }
-  // CTAs with work: their shares are at least a piece's cost, so that each holds the start of one
-  const long most = total / RowWork<CAP>::NEAR;
+  // CTAs with work: their shares are at least a piece's cost, so that each holds the start of one. The first `extra` have one more.
+  const long most = quot(total, RowWork<CAP>::NEAR);
   const long use = most < 1 ? (total > 0) : most < n_ctas ? most : n_ctas;
   int* meta = p.meta + cta * 8;
   if (tid == 0) meta[0] = 0;                  // parts of the unit that this CTA begins and others end
   if (cta >= use) return;
-  const long lo = total * cta / use, hi = total * (cta + 1) / use;
+  const long share = quot(total, use), extra = total - share * use;
+  auto start_of = [&](long i) -> long { return share * i + (i < extra ? i : extra); };
+  auto cta_of = [&](long c) -> long { return c < (share + 1) * extra ? quot(c, share + 1) : extra + quot(c - (share + 1) * extra, share); };
+  const long lo = start_of(cta), hi = start_of(cta + 1);
   if (R.B <= GEO::THREADS) {
-    if (lo >= ex && lo < ex + mine) { s_at[0] = tid; s_at[1] = ex; }
+    if (lo >= ex && lo < ex + mine) { s_at[0] = tid; s_at[1] = ex; s_row = own; }
   } else {
     long before = 0;
     for (int b0 = 0; before <= lo; b0 += GEO::THREADS) {
       long all;
       mine = pieces_of(b0 + tid);
       ex = before + block_scan<GEO::THREADS>(mine, s_warp, &all);
-      if (lo >= ex && lo < ex + mine) { s_at[0] = b0 + tid; s_at[1] = ex; }
+      if (lo >= ex && lo < ex + mine) { s_at[0] = b0 + tid; s_at[1] = ex; s_row = own; }
       before += all;
     }
   }
   __syncthreads();
   int b = static_cast<int>(s_at[0]);
   long row_at = s_at[1];
-  __syncthreads();
+  Row row = s_row;
 
   uint8_t* ring = smem + warp * (ST * GEO::STAGE);
   const uint32_t ring_u = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
@@ -271,14 +282,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
   float* sq_base = reinterpret_cast<float*>(sq + GEO::q_bytes(CAP));                       // [UR][2 half]
   float4* s_turn = reinterpret_cast<float4*>(sq_base + UR * 2 * half);                     // [TILE][half / 2]: cos, cos, sin, sin of two pairs
   uint8_t* s_turned = reinterpret_cast<uint8_t*>(s_turn + TILE * (half >> 1)) + warp * GEO::turned_bytes(half);
-  if constexpr (CAP) {
-    for (int i = tid; i < TILE * (half >> 1); i += GEO::THREADS) {
-      const int d = min(i / (half >> 1), p.a.n_pos - 1), j = i % (half >> 1);
-      const float2 c = *reinterpret_cast<const float2*>(p.a.cos + static_cast<long>(d) * half + 2 * j), sn = *reinterpret_cast<const float2*>(p.a.sin + static_cast<long>(d) * half + 2 * j);
-      s_turn[i] = make_float4(c.x, c.y, sn.x, sn.y);
-    }
-  }
-
   // ---- the part of a unit that this CTA does next
   struct Part { int b, q0, start, h, r0, n_rows, p0, n_pieces, pieces, pos0, p_first, p_last, tile0; long last_cost; };
   long at = lo;
@@ -286,15 +289,14 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
   // (at: where the part starts, in costs; its pieces are those that start in at .. hi. Moves at to the part's end; false: none left.)
   auto locate = [&]() -> bool {
     while (at < hi) {
-      const Row row = load_row(R, b);
       const RowWork<CAP> wk = row_work<GEO, CAP>(row, G, p.a.cap);
       const long each = wk.cost(), count = wk.units * each * Hkv;
       if (at >= row_at + count) {             // (rows without tokens have no pieces)
         row_at += count;
-        ++b;
+        row = load_row(R, ++b);
         continue;
       }
-      const int unit = static_cast<int>((at - row_at) / each);
+      const int unit = static_cast<int>(quot(at - row_at, each));
       const long unit_at = row_at + unit * each;
       sg.p0 = wk.piece_at(at - unit_at);
       const int p1 = hi - unit_at >= each ? wk.pieces : wk.piece_at(hi - unit_at);
@@ -397,26 +399,84 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
     for (int k = 0; k < ST - 1; ++k) on_ring[k] = issue(k, k);
   };
   if (!locate()) return;
-  begin();
+  bool begun = false;
   while (true) {
     const int h = sg.h, r0 = sg.r0, n_rows = sg.n_rows, n_pieces = sg.n_pieces, pos0 = sg.pos0, p_first = sg.p_first, p_last = sg.p_last, tile0 = sg.tile0;
     const int q0 = sg.q0, start = sg.start, p0 = sg.p0, pieces = sg.pieces;
     int stage = 0;                             // of tile k
 
-    // ---- the unit's queries: rotated (near at their positions, far by the cap), brought to about one, in the MMA's order
-    for (int r = warp; r < UR; r += W) {
+    // ---- the unit's queries, a warp a row: all loads first (they and the first tiles are under way together), then rotated (by their
+    // positions; under a cap by the cap, the near rotation follows tile by tile), brought to about one, in the products' order
+    constexpr int RPW = (UR + W - 1) / W, CPL = HD / 32;
+    float x[RPW][CPL], y[RPW][CPL], co[RPW][CPL], si[RPW][CPL];
+    {
+      // (addresses are clamped to valid ones instead of branched over, so that the loads of a row stand side by side)
+      long off[RPW], table[RPW];
+#pragma unroll
+      for (int j = 0; j < RPW; ++j) {
+        const int r = warp + j * W, rr = r0 + r;
+        const bool live = r < n_rows && p_last >= 0;
+        off[j] = (static_cast<long>(q0) + (live ? rr / G : 0)) * p.a.q_ts + static_cast<long>(h * G + (live ? rr % G : 0)) * p.a.q_hs;
+        int at_pos = pos0 + (live ? rr / G : 0) - start;
+        if (live && half > 0 && at_pos >= p.a.n_pos) { *R.err = ST_ROPE; at_pos = p.a.n_pos - 1; }
+        table[j] = static_cast<long>(CAP ? p.a.cap : max(0, min(at_pos, p.a.n_pos - 1))) * half;
+        if (lane == 0 && r < UR) s_pos[r] = live ? pos0 + rr / G : -1;
+      }
+      auto partner = [&](int c) { return c < half ? c + half : c < 2 * half ? c - half : c; };
+      if (p.a.q_f32) {
+        const float* q = static_cast<const float*>(p.a.q);
+#pragma unroll
+        for (int j = 0; j < RPW; ++j)
+#pragma unroll
+          for (int i = 0; i < CPL; ++i) { x[j][i] = q[off[j] + lane + 32 * i]; y[j][i] = q[off[j] + partner(lane + 32 * i)]; }
+      } else {
+        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.a.q);
+        __nv_bfloat16 xb[RPW][CPL], yb[RPW][CPL];
+#pragma unroll
+        for (int j = 0; j < RPW; ++j)
+#pragma unroll
+          for (int i = 0; i < CPL; ++i) { xb[j][i] = q[off[j] + lane + 32 * i]; yb[j][i] = q[off[j] + partner(lane + 32 * i)]; }
+#pragma unroll
+        for (int j = 0; j < RPW; ++j)
+#pragma unroll
+          for (int i = 0; i < CPL; ++i) { x[j][i] = __bfloat162float(xb[j][i]); y[j][i] = __bfloat162float(yb[j][i]); }
+      }
+      if (half > 0) {
+#pragma unroll
+        for (int j = 0; j < RPW; ++j)
+#pragma unroll
+          for (int i = 0; i < CPL; ++i) {
+            const int c = lane + 32 * i;
+            const long e = table[j] + (c < half ? c : c < 2 * half ? c - half : 0);
+            co[j][i] = p.a.cos[e];
+            si[j][i] = p.a.sin[e];
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < RPW; ++j)
+#pragma unroll
+          for (int i = 0; i < CPL; ++i) { co[j][i] = 1.f; si[j][i] = 0.f; }
+      }
+    }
+    if (!begun) begin();
+    if (CAP && !begun) {
+      for (int i = tid; i < TILE * (half >> 1); i += GEO::THREADS) {
+        const int d = min(i / (half >> 1), p.a.n_pos - 1), j = i % (half >> 1);
+        const float2 c = *reinterpret_cast<const float2*>(p.a.cos + static_cast<long>(d) * half + 2 * j), sn = *reinterpret_cast<const float2*>(p.a.sin + static_cast<long>(d) * half + 2 * j);
+        s_turn[i] = make_float4(c.x, c.y, sn.x, sn.y);
+      }
+    }
+    begun = true;
+#pragma unroll
+    for (int j = 0; j < RPW; ++j) {
+      const int r = warp + j * W;
+      if (r >= UR) break;
       const bool live = r < n_rows && p_last >= 0;
-      const int rr = r0 + r;
-      const long tok = q0 + (live ? rr / G : 0);
-      const int head = h * G + (live ? rr % G : 0);
-      const long off = tok * p.a.q_ts + head * p.a.q_hs;
-      auto qv = [&](int c) -> float {
-        return p.a.q_f32 ? static_cast<const float*>(p.a.q)[off + c] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.a.q)[off + c]);
-      };
-      float x[HD / 32];
       float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) { x[i] = live ? qv(lane + 32 * i) : 0.f; top = fmaxf(top, fabsf(x[i])); }
+      for (int i = 0; i < CPL; ++i) { x[j][i] = live ? x[j][i] : 0.f; y[j][i] = live ? y[j][i] : 0.f; }
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) top = fmaxf(top, fabsf(x[j][i]));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       int ex = 0;
@@ -424,20 +484,9 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
       ex = max(-120, min(120, ex));
       const float down = exp2f(static_cast<float>(-ex));
       if (lane == 0) s_mul[r] = p.a.scale * 1.44269504088896340736f * exp2f(static_cast<float>(ex));
-      if (lane == 0) s_pos[r] = live ? pos0 + rr / G : -1;
-      int qpos = pos0 + rr / G - start;
-      if (live && half > 0 && qpos >= p.a.n_pos) { *R.err = ST_ROPE; qpos = p.a.n_pos - 1; }
-      qpos = CAP ? p.a.cap : max(qpos, 0);
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
+      for (int i = 0; i < CPL; ++i) {
         const int c = lane + 32 * i;
-        float turned = x[i];                   // by the position, under a cap by the cap
-        if (live && c < 2 * half) {
-          const bool lowside = c < half;
-          const int ai = lowside ? c : c - half;
-          const float y = qv(lowside ? c + half : c - half), sg = lowside ? -y : y;
-          turned = x[i] * p.a.cos[static_cast<long>(qpos) * half + ai] + sg * p.a.sin[static_cast<long>(qpos) * half + ai];
-        }
         // the order of the plain products (a lane owns the 16 channels 16 t .. of each slice), and of the rotating ones (its
         // channels are 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16)
         const int cc = c & 63;
@@ -453,10 +502,10 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
             reinterpret_cast<__nv_bfloat16*>(to + GEO::QB)[idx] = __float2bfloat16(isfinite(v) ? v - __bfloat162float(hi) : 0.f);
           }
         };
-        put(sq, plain_at, turned * down);
+        put(sq, plain_at, c < 2 * half ? (x[j][i] * co[j][i] + y[j][i] * (c < half ? -si[j][i] : si[j][i])) * down : x[j][i] * down);
         if constexpr (CAP) {
-          put(sq + GEO::QCOPIES * GEO::QB, near_at, x[i] * down);          // (its rotary channels are not read)
-          if (c < 2 * half) sq_base[r * 2 * half + c] = x[i] * down;
+          put(sq + GEO::QCOPIES * GEO::QB, near_at, x[j][i] * down);          // (its rotary channels are not read)
+          if (c < 2 * half) sq_base[r * 2 * half + c] = x[j][i] * down;
         }
       }
     }
@@ -805,37 +854,39 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
     const long last_cost = sg.last_cost;
     const bool more = locate();                // (the next part, from here on)
     if (!more) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (GEO::BESIDE && more) begin();
+    if (GEO::BESIDE && more) begin();          // (`begun` stays true)
     __syncthreads();
     const bool begins = p0 == 0, ends = p0 + n_pieces == pieces;
     const int slot = begins ? 1 : 0;
     float* wo = p.ws + (static_cast<long>(cta) * 2 + slot) * UR * (HD + 2);
-    for (int idx = tid; idx < n_rows * HD; idx += GEO::THREADS) {
-      const int r = idx / HD, c = idx % HD;
+    for (int idx = tid; idx < n_rows * (HD / 4); idx += GEO::THREADS) {
+      const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
       float mm = -INFINITY;
 #pragma unroll
       for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_m[w][r]);
       const float ref = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f, oo = 0.f;
+      float ll = 0.f;
+      float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
+      for (int w = 0; w < W; ++w) {            // (a warp that saw nothing holds zeros)
         const float f = exp2_fast(s_m[w][r] - ref);
+        const float4 z = *reinterpret_cast<const float4*>(so + (w * UR + r) * HD + c);
         ll += s_l[w][r] * f;
-        // (a warp that saw nothing holds zeros)
-        oo += so[(static_cast<long>(w) * UR + r) * HD + c] * f;
+        oo.x += z.x * f; oo.y += z.y * f; oo.z += z.z * f; oo.w += z.w * f;
       }
       if (begins && ends) {
         const int rr = r0 + r;
-        // a row of scores without one above -inf has no weights: zeros
-        static_cast<__nv_bfloat16*>(p.a.out)[((static_cast<long>(q0) + rr / G) * p.a.Hq + h * G + rr % G) * HD + c] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;          // a row without a score above -inf has no weights: zeros
+        const uint2 out = make_uint2(pack<false>(oo.x * inv, oo.y * inv), pack<false>(oo.z * inv, oo.w * inv));
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.a.out) + ((static_cast<long>(q0) + rr / G) * p.a.Hq + h * G + rr % G) * HD + c) = out;
       } else {
-        wo[r * HD + c] = oo;
+        *reinterpret_cast<float4*>(wo + r * HD + c) = oo;
         if (c == 0) { wo[UR * HD + 2 * r] = mm; wo[UR * HD + 2 * r + 1] = ll; }
       }
     }
     if (tid == 0 && begins && !ends) {           // the first part: how many CTAs hold the others follows from the shares
       meta[1] = h; meta[2] = r0; meta[3] = n_rows; meta[4] = q0;
-      meta[0] = static_cast<int>(((last_cost + 1) * use - 1) / total) - cta + 1;
+      meta[0] = static_cast<int>(cta_of(last_cost)) - cta + 1;
     }
     if (!more) break;
     if constexpr (!GEO::BESIDE) {
