@@ -1,6 +1,7 @@
 // Python bindings of the sm_100a kernels: tensors in, raw pointers + the current CUDA stream out.
 // Shape and dtype checks live here so that no kernel ever receives a pointer it was not written for.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -417,12 +418,13 @@ Tensor whole_heads(const Tensor& t) {
 struct PagedCache {
   Tensor k, v;
   c10::optional<Tensor> ks, vs;
+  Tensor err;                  // the device's status word
   int hd, heads, n_pages, page_shift;
   ghb::PagedPool pool() const {
     return {k.data_ptr(), v.data_ptr(), ks.has_value() ? static_cast<uint8_t*>(ks->data_ptr()) : nullptr, vs.has_value() ? static_cast<uint8_t*>(vs->data_ptr()) : nullptr, hd, ks.has_value()};
   }
 };
-PagedCache paged_cache(const Tensor& k, const Tensor& v, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs) {
+PagedCache paged_cache(const Tensor& k, const Tensor& v, const c10::optional<Tensor>& ks, const c10::optional<Tensor>& vs, const Tensor& err) {
   const bool fp4 = k.scalar_type() == torch::kUInt8;
   TORCH_CHECK_VALUE(k.is_cuda() && k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
                     "PagedKV: k and v are [pages, kv heads, page size, channels] of one type on one device, got ", k.sizes(), " and ", v.sizes());
@@ -438,9 +440,9 @@ PagedCache paged_cache(const Tensor& k, const Tensor& v, const c10::optional<Ten
   for (const Tensor* t : {&k, &v, fp4 ? &*ks : &k, fp4 ? &*vs : &v})
     TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "PagedKV: the tensors start on 16-byte boundaries");
   TORCH_CHECK_VALUE(k.size(0) <= 0x7fffffff && k.size(1) <= 0x7fffffff && page <= (1 << 30), "PagedKV: sizes");
-  return {k, v, ks, vs, static_cast<int>(hd), static_cast<int>(k.size(1)), static_cast<int>(k.size(0)), __builtin_ctzll(page)};
+  return {k, v, ks, vs, err, static_cast<int>(hd), static_cast<int>(k.size(1)), static_cast<int>(k.size(0)), __builtin_ctzll(page)};
 }
-ghb::PagedRows rows_of(const PagedCache& c, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start, int64_t n, Tensor& err, const char* what) {
+ghb::PagedRows rows_of(const PagedCache& c, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start, int64_t n, const char* what) {
   TORCH_CHECK(pages.dim() == 2 && q_start.dim() == 1 && lens.dim() == 1 && q_start.numel() == lens.numel() + 1 && pages.size(0) == lens.numel(), what,
               ": pages [B, width], q_start [B + 1], lens [B] of one batch");
   for (const Tensor* t : {&pages, &q_start, &lens}) TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->device() == c.k.device(), what, ": pages, q_start and lens are int32 on the cache's device");
@@ -448,7 +450,7 @@ ghb::PagedRows rows_of(const PagedCache& c, const Tensor& pages, const Tensor& q
   if (start.has_value()) TORCH_CHECK(start->scalar_type() == torch::kInt32 && start->device() == c.k.device() && start->sizes() == lens.sizes() && start->is_contiguous(), what, ": start int32 [B]");
   TORCH_CHECK(n >= 0 && n <= 0x7fffffff && lens.numel() < 0x7fffffff && pages.size(1) <= (0x7fffffffll >> c.page_shift), what, ": a row's table holds more positions than 32 bits count");
   return {pages.data_ptr<int>(), static_cast<long>(pages.stride(0)), static_cast<int>(pages.size(1)), q_start.data_ptr<int>(), lens.data_ptr<int>(),
-          start.has_value() ? start->data_ptr<int>() : nullptr, static_cast<int>(lens.numel()), static_cast<int>(n), c.heads, c.n_pages, c.page_shift, err.data_ptr<int>()};
+          start.has_value() ? start->data_ptr<int>() : nullptr, static_cast<int>(lens.numel()), static_cast<int>(n), c.heads, c.n_pages, c.page_shift, c.err.data_ptr<int>()};
 }
 // These ops have no backward: an input that a gradient would be asked of is refused, not silently cut off.
 void no_grad(const Tensor& t, const char* what) {
@@ -465,20 +467,20 @@ Rope rope_of(const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin,
   return {cos->data_ptr<float>(), sin->data_ptr<float>(), static_cast<int>(half), static_cast<int>(std::min<int64_t>(cos->size(0), 0x7fffffff))};
 }
 void paged_append(const PagedCache& c, const Tensor& k_, const Tensor& v_, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start,
-                  const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, Tensor& err) {
+                  const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin) {
   const c10::cuda::CUDAGuard guard(c.k.device());
   TORCH_CHECK(k_.dim() == 3 && v_.sizes() == k_.sizes() && k_.size(1) == c.heads && k_.size(2) == c.hd && k_.device() == c.k.device() && v_.device() == c.k.device(),
               "paged_append: k, v [n, ", c.heads, ", ", c.hd, "] on the cache's device, got ", k_.sizes(), " and ", v_.sizes());
   TORCH_CHECK((is_bf16(k_) || is_f32(k_)) && k_.scalar_type() == v_.scalar_type(), "paged_append: k, v bfloat16 or float32");
   no_grad(k_, "paged_append"); no_grad(v_, "paged_append");
-  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, start, k_.size(0), err, "paged_append");
+  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, start, k_.size(0), "paged_append");
   const Rope rope = rope_of(cos, sin, c.hd, c.k, "paged_append");
   const Tensor k = whole_heads(k_), v = whole_heads(v_);
   check(ghb::paged_append(r, c.pool(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), is_f32(k), rope.cos, rope.sin, rope.half, rope.n_pos, stream()),
         "paged_append");
 }
 std::tuple<Tensor, Tensor> paged_read(const PagedCache& c, const Tensor& pages, const Tensor& q_start, const Tensor& lens, int64_t n, const c10::optional<Tensor>& k_out,
-                                      const c10::optional<Tensor>& v_out, Tensor& err) {
+                                      const c10::optional<Tensor>& v_out) {
   const c10::cuda::CUDAGuard guard(c.k.device());
   const bool fill = !k_out.has_value();
   TORCH_CHECK(n >= 0 && fill == !v_out.has_value(), "paged_read: n >= 0, out two tensors or none");
@@ -488,22 +490,23 @@ std::tuple<Tensor, Tensor> paged_read(const PagedCache& c, const Tensor& pages, 
   for (const Tensor* o : {&ko, &vo})
     TORCH_CHECK(o->dim() == 3 && is_bf16(*o) && o->is_contiguous() && o->size(0) == n && o->size(1) == c.heads && o->size(2) == c.hd && o->device() == c.k.device() &&
                 reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0, "paged_read: out is two contiguous bfloat16 tensors [", n, ", ", c.heads, ", ", c.hd, "], got ", o->sizes());
-  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, c10::nullopt, n, err, "paged_read");
+  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, c10::nullopt, n, "paged_read");
   check(ghb::paged_read(r, c.pool(), ko.data_ptr(), vo.data_ptr(), fill, stream()), "paged_read");
   return {ko, vo};
 }
-Tensor paged_attention(const Tensor& q, const PagedCache& c, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start,
-                       const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, int64_t cap, const c10::optional<double>& scale, const c10::optional<Tensor>& out_, Tensor& err) {
+Tensor paged_attention(const Tensor& q_, const PagedCache& c, const Tensor& pages, const Tensor& q_start, const Tensor& lens, const c10::optional<Tensor>& start,
+                       const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin, int64_t cap, const c10::optional<double>& scale, const c10::optional<Tensor>& out_) {
   const c10::cuda::CUDAGuard guard(c.k.device());
-  TORCH_CHECK(q.dim() == 3 && (is_bf16(q) || is_f32(q)) && q.device() == c.k.device() && q.size(2) == c.hd && q.size(1) > 0 && q.size(1) % c.heads == 0,
-              "paged_attention: q bfloat16 or float32 [n, a multiple of ", c.heads, ", ", c.hd, "] on the cache's device, got ", q.sizes());
-  TORCH_CHECK(q.stride(2) == 1, "paged_attention: q with unit inner stride");
-  no_grad(q, "paged_attention");
+  TORCH_CHECK(q_.dim() == 3 && (is_bf16(q_) || is_f32(q_)) && q_.device() == c.k.device() && q_.size(2) == c.hd && q_.size(1) > 0 && q_.size(1) % c.heads == 0,
+              "paged_attention: q bfloat16 or float32 [n, a multiple of ", c.heads, ", ", c.hd, "] on the cache's device, got ", q_.sizes());
+  TORCH_CHECK(q_.stride(2) == 1, "paged_attention: q with unit inner stride");
+  no_grad(q_, "paged_attention");
+  const Tensor q = whole_heads(q_);
   const bool fill = !out_.has_value();
   Tensor out = fill ? at::empty(q.sizes(), q.options().dtype(torch::kBFloat16)) : *out_;
   TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.sizes() == q.sizes() && out.device() == c.k.device() && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
               "paged_attention: out is a contiguous bfloat16 tensor of q's shape");
-  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, start, q.size(0), err, "paged_attention");
+  const ghb::PagedRows r = rows_of(c, pages, q_start, lens, start, q.size(0), "paged_attention");
   TORCH_CHECK((static_cast<int64_t>(c.n_pages) * c.heads << c.page_shift) <= 0x7fffffff, "paged_attention: the cache has more than 2^31 entries of a head");
   const Rope rope = rope_of(cos, sin, c.hd, c.k, "paged_attention");
   TORCH_CHECK(cap == 0 || (rope.half > 0 && cap > 0 && cap < rope.n_pos), "paged_attention: a rotary distance cap is >= 1 and inside the rope table");
@@ -516,8 +519,9 @@ Tensor paged_attention(const Tensor& q, const PagedCache& c, const Tensor& pages
   ghb::PagedAttnPlan plan;
   check(ghb::paged_attention_plan(r, c.pool(), a.Hq, sm_count(), &plan), "paged_attention");
   // this call's own work space (a captured call's comes from its graph's pool)
-  const Tensor ws = at::empty({plan.ws_floats + plan.ws_ints}, q.options().dtype(torch::kFloat32));
-  check(ghb::paged_attention(r, c.pool(), a, plan, ws.data_ptr<float>(), reinterpret_cast<int*>(ws.data_ptr<float>() + plan.ws_floats), stream()), "paged_attention");
+  const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(4 * (plan.ws_floats + plan.ws_ints));
+  float* const w = static_cast<float*>(ws.get());
+  check(ghb::paged_attention(r, c.pool(), a, plan, w, reinterpret_cast<int*>(w + plan.ws_floats), stream()), "paged_attention");
   return out;
 }
 std::tuple<Tensor, Tensor> verify_drafts(const Tensor& target, const c10::optional<Tensor>& draft, const Tensor& drafts, const Tensor& u_accept, const Tensor& u_sample,

@@ -161,6 +161,23 @@ __device__ __forceinline__ uint32_t low_nibbles(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
+// N neighbouring channels (2, 4 or 8) as float32
+template <int N> __device__ __forceinline__ void load_channels(const float* p, float* x) {
+  if constexpr (N == 2) { const float2 u = *reinterpret_cast<const float2*>(p); x[0] = u.x; x[1] = u.y; }
+  else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) { const float4 u = *reinterpret_cast<const float4*>(p + i); x[i] = u.x; x[i + 1] = u.y; x[i + 2] = u.z; x[i + 3] = u.w; }
+  }
+}
+template <int N> __device__ __forceinline__ void load_channels(const __nv_bfloat16* p, float* x) {
+  uint32_t w[N / 2];
+  if constexpr (N == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
+  else if constexpr (N == 4) { const uint2 u = *reinterpret_cast<const uint2*>(p); w[0] = u.x; w[1] = u.y; }
+  else { const uint4 u = *reinterpret_cast<const uint4*>(p); w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; }
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) { const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+}
+
 // Row rho (0 .. 7) of an 8-row group of the tiles is position place(rho) of the group. 4 bits: chosen so that both the keys' reads
 // (8 bytes of rows rho = 0..3 or 4..7 at once) and the values' (4 bytes of rows 0,2,4,6 or 1,3,5,7) touch four
 // 32-byte rows that differ modulo 4, hence all 32 banks. bfloat16 rows are 128 bytes and swizzled by 16-byte chunk instead.
@@ -407,55 +424,33 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
 
     // ---- the unit's queries, a warp a row: all loads first (they and the first tiles are under way together), then rotated (by their
     // positions; under a cap by the cap, the near rotation follows tile by tile), brought to about one, in the products' order
+    // (a lane takes HD / 32 neighbouring channels: 2, 4 or 8, which divides half, so that their partners are neighbours too)
     constexpr int RPW = (UR + W - 1) / W, CPL = HD / 32;
+    const int c0 = lane * CPL;
+    const bool turns = c0 < 2 * half, low = c0 < half;
     float x[RPW][CPL], y[RPW][CPL], co[RPW][CPL], si[RPW][CPL];
-    {
-      // (addresses are clamped to valid ones instead of branched over, so that the loads of a row stand side by side)
-      long off[RPW], table[RPW];
 #pragma unroll
-      for (int j = 0; j < RPW; ++j) {
-        const int r = warp + j * W, rr = r0 + r;
-        const bool live = r < n_rows && p_last >= 0;
-        off[j] = (static_cast<long>(q0) + (live ? rr / G : 0)) * p.a.q_ts + static_cast<long>(h * G + (live ? rr % G : 0)) * p.a.q_hs;
-        int at_pos = pos0 + (live ? rr / G : 0) - start;
-        if (live && half > 0 && at_pos >= p.a.n_pos) { *R.err = ST_ROPE; at_pos = p.a.n_pos - 1; }
-        table[j] = static_cast<long>(CAP ? p.a.cap : max(0, min(at_pos, p.a.n_pos - 1))) * half;
-        if (lane == 0 && r < UR) s_pos[r] = live ? pos0 + rr / G : -1;
-      }
-      auto partner = [&](int c) { return c < half ? c + half : c < 2 * half ? c - half : c; };
+    for (int j = 0; j < RPW; ++j) {
+      const int r = warp + j * W, rr = r0 + r;
+      const bool live = r < n_rows && p_last >= 0;
+      // (addresses are clamped to valid ones instead of branched over, so that the loads stand side by side)
+      const int i = live ? rr / G : 0, head = h * G + (live ? rr % G : 0);
+      const long off = (static_cast<long>(q0) + i) * p.a.q_ts + head * p.a.q_hs;
+      int at_pos = pos0 + i - start;
+      if (live && half > 0 && at_pos >= p.a.n_pos) { *R.err = ST_ROPE; at_pos = p.a.n_pos - 1; }
+      if (lane == 0 && r < UR) s_pos[r] = live ? pos0 + i : -1;
+      const int partner = turns ? (low ? c0 + half : c0 - half) : c0;
       if (p.a.q_f32) {
-        const float* q = static_cast<const float*>(p.a.q);
-#pragma unroll
-        for (int j = 0; j < RPW; ++j)
-#pragma unroll
-          for (int i = 0; i < CPL; ++i) { x[j][i] = q[off[j] + lane + 32 * i]; y[j][i] = q[off[j] + partner(lane + 32 * i)]; }
+        load_channels<CPL>(static_cast<const float*>(p.a.q) + off + c0, x[j]);
+        load_channels<CPL>(static_cast<const float*>(p.a.q) + off + partner, y[j]);
       } else {
-        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.a.q);
-        __nv_bfloat16 xb[RPW][CPL], yb[RPW][CPL];
-#pragma unroll
-        for (int j = 0; j < RPW; ++j)
-#pragma unroll
-          for (int i = 0; i < CPL; ++i) { xb[j][i] = q[off[j] + lane + 32 * i]; yb[j][i] = q[off[j] + partner(lane + 32 * i)]; }
-#pragma unroll
-        for (int j = 0; j < RPW; ++j)
-#pragma unroll
-          for (int i = 0; i < CPL; ++i) { x[j][i] = __bfloat162float(xb[j][i]); y[j][i] = __bfloat162float(yb[j][i]); }
+        load_channels<CPL>(static_cast<const __nv_bfloat16*>(p.a.q) + off + c0, x[j]);
+        load_channels<CPL>(static_cast<const __nv_bfloat16*>(p.a.q) + off + partner, y[j]);
       }
       if (half > 0) {
-#pragma unroll
-        for (int j = 0; j < RPW; ++j)
-#pragma unroll
-          for (int i = 0; i < CPL; ++i) {
-            const int c = lane + 32 * i;
-            const long e = table[j] + (c < half ? c : c < 2 * half ? c - half : 0);
-            co[j][i] = p.a.cos[e];
-            si[j][i] = p.a.sin[e];
-          }
-      } else {
-#pragma unroll
-        for (int j = 0; j < RPW; ++j)
-#pragma unroll
-          for (int i = 0; i < CPL; ++i) { co[j][i] = 1.f; si[j][i] = 0.f; }
+        const long e = static_cast<long>(CAP ? p.a.cap : max(0, min(at_pos, p.a.n_pos - 1))) * half + (turns ? (low ? c0 : c0 - half) : 0);
+        load_channels<CPL>(p.a.cos + e, co[j]);
+        load_channels<CPL>(p.a.sin + e, si[j]);
       }
     }
     if (!begun) begin();
@@ -484,28 +479,29 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
       ex = max(-120, min(120, ex));
       const float down = exp2f(static_cast<float>(-ex));
       if (lane == 0) s_mul[r] = p.a.scale * 1.44269504088896340736f * exp2f(static_cast<float>(ex));
+      float turned[CPL];
 #pragma unroll
       for (int i = 0; i < CPL; ++i) {
-        const int c = lane + 32 * i;
-        // the order of the plain products (a lane owns the 16 channels 16 t .. of each slice), and of the rotating ones (its
-        // channels are 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16)
-        const int cc = c & 63;
-        const int plain_at = ((((c >> 6) * 4 + ((cc & 15) >> 2)) * 32 + r * 4 + (cc >> 4)) << 2) + (cc & 3);
-        const int near_at = (((c >> 4) * 32 + r * 4 + ((c & 7) >> 1)) << 2) + ((c >> 2) & 2) + (c & 1);
-        auto put = [&](uint8_t* to, int idx, float v) {
-          if constexpr (FP4) {
-            reinterpret_cast<__half*>(to)[idx] = __float2half_rn(v);
-          } else {
-            const __nv_bfloat16 hi = __float2bfloat16(v);
-            reinterpret_cast<__nv_bfloat16*>(to)[idx] = hi;
-            // (an infinity has no remainder)
-            reinterpret_cast<__nv_bfloat16*>(to + GEO::QB)[idx] = __float2bfloat16(isfinite(v) ? v - __bfloat162float(hi) : 0.f);
-          }
-        };
-        put(sq, plain_at, c < 2 * half ? (x[j][i] * co[j][i] + y[j][i] * (c < half ? -si[j][i] : si[j][i])) * down : x[j][i] * down);
+        turned[i] = (turns ? x[j][i] * co[j][i] + y[j][i] * (low ? -si[j][i] : si[j][i]) : x[j][i]) * down;
+        x[j][i] *= down;
+      }
+      // Two channels at a time to their places: in the order of the plain products (a lane owns the 16 channels 16 t .. of each slice),
+      // and of the rotating ones (its channels are 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16).
+      auto put = [&](uint8_t* to, int idx, float a, float z) {
+        const uint32_t hi = pack<FP4>(a, z);
+        *reinterpret_cast<uint32_t*>(to + idx * 2) = hi;
+        if constexpr (!FP4) {
+          const float2 f = unpack<FP4>(hi);       // (an infinity has no remainder)
+          *reinterpret_cast<uint32_t*>(to + GEO::QB + idx * 2) = pack<FP4>(isfinite(a) ? a - f.x : 0.f, isfinite(z) ? z - f.y : 0.f);
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < CPL; i += 2) {
+        const int c = c0 + i, cc = c & 63;
+        put(sq, ((((c >> 6) * 4 + ((cc & 15) >> 2)) * 32 + r * 4 + (cc >> 4)) << 2) + (cc & 3), turned[i], turned[i + 1]);
         if constexpr (CAP) {
-          put(sq + GEO::QCOPIES * GEO::QB, near_at, x[j][i] * down);          // (its rotary channels are not read)
-          if (c < 2 * half) sq_base[r * 2 * half + c] = x[j][i] * down;
+          put(sq + GEO::QCOPIES * GEO::QB, (((c >> 4) * 32 + r * 4 + ((c & 7) >> 1)) << 2) + ((c >> 2) & 2), x[j][i], x[j][i + 1]);      // (its rotary channels are not read)
+          if (turns) *reinterpret_cast<float2*>(sq_base + r * 2 * half + c) = make_float2(x[j][i], x[j][i + 1]);
         }
       }
     }

@@ -45,10 +45,12 @@ def _native():
     return _native_module
 
 
-def native_cache(cache) -> None:
-    """Checks a PagedKV on a GPU (in the binding, once); nothing to do in reference mode."""
+def _check_cache(cache) -> None:
     if _MODE == "native":
         _native()._cache(cache)
+
+
+paged.NATIVE_CHECK = _check_cache
 
 
 def rmsnorm(x, weight, eps, out_dtype=None):
@@ -258,7 +260,7 @@ def paged_append(cache, k, v, pages, q_start, lens, start=None, rope=None):
     row; a prompt is many. On CUDA: bfloat16 or float32 k, v, head dimension 64 / 128 / 256, a multiple of 16 rotary
     channels; no read-back, so it can be captured. A wrong table value (page id, length, range, position) is left out and
     reported on the status word (`check_status`); on the CPU it raises."""
-    if use_native(cache.k):
+    if cache._k.is_cuda and _MODE == "native":
         return _native().paged_append(cache, k, v, pages, q_start, lens, start, rope)
     return paged.paged_append(cache, k, v, pages, q_start, lens, start, rope)
 
@@ -267,7 +269,7 @@ def paged_read(cache, pages, q_start, lens, n, out=None):
     """(k, v), each (n, Hkv, hd): row b's last q_start[b + 1] - q_start[b] cached entries as packed tokens, as they are
     cached (the inverse of `paged_append`, without undoing a rotation); 4-bit entries as the bfloat16 values they stand
     for. out: two tensors to write into (their padding rows stay as they are)."""
-    if use_native(cache.k):
+    if cache._k.is_cuda and _MODE == "native":
         return _native().paged_read(cache, pages, q_start, lens, n, out)
     return paged.paged_read(cache, pages, q_start, lens, n, out)
 
@@ -279,7 +281,7 @@ def paged_attention(q, cache, pages, q_start, lens, start=None, rope=None, cap=N
     cap): the cache holds unrotated keys, a key at distance d <= C is scored R(p)q . R(t)k, beyond it R(C)q . k. No rope:
     position-free. A token that sees nothing gets zeros. scale: default hd ** -0.5. Forward only; on CUDA q is bfloat16 or
     float32, the output bfloat16, under a cap 16, 32 or 64 rotary channels."""
-    if use_native(cache.k):
+    if cache._k.is_cuda and _MODE == "native":
         return _native().paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out)
     return paged.paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out)
 

@@ -698,22 +698,22 @@ def attention(q, k, v, doc, q_far, k_far, cap, pos=None, single_doc=False):
 # ------------------------------------------------------------------------------------------------------------ paged cache, drafts
 
 def _cache(cache):
-    """The binding's checked form of a PagedKV's tensors, made on first use."""
+    """The binding's checked form of a PagedKV's tensors (with its device's status word), made on first use."""
     c = cache.native
     if c is None:
-        c = cache.native = ext().paged_cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
+        c = cache.native = ext().paged_cache(cache.k, cache.v, cache.k_scale, cache.v_scale, err_flag(cache.k.device))
     return c
 
 
 def paged_append(cache, k, v, pages, q_start, lens, start, rope):
     cos, sin = rope or (None, None)
-    ext().paged_append(_cache(cache), k, v, pages, q_start, lens, start, cos, sin, err_flag(cache.k.device))
+    (_ext or ext()).paged_append(cache.native or _cache(cache), k, v, pages, q_start, lens, start, cos, sin)
     _count()
 
 
 def paged_read(cache, pages, q_start, lens, n, out):
     ko, vo = out or (None, None)
-    r = ext().paged_read(_cache(cache), pages, q_start, lens, n, ko, vo, err_flag(cache.k.device))
+    r = (_ext or ext()).paged_read(cache.native or _cache(cache), pages, q_start, lens, n, ko, vo)
     _count()
     return r
 
@@ -724,7 +724,7 @@ def paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out
         cap = 0
     elif rope is None or cap < 1:
         raise ValueError("paged_attention: a rotary distance cap is an integer >= 1 beside a rope table")
-    out = ext().paged_attention(q, _cache(cache), pages, q_start, lens, start, cos, sin, cap, scale, out, err_flag(cache.k.device))
+    out = (_ext or ext()).paged_attention(q, cache.native or _cache(cache), pages, q_start, lens, start, cos, sin, cap, scale, out)
     _count(2)
     return out
 

@@ -26,12 +26,15 @@ which allocates its own output leaves zeros there. Rows may have no tokens.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 E2M1_GRID = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 E4M3 = torch.float8_e4m3fn
 BLOCK = 16
 LARGEST = 6.0 * 448.0
+NATIVE_CHECK = None             # set by `ops`: checks a cache on a GPU (in the binding, once)
 
 
 class PagedKV:
@@ -43,9 +46,8 @@ class PagedKV:
         self._k, self._v, self._ks, self._vs = k, v, k_scale, v_scale          # (fixed: the binding holds them too)
         self.native = None              # the CUDA binding's form of these tensors (ops/native.py)
         if k.is_cuda:
-            from . import native_cache
-
-            native_cache(self)          # checks in the binding
+            if NATIVE_CHECK is not None:
+                NATIVE_CHECK(self)      # in the binding
             return
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise ValueError(f"PagedKV: k and v are [pages, kv heads, page size, channels] of one type on one device, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
@@ -81,10 +83,7 @@ class PagedKV:
             raise ValueError(f"PagedKV: fmt {fmt!r}: 'bf16', 'fp4' (on the CPU also 'fp32', 'fp64')")
         return cls(*(make(n, (*lead, head_dim), dtypes[fmt]) for n in ("k", "v")))
 
-    k = property(lambda self: self._k)
-    v = property(lambda self: self._v)
-    k_scale = property(lambda self: self._ks)
-    v_scale = property(lambda self: self._vs)
+    k, v, k_scale, v_scale = (property(operator.attrgetter(n)) for n in ("_k", "_v", "_ks", "_vs"))
 
     @property
     def fp4(self) -> bool:
