@@ -409,9 +409,9 @@ void decode_attention_grid(const Tensor& q, const Tensor& k, const Tensor& v, co
 
 // ---- paged key/value cache (csrc/paged.cuh). The values of the tables are checked by the kernels; here their types and shapes.
 // 16-byte loads of whole heads: a tensor whose strides or address do not allow them is copied.
-Tensor whole_heads(const Tensor& t) {
-  const int64_t per = 16 / t.element_size();
-  const bool ok = t.stride(2) == 1 && t.stride(1) % per == 0 && t.stride(0) % per == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+Tensor whole_heads(const Tensor& t, int64_t bytes) {
+  const int64_t per = bytes / t.element_size();
+  const bool ok = t.stride(2) == 1 && t.stride(1) % per == 0 && t.stride(0) % per == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0;
   return ok ? t : t.contiguous().clone(at::MemoryFormat::Contiguous);
 }
 // The cache's tensors, checked once; what the calls need of them.
@@ -438,7 +438,7 @@ PagedCache paged_cache(const Tensor& k, const Tensor& v, const c10::optional<Ten
     TORCH_CHECK_VALUE(s->scalar_type() == torch::kFloat8_e4m3fn && s->is_contiguous() && s->dim() == 4 && s->size(0) == k.size(0) && s->size(1) == k.size(1) && s->size(2) == page &&
                       s->size(3) == hd / 16 && s->device() == k.device(), "PagedKV: scales are contiguous float8_e4m3fn [pages, kv heads, page size, channels / 16] beside the codes");
   for (const Tensor* t : {&k, &v, fp4 ? &*ks : &k, fp4 ? &*vs : &v})
-    TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "PagedKV: the tensors start on 16-byte boundaries");
+    TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->data_ptr()) % 32 == 0, "PagedKV: the tensors start on 32-byte boundaries");
   TORCH_CHECK_VALUE(k.size(0) <= 0x7fffffff && k.size(1) <= 0x7fffffff && page <= (1 << 30), "PagedKV: sizes");
   return {k, v, ks, vs, err, static_cast<int>(hd), static_cast<int>(k.size(1)), static_cast<int>(k.size(0)), __builtin_ctzll(page)};
 }
@@ -475,7 +475,7 @@ void paged_append(const PagedCache& c, const Tensor& k_, const Tensor& v_, const
   no_grad(k_, "paged_append"); no_grad(v_, "paged_append");
   const ghb::PagedRows r = rows_of(c, pages, q_start, lens, start, k_.size(0), "paged_append");
   const Rope rope = rope_of(cos, sin, c.hd, c.k, "paged_append");
-  const Tensor k = whole_heads(k_), v = whole_heads(v_);
+  const Tensor k = whole_heads(k_, 32), v = whole_heads(v_, 32);
   check(ghb::paged_append(r, c.pool(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), is_f32(k), rope.cos, rope.sin, rope.half, rope.n_pos, stream()),
         "paged_append");
 }
@@ -489,7 +489,7 @@ std::tuple<Tensor, Tensor> paged_read(const PagedCache& c, const Tensor& pages, 
   Tensor ko = fill ? at::empty({n, c.heads, c.hd}, opts) : *k_out, vo = fill ? at::empty({n, c.heads, c.hd}, opts) : *v_out;
   for (const Tensor* o : {&ko, &vo})
     TORCH_CHECK(o->dim() == 3 && is_bf16(*o) && o->is_contiguous() && o->size(0) == n && o->size(1) == c.heads && o->size(2) == c.hd && o->device() == c.k.device() &&
-                reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0, "paged_read: out is two contiguous bfloat16 tensors [", n, ", ", c.heads, ", ", c.hd, "], got ", o->sizes());
+                reinterpret_cast<uintptr_t>(o->data_ptr()) % 32 == 0, "paged_read: out is two contiguous bfloat16 tensors [", n, ", ", c.heads, ", ", c.hd, "], got ", o->sizes());
   const ghb::PagedRows r = rows_of(c, pages, q_start, lens, c10::nullopt, n, "paged_read");
   check(ghb::paged_read(r, c.pool(), ko.data_ptr(), vo.data_ptr(), fill, stream()), "paged_read");
   return {ko, vo};
@@ -501,7 +501,7 @@ Tensor paged_attention(const Tensor& q_, const PagedCache& c, const Tensor& page
               "paged_attention: q bfloat16 or float32 [n, a multiple of ", c.heads, ", ", c.hd, "] on the cache's device, got ", q_.sizes());
   TORCH_CHECK(q_.stride(2) == 1, "paged_attention: q with unit inner stride");
   no_grad(q_, "paged_attention");
-  const Tensor q = whole_heads(q_);
+  const Tensor q = whole_heads(q_, 16);
   const bool fill = !out_.has_value();
   Tensor out = fill ? at::empty(q.sizes(), q.options().dtype(torch::kBFloat16)) : *out_;
   TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.sizes() == q.sizes() && out.device() == c.k.device() && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,

@@ -1,8 +1,8 @@
 // Appending to and reading from a paged key/value cache in bfloat16 or 4 bits (layout and checks: paged.cuh).
 //
-// Append: one thread owns 16 consecutive channels (one 4-bit block) of one token, in one key or value head or in several: two 16-byte
-// loads, the rotation, the block's largest magnitude in registers, one 8-byte store of codes and one byte of scale (or two
-// 16-byte stores of bfloat16). Neighbouring threads own neighbouring tokens of one head, whose entries are neighbours in the page: codes
+// Append: one thread owns 16 consecutive channels (one 4-bit block) of one token, in one key or value head or in several: loads of 32
+// bytes, the rotation, the block's largest magnitude in registers, one 8-byte store of codes and one byte of scale (or one
+// 32-byte store of bfloat16). Neighbouring threads own neighbouring tokens of one head, whose entries are neighbours in the page: codes
 // and scales leave as whole sectors. Rotation: channel i < half with channel i + half, by the table row of the token's position
 // counted from the row's start, x cos - y sin and y cos + x sin, rounded once to 32 bits, because a key next to a border of the 4-bit
 // grid must fall on the side where the formula has it. Scale: max / 6 rounded to E4M3, code: x / scale rounded to E2M1,
@@ -24,14 +24,33 @@ __device__ __forceinline__ const int* stage_q_start(const PagedRows& r, int* s) 
   return s;
 }
 
+// 32 bytes a lane and instruction: whole sectors
+__device__ __forceinline__ void load32(const void* p, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+// 16 values as they lie in memory, and as float32
+template <typename T> struct Raw16 { uint32_t w[4 * sizeof(T)]; };
+template <typename T> __device__ __forceinline__ void load16(const T* p, Raw16<T>& r) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) load32(reinterpret_cast<const char*>(p) + 32 * i, r.w + 8 * i);
+}
+__device__ __forceinline__ void widen(const Raw16<float>& r, float* x) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r.w[i]);
+}
+__device__ __forceinline__ void widen(const Raw16<__nv_bfloat16>& r, float* x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { x[2 * i] = __uint_as_float(r.w[i] << 16); x[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u); }
+}
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
   const uint4 u = *reinterpret_cast<const uint4*>(p);
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-    x[2 * i] = f.x; x[2 * i + 1] = f.y;
-  }
+  for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
 __device__ __forceinline__ void load8(const float* p, float* x) {
   const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
@@ -50,18 +69,20 @@ __device__ __forceinline__ float two_products(float a, float c, float b, float s
   return isfinite(r) ? r : sum;          // (a remainder of an infinity is not a number)
 }
 
-// x[0 .. 16) at channels c0 .. of a head at `head`, rotated where they are rotary (half a multiple of 8): co, si are the table's
-// entries of these channels, the sine with the channel's sign.
+// x[0 .. 16) at channels c0 .. of a head at `head`, rotated where they are rotary (half a multiple of 8) by the table's row at co, si.
 template <typename T>
 __device__ __forceinline__ void rotate16(const T* head, int c0, int half, const float* co, const float* si, float* x) {
 #pragma unroll
   for (int g = 0; g < 16; g += 8) {
     const int c = c0 + g;
     if (c >= 2 * half) continue;
-    float y[8];
-    load8(head + (c < half ? c + half : c - half), y);
+    const bool low = c < half;
+    float y[8], cs[8], sn[8];
+    load8(head + (low ? c + half : c - half), y);
+    load8(co + (low ? c : c - half), cs);
+    load8(si + (low ? c : c - half), sn);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[g + i] = two_products(x[g + i], co[g + i], y[i], si[g + i]);
+    for (int i = 0; i < 8; ++i) x[g + i] = two_products(x[g + i], cs[i], y[i], low ? -sn[i] : sn[i]);
   }
 }
 
@@ -73,12 +94,23 @@ __device__ __forceinline__ float quotient(float a, float b, float inv) {
   const float q = __fmul_rn(a, inv);
   return __fmaf_rn(__fmaf_rn(-q, b, a), inv, q);
 }
+// Two at once in the packed instructions: a is two values, nb is -b twice, inv its reciprocal twice.
+__device__ __forceinline__ uint64_t both(float lo, float hi) { uint64_t p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi)); return p; }
+__device__ __forceinline__ float2 quotients(uint64_t a, uint64_t nb, uint64_t inv) {
+  uint64_t q, r;
+  float2 y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(a), "l"(inv));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(nb), "l"(a));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(r), "l"(inv), "l"(q));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(r));
+  return y;
+}
 
 // 16 values -> 8 bytes of codes and the scale's byte.
 __device__ __forceinline__ uint8_t quantize16(float* x, uint2& codes) {
   float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x[i])));
+  for (int i = 0; i < 16; i += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(fabsf(x[i])), "f"(fabsf(x[i + 1])));
   if (!(top <= LARGEST)) {
     top = 0.f;
 #pragma unroll
@@ -92,9 +124,10 @@ __device__ __forceinline__ uint8_t quantize16(float* x, uint2& codes) {
   uint32_t w[2] = {0u, 0u};
   if (s > 0.f) {
     const float inv = __frcp_rn(s);
+    const uint64_t nb = both(-s, -s), inv2 = both(inv, inv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 y = make_float2(quotient(x[2 * i], s, inv), quotient(x[2 * i + 1], s, inv));
+      const float2 y = quotients(both(x[2 * i], x[2 * i + 1]), nb, inv2);
       w[i >> 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(y, __NV_E2M1, cudaRoundNearest)) << (8 * (i & 3));
     }
   }
@@ -104,9 +137,8 @@ __device__ __forceinline__ uint8_t quantize16(float* x, uint2& codes) {
 
 // Where a thread works: packed token j, its row and position, the entry of the position in head 0 (head h: h pages' slots further), or
 // none. Looked up once for all the heads that the thread does.
-struct Spot { long j; int b, t, start; long entry; };
+struct Spot { int b, t, start; long entry; };
 __device__ __forceinline__ bool spot_of(const PagedRows& r, const int* qs, long j, Spot& s) {
-  s.j = j;
   s.entry = -1;
   s.b = row_of(qs, r.B, static_cast<int>(j));
   if (s.b < 0) return false;             // padding
@@ -120,7 +152,7 @@ __device__ __forceinline__ bool spot_of(const PagedRows& r, const int* qs, long 
 
 // One thread: 16 channels (block blk) of one token, in the keys and values (2 Hkv of them) z0 .. z0 + per.
 template <typename T, bool FP4>
-__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(PagedRows r, PagedPool c, const T* k, long k_ts, long k_hs, const T* v, long v_ts,
+__global__ void __launch_bounds__(APPEND_THREADS, 4) paged_append_kernel(PagedRows r, PagedPool c, const T* k, long k_ts, long k_hs, const T* v, long v_ts,
                                                                       long v_hs, const float* cos, const float* sin, int half, int n_pos, int per) {
   __shared__ int sqs[ROWS_IN_SMEM];
   const int* qs = stage_q_start(r, sqs);
@@ -129,51 +161,51 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(PagedRows 
   const int blk = static_cast<int>(item) & (blocks - 1);
   const long j = item >> b_log;
   if (j >= r.n) return;
+  const int z0 = blockIdx.y * per, z1 = min(2 * r.Hkv, z0 + per);
+  auto head_of = [&](int z) { return z >= r.Hkv ? v + j * v_ts + (z - r.Hkv) * v_hs : k + j * k_ts + z * k_hs; };
+  constexpr int AHEAD = sizeof(T) == 2 && !FP4 ? 2 : 1;        // heads on their way together, as registers allow
+  Raw16<T> raw[AHEAD];
+  auto load = [&](int z) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) load16(head_of(min(z + i, z1 - 1)) + blk * 16, raw[i]);
+  };
+  load(z0);        // under way during the look-ups
   Spot s;
   if (!spot_of(r, qs, j, s) || s.entry < 0) return;
-  const int z0 = blockIdx.y * per, z1 = min(2 * r.Hkv, z0 + per);
-  const bool turns = blk * 16 < 2 * half && z0 < r.Hkv;
-  float co[16], si[16];
+  const bool turns = blk * 16 < 2 * half;
   if (half > 0 && z0 < r.Hkv) {
     const int p = s.t - s.start;
     if (p < 0 || p >= n_pos) { *r.err = p < 0 ? ST_START : ST_ROPE; return; }
-    if (turns) {
-#pragma unroll
-      for (int g = 0; g < 16; g += 8) {
-        const int ch = blk * 16 + g, at = ch < half ? ch : ch - half;
-        if (ch >= 2 * half) continue;
-        load8(cos + static_cast<long>(p) * half + at, co + g);
-        load8(sin + static_cast<long>(p) * half + at, si + g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) si[g + i] = ch < half ? -si[g + i] : si[g + i];
-      }
-    }
+    cos += static_cast<long>(p) * half;
+    sin += static_cast<long>(p) * half;
   }
-  for (int z = z0; z < z1; ++z) {
-    const bool value = z >= r.Hkv;
-    const int h = value ? z - r.Hkv : z;
-    const T* head = value ? v + j * v_ts + h * v_hs : k + j * k_ts + h * k_hs;
-    const long e = s.entry + (static_cast<long>(h) << r.page_shift);
-    float x[16];
-    load8(head + blk * 16, x);
-    load8(head + blk * 16 + 8, x + 8);
-    if (turns && !value) rotate16(head, blk * 16, half, co, si, x);
-    if (FP4) {
-      uint2 codes;
-      const uint8_t sb = quantize16(x, codes);
-      uint8_t* base = static_cast<uint8_t*>(value ? c.v : c.k);
-      *reinterpret_cast<uint2*>(base + e * (c.hd >> 1) + blk * 8) = codes;
-      (value ? c.v_scale : c.k_scale)[e * blocks + blk] = sb;
-    } else {
-      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(value ? c.v : c.k) + e * c.hd + blk * 16;
-      uint32_t w[8];
+  for (int zz = z0; zz < z1; zz += AHEAD) {
+    if (zz > z0) load(zz);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __nv_bfloat162 p2 = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&p2);
+    for (int i = 0; i < AHEAD; ++i) {
+      const int z = zz + i;
+      if (z >= z1) break;
+      const bool value = z >= r.Hkv;
+      const int h = value ? z - r.Hkv : z;
+      const long e = s.entry + (static_cast<long>(h) << r.page_shift);
+      float x[16];
+      widen(raw[i], x);
+      if (turns && !value) rotate16(head_of(z), blk * 16, half, cos, sin, x);
+      if (FP4) {
+        uint2 codes;
+        const uint8_t sb = quantize16(x, codes);
+        uint8_t* base = static_cast<uint8_t*>(value ? c.v : c.k);
+        *reinterpret_cast<uint2*>(base + e * (c.hd >> 1) + blk * 8) = codes;
+        (value ? c.v_scale : c.k_scale)[e * blocks + blk] = sb;
+      } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const __nv_bfloat162 p2 = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&p2);
+        }
+        store32(static_cast<__nv_bfloat16*>(value ? c.v : c.k) + e * c.hd + blk * 16, w);
       }
-      reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
 }
@@ -194,15 +226,15 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_read_kernel(PagedRows r,
   for (int z = z0; z < z1; ++z) {
     const bool value = z >= r.Hkv;
     const int h = value ? z - r.Hkv : z;
-    uint4* o = reinterpret_cast<uint4*>((value ? vo : ko) + (j * r.Hkv + h) * c.hd + blk * 16);
-    if (s.entry < 0) { o[0] = make_uint4(0, 0, 0, 0); o[1] = make_uint4(0, 0, 0, 0); continue; }
+    __nv_bfloat16* o = (value ? vo : ko) + (j * r.Hkv + h) * c.hd + blk * 16;
+    uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (s.entry < 0) { store32(o, w); continue; }
     const long e = s.entry + (static_cast<long>(h) << r.page_shift);
     if (FP4) {
       const uint8_t* base = static_cast<const uint8_t*>(value ? c.v : c.k);
       const uint2 codes = *reinterpret_cast<const uint2*>(base + e * (c.hd >> 1) + blk * 8);
       const float sc = e4m3_to_float((value ? c.v_scale : c.k_scale)[e * blocks + blk]);
       const uint32_t cw[2] = {codes.x, codes.y};
-      uint32_t w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const __half2 hv = __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>((cw[i >> 2] >> (8 * (i & 3))) & 0xff), __NV_E2M1));
@@ -210,25 +242,23 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_read_kernel(PagedRows r,
         const __nv_bfloat162 p2 = __floats2bfloat162_rn(f.x * sc, f.y * sc);
         w[i] = *reinterpret_cast<const uint32_t*>(&p2);
       }
-      o[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      o[1] = make_uint4(w[4], w[5], w[6], w[7]);
     } else {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(value ? c.v : c.k) + e * c.hd + blk * 16);
-      const uint4 a = src[0], b4 = src[1];
-      o[0] = a; o[1] = b4;
+      load32(static_cast<const __nv_bfloat16*>(value ? c.v : c.k) + e * c.hd + blk * 16, w);
     }
+    store32(o, w);
   }
 }
 
 namespace {
-// The grid: CTAs over (token, 16-channel block), and over the 2 Hkv keys and values, `per` of them a thread. One where that leaves
-// enough threads to fill the GPU (a decode step: latency); as many as still do at large sizes, where a thread's look-up of its row and
-// page costs as much as a block (81k tokens of 8 heads, 4 bits: append 126 us at one, NNN at all; reading back 56 and NNN).
+// The grid: CTAs over (token, 16-channel block), and over the 2 Hkv keys and values, `per` of them a thread: one where that leaves
+// enough threads to fill the GPU (a decode step: latency), more where `ctas_sm` CTAs an SM remain, so that a thread's look-up of its row
+// and page serves several blocks. Measured, per = 1 / the rule: 19k tokens of 2 heads of 128 appended in bfloat16 16.8 / 14.8 us
+// (CTAs of 64 registers: 4 an SM are one wave), 81k tokens of 8 heads of 64 read back from 4 bits 56 / 42 us (more, smaller ones).
 struct Grid { dim3 g; int per; bool ok; };
-Grid append_grid(const PagedRows& r, int hd, int half) {
+Grid grid_of(const PagedRows& r, int hd, int half, int ctas_sm) {
   const long x = (static_cast<long>(r.n) * (hd >> 4) + APPEND_THREADS - 1) / APPEND_THREADS;
   const long pairs = 2l * r.Hkv;
-  long per = x * pairs / (148l * 16);          // 16 CTAs an SM
+  long per = x * pairs / (148l * ctas_sm);
   per = per < 1 ? 1 : per > pairs ? pairs : per;
   const long y = (pairs + per - 1) / per;
   const bool ok = x <= 0x7fffffffL && y <= 65535 && (hd == 64 || hd == 128 || hd == 256) && half % 8 == 0 && 2 * half <= hd;
@@ -239,7 +269,7 @@ Grid append_grid(const PagedRows& r, int hd, int half) {
 int paged_append(const PagedRows& r, const PagedPool& c, const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, bool f32,
                  const float* cos, const float* sin, int half, int n_pos, cudaStream_t st) {
   if (r.n == 0) return 0;
-  const Grid g = append_grid(r, c.hd, half);
+  const Grid g = grid_of(r, c.hd, half, 4);
   if (!g.ok) return 1;
 #define GHB_APPEND(T, F) paged_append_kernel<T, F><<<g.g, APPEND_THREADS, 0, st>>>(r, c, static_cast<const T*>(k), k_ts, k_hs, static_cast<const T*>(v), v_ts, v_hs, cos, sin, half, n_pos, g.per)
   if (f32) { if (c.fp4) GHB_APPEND(float, true); else GHB_APPEND(float, false); }
@@ -250,7 +280,7 @@ int paged_append(const PagedRows& r, const PagedPool& c, const void* k, long k_t
 
 int paged_read(const PagedRows& r, const PagedPool& c, void* ko, void* vo, bool fill, cudaStream_t st) {
   if (r.n == 0) return 0;
-  const Grid g = append_grid(r, c.hd, 0);
+  const Grid g = grid_of(r, c.hd, 0, 16);
   if (!g.ok) return 1;
   if (c.fp4) paged_read_kernel<true><<<g.g, APPEND_THREADS, 0, st>>>(r, c, static_cast<__nv_bfloat16*>(ko), static_cast<__nv_bfloat16*>(vo), fill, g.per);
   else paged_read_kernel<false><<<g.g, APPEND_THREADS, 0, st>>>(r, c, static_cast<__nv_bfloat16*>(ko), static_cast<__nv_bfloat16*>(vo), fill, g.per);

@@ -21,12 +21,12 @@ namespace ghb {
 
 namespace cg = cooperative_groups;
 
-constexpr int VWARPS = 16;
+constexpr int VWARPS = 16;         // at most, a CTA
 constexpr int VMAXCL = 8;
 
 template <typename T> __device__ __forceinline__ double to_double(T x) { return static_cast<double>(static_cast<float>(x)); }
 
-// Four consecutive weights at j (j + 3 < V): p, or max(p - q, 0), or p without token x. Anything not above zero (NaN too) is 0.
+// The weight of a token: p, or max(p - q, 0), or p without token x. Anything not above zero (NaN too) is 0.
 template <typename T>
 struct Weights {
   const T* p; const T* q; int x;       // q null: no subtraction; x: the token left out, or -1
@@ -35,21 +35,6 @@ struct Weights {
     double w = to_double(p[j]);
     if (q) w -= to_double(q[j]);
     return (w > 0.0 && j != x) ? w : 0.0;
-  }
-  __device__ __forceinline__ void four(int j, double* w) const {
-    float a[4], b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (wide) {
-      load4(p + j, a);
-      if (q) load4(q + j, b);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { a[i] = static_cast<float>(p[j + i]); if (q) b[i] = static_cast<float>(q[j + i]); }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const double d = static_cast<double>(a[i]) - static_cast<double>(b[i]);
-      w[i] = (d > 0.0 && j + i != x) ? d : 0.0;
-    }
   }
   static __device__ __forceinline__ void load4(const float* s, float* a) {
     const float4 u = *reinterpret_cast<const float4*>(s);
@@ -62,28 +47,69 @@ struct Weights {
   }
 };
 
+// The lane's whole groups of four at j, j + stride, .. below hi, DEEP of them at a time: all loads of a step stand before its first sum
+// and no branch between them (in place of a group behind the end the last one is read, and not counted), so that 16 bytes * DEEP * (one or two
+// arrays) a lane are under way. A rest of one to three tokens is left.
+template <typename T, bool Q>
+__device__ __forceinline__ void wide_sum(const Weights<T>& w, int j, int hi, int stride, double& s0, double& s1) {
+  constexpr int DEEP = 4;
+  const int end = (hi & ~3) - 4;          // the last whole group
+  for (; j <= end; j += DEEP * stride) {
+    float a[DEEP][4], b[DEEP][4];
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) {
+      const int at = min(j + i * stride, end);
+      w.load4(w.p + at, a[i]);
+      if (Q) w.load4(w.q + at, b[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const double d = Q ? static_cast<double>(a[i][c]) - static_cast<double>(b[i][c]) : static_cast<double>(a[i][c]);
+        (i & 1 ? s1 : s0) += d > 0.0 && j + i * stride <= end && j + i * stride + c != w.x ? d : 0.0;
+      }
+  }
+}
+// The sum of the lane's groups (lo a multiple of four; the whole range is walked where stride is 128 and j = lo + 4 lane).
+template <typename T>
+__device__ __forceinline__ double lane_sum(const Weights<T>& w, int j, int hi, int stride) {
+  double s0 = 0.0, s1 = 0.0;
+  if (w.wide) {
+    if (w.q) wide_sum<T, true>(w, j, hi, stride, s0, s1); else wide_sum<T, false>(w, j, hi, stride, s0, s1);
+    const int rest = hi & ~3;                 // the vocabulary's last one to three tokens: a group that nobody read whole
+    if (rest < hi && rest >= j && (rest - j) % stride == 0) for (int i = rest; i < hi; ++i) s0 += w.one(i);
+  } else {
+    for (; j < hi; j += stride) for (int i = j; i < min(hi, j + 4); ++i) s0 += w.one(i);
+  }
+  return s0 + s1;
+}
+
 template <typename T>
 __device__ __forceinline__ double range_sum(const Weights<T>& w, int lo, int hi, int lane) {
-  double s0 = 0.0, s1 = 0.0;
-  int j = lo + lane * 4;
-  for (; j + 3 * 128 + 3 < hi; j += 4 * 128) {       // four independent groups in flight
-    double a[4][4];
+  double s = lane_sum(w, lo + lane * 4, hi, 128);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w.four(j + 128 * i, a[i]);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// 1 / 32 of the range a lane, so that all of it is on its way at once: the lane's part that the threshold falls into, and what lies
+// before it in `before`; the last part of positive weight where none does. The part is walked by range_pick.
+template <typename T>
+__device__ __forceinline__ void narrow(const Weights<T>& w, int& lo, int& hi, double& before, double thr, int lane) {
+  const int part = ((hi - lo + 31) / 32 + 3) & ~3, l0 = min(hi, lo + lane * part), l1 = min(hi, l0 + part);
+  const double s = l0 < l1 ? lane_sum(w, l0, l1, 4) : 0.0;
+  double upto = s;
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      s0 += (a[i][0] + a[i][1]) + (a[i][2] + a[i][3]);
-      s1 += (a[i + 1][0] + a[i + 1][1]) + (a[i + 1][2] + a[i + 1][3]);
-    }
-  }
-  for (; j < hi; j += 128) {
-    if (j + 3 < hi) { double a[4]; w.four(j, a); s0 += (a[0] + a[1]) + (a[2] + a[3]); }
-    else for (int i = j; i < hi; ++i) s0 += w.one(i);
-  }
-  s0 += s1;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-  return s0;
+  for (int o = 1; o < 32; o <<= 1) { const double up = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += up; }
+  double ahead = __shfl_up_sync(0xffffffffu, upto, 1);
+  if (lane == 0) ahead = 0.0;
+  const unsigned hits = __ballot_sync(0xffffffffu, s > 0.0 && before + upto > thr), lives = __ballot_sync(0xffffffffu, s > 0.0);
+  if (!lives) return;
+  const int at = hits ? __ffs(hits) - 1 : 31 - __clz(lives);
+  before += __shfl_sync(0xffffffffu, ahead, at);
+  lo = __shfl_sync(0xffffffffu, l0, at);
+  hi = __shfl_sync(0xffffffffu, l1, at);
 }
 
 // First token of lo .. hi whose running sum, from `before` on, exceeds thr; the last one of positive weight where none does.
@@ -119,7 +145,7 @@ __device__ __forceinline__ int range_pick(const Weights<T>& w, int lo, int hi, d
 }
 
 template <typename T>
-__global__ void __launch_bounds__(VWARPS * 32) verify_drafts_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(VWARPS * 32, 2) verify_drafts_kernel(VerifyArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ double totals[2][VMAXCL * VWARPS];
   __shared__ int s_kept;
@@ -157,8 +183,8 @@ __global__ void __launch_bounds__(VWARPS * 32) verify_drafts_kernel(VerifyArgs a
   w.p = target + kept * a.t_ns;
   w.q = refused && draft ? draft + kept * a.d_ns : nullptr;
   w.x = refused && !draft ? static_cast<int>(drafts[kept] >= 0 && drafts[kept] < a.V ? drafts[kept] : -1) : -1;
-  w.wide = (reinterpret_cast<uintptr_t>(w.p) | reinterpret_cast<uintptr_t>(w.q)) % (4 * sizeof(T)) == 0;
-  const int ranges = CL * VWARPS, mine = rank * VWARPS + warp;
+  w.wide = (reinterpret_cast<uintptr_t>(w.p) | reinterpret_cast<uintptr_t>(w.q)) % (4 * sizeof(T)) == 0 && a.V >= 4;
+  const int warps = static_cast<int>(blockDim.x) >> 5, ranges = CL * warps, mine = rank * warps + warp;
   const int per = ((a.V + ranges - 1) / ranges + 3) & ~3;
   const int lo = min(a.V, mine * per), hi = min(a.V, lo + per);
   double total = 0.0, t4[4], ahead = 0.0;
@@ -204,7 +230,9 @@ __global__ void __launch_bounds__(VWARPS * 32) verify_drafts_kernel(VerifyArgs a
   }
   long* out = a.tokens + static_cast<long>(b) * (a.N + 1);
   if (owner == mine) {
-    const int pick = range_pick(w, lo, hi, before, thr, lane);
+    int from = lo, to = hi;
+    narrow(w, from, to, before, thr, lane);
+    const int pick = range_pick(w, from, to, before, thr, lane);
     if (lane == 0) out[kept] = pick < 0 ? 0 : pick;
   }
   if (rank == 0) {
@@ -220,12 +248,18 @@ __global__ void __launch_bounds__(VWARPS * 32) verify_drafts_kernel(VerifyArgs a
 int verify_drafts(const VerifyArgs& a, cudaStream_t st) {
   if (a.B == 0) return 0;
   if (a.V < 1 || a.N < 0 || a.B > 0x7fffffff / VMAXCL) return 1;
-  // CTAs a row: as many as keep the grid within two an SM (one wave), each with some hundreds of probabilities a warp
-  int cl = 1;
-  while (cl < VMAXCL && a.V >= 2 * cl * 4096 && static_cast<long>(a.B) * cl * 2 <= 296) cl *= 2;
+  // CTAs a row: 8, 4 or 2 of 8 warps, as long as the grid leaves an eighth of the GPU's places (4 such CTAs an SM) free: whole clusters
+  // wait for places in one GPC. Two of 16 warps where those still are one wave. Measured at 64,000 float32 probabilities with a
+  // draft's, 8 / 4 / 2 CTAs of 8 warps, 2 of 16: 24 rows 8.2 / 9.8 / 14.4, 11.1 us; 96 rows 17.3 / 14.6 / 19.8, 16.6 us;
+  // 148 rows 24.4 / 22.4 / 22.2, 18.5 us; 600 rows 74 / 58 / 56, 64 us. Cluster sizes that are no powers of two were slower than both
+  // neighbours. A warp has 128 probabilities at least.
+  int cl = VMAXCL, warps = VWARPS / 2;
+  while (cl > 2 && static_cast<long>(a.B) * cl > 148 * 7 / 2) cl >>= 1;
+  if (cl == 2 && a.B <= 148) warps = VWARPS;
+  while (cl > 1 && a.V < 128 * warps * cl) cl >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.B * cl);
-  cfg.blockDim = dim3(VWARPS * 32);
+  cfg.blockDim = dim3(warps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
