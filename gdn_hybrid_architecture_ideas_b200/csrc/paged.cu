@@ -152,7 +152,7 @@ __device__ __forceinline__ bool spot_of(const PagedRows& r, const int* qs, long 
 
 // One thread: 16 channels (block blk) of one token, in the keys and values (2 Hkv of them) z0 .. z0 + per.
 template <typename T, bool FP4>
-__global__ void __launch_bounds__(APPEND_THREADS, 4) paged_append_kernel(PagedRows r, PagedPool c, const T* k, long k_ts, long k_hs, const T* v, long v_ts,
+__global__ void __launch_bounds__(APPEND_THREADS, 3) paged_append_kernel(PagedRows r, PagedPool c, const T* k, long k_ts, long k_hs, const T* v, long v_ts,
                                                                       long v_hs, const float* cos, const float* sin, int half, int n_pos, int per) {
   __shared__ int sqs[ROWS_IN_SMEM];
   const int* qs = stage_q_start(r, sqs);
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) paged_append_kernel(PagedRo
     sin += static_cast<long>(p) * half;
   }
   for (int zz = z0; zz < z1; zz += AHEAD) {
-    if (zz > z0) load(zz);
+    if (AHEAD > 1 && zz > z0) load(zz);
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int z = zz + i;
@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) paged_append_kernel(PagedRo
       const long e = s.entry + (static_cast<long>(h) << r.page_shift);
       float x[16];
       widen(raw[i], x);
+      if (AHEAD == 1 && z + 1 < z1) load(z + 1);        // while this one is rounded
       if (turns && !value) rotate16(head_of(z), blk * 16, half, cos, sin, x);
       if (FP4) {
         uint2 codes;
@@ -253,7 +254,7 @@ namespace {
 // The grid: CTAs over (token, 16-channel block), and over the 2 Hkv keys and values, `per` of them a thread: one where that leaves
 // enough threads to fill the GPU (a decode step: latency), more where `ctas_sm` CTAs an SM remain, so that a thread's look-up of its row
 // and page serves several blocks. Measured, per = 1 / the rule: 19k tokens of 2 heads of 128 appended in bfloat16 16.8 / 14.8 us
-// (CTAs of 64 registers: 4 an SM are one wave), 81k tokens of 8 heads of 64 read back from 4 bits 56 / 42 us (more, smaller ones).
+// (3 CTAs an SM reside), 81k tokens of 8 heads of 64 read back from 4 bits 56 / 42 us (more, smaller ones).
 struct Grid { dim3 g; int per; bool ok; };
 Grid grid_of(const PagedRows& r, int hd, int half, int ctas_sm) {
   const long x = (static_cast<long>(r.n) * (hd >> 4) + APPEND_THREADS - 1) / APPEND_THREADS;
