@@ -26,7 +26,8 @@
 // part of a tile that lies in one page is contiguous, so with pages of a tile or more the addresses are one base and constants.
 // (Bulk copies cost one instruction instead of nine, but about 32 clocks each in the SM's copy engine, which bound
 // the loop; one more warp that loads for all the others ties them to the slowest. Both were measured slower.) What no
-// row sees gets scales of zero (4 bits), so that its values are zero.
+// row sees gets scales of zero (4 bits), so that its values are zero; in bfloat16 a tile with masked infinities or NaN is summed
+// position by position.
 #include <atomic>
 
 #include "paged.cuh"
@@ -54,7 +55,6 @@ template <bool FP4, int HD>
 struct Geo : Cfg<FP4, HD> {
   using B = Cfg<FP4, HD>;
   static constexpr int MT = B::MT, ST = B::ST;
-  static constexpr bool SPLIT = ST == 1;             // one stage: the values arrive while the scores are formed
   static constexpr int TILE = 16 * MT;
   static constexpr int H = HD / 64;                  // 64-channel slices
   static constexpr int ROW = FP4 ? HD / 2 : HD * 2;  // bytes of a position
@@ -370,7 +370,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
         const long off = static_cast<long>(e) * GEO::ROW;
 #pragma unroll
         for (int i = 0; i < N; ++i) cp16(st + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH), k_lane + off + i * 512);
-        if constexpr (GEO::SPLIT) cp_commit();
 #pragma unroll
         for (int i = 0; i < N; ++i) cp16(st + GEO::KB + place_of((i * 32 + lane) / CH, (i * 32 + lane) % CH), v_lane + off + i * 512);
         if constexpr (FP4) {
@@ -393,7 +392,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
           }
         };
         copy(st, p.c.k);
-        if constexpr (GEO::SPLIT) cp_commit();
         copy(st + GEO::KB, p.c.v);
         if constexpr (FP4) {
 #pragma unroll
@@ -529,20 +527,44 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
 #pragma unroll
       for (int i = 0; i < ST - 1; ++i) on_ring[i] = on_ring[i + 1];        // the masks travel with the ring
       uint8_t* st = ring + stage * GEO::STAGE;
-      cp_wait<GEO::SPLIT ? 1 : ST - 1>();
+      cp_wait<ST - 1>();
       __syncwarp();
       stage = stage == ST - 1 ? 0 : stage + 1;
       if (on) {
         const bool masked = on != all_on || first < start || first + TILE - 1 > p_first;
         if (FP4 && masked) {
-          // what no row sees may hold anything: its scales become zero, so that its values are zero
+          // What no row sees may hold anything: its scales become zero, so that its values are zero. A scale that is not a number
+          // where some rows see it and others do not: zero too, and the block's channels of the rows that see it are set by hand.
+          bool odd = false;
           for (int pos = lane; pos < TILE; pos += 32) {
-            if (!((on >> (pos >> c_shift)) & 1) || first + pos < start || first + pos > p_last) {
+            uint32_t* sw = reinterpret_cast<uint32_t*>(st + 2 * GEO::KB + GEO::SB + pos * GEO::S);
+            const bool hidden = !((on >> (pos >> c_shift)) & 1) || first + pos < start || first + pos > p_last;
 #pragma unroll
-              for (int i = 0; i < GEO::S / 4; ++i) *reinterpret_cast<uint32_t*>(st + 2 * GEO::KB + GEO::SB + pos * GEO::S + 4 * i) = 0u;
+            for (int i = 0; i < GEO::S / 4; ++i) {
+              if (hidden) sw[i] = 0u;
+              odd |= (((sw[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
             }
           }
           __syncwarp();
+#pragma unroll 1
+          for (int again = opaque(__any_sync(0xffffffffu, odd)); again > 0; again = opaque(0)) {
+#pragma unroll 1
+            for (int pos = 0; pos < TILE; ++pos)
+#pragma unroll
+              for (int hs = 0; hs < H; ++hs) {
+                uint8_t* sb = st + 2 * GEO::KB + GEO::SB + pos * GEO::S + hs * 4 + (g >> 1);
+                const bool nan = (*sb & 0x7f) == 0x7f;
+                __syncwarp();
+                if (nan) {
+                  *sb = 0;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) if (first + pos <= prow[e & 1]) o[hs * 4 + i][e] = NAN;
+                }
+              }
+            __syncwarp();
+          }
         }
         float s[MT][4];
         // Products that add into one accumulator wait for one another: wide heads take two by turns of their slices, bfloat16 two more
@@ -740,10 +762,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
           for (int q = 0; q < 2; ++q)
             pk[mt][q] = pack<FP4>(exp2_fast(fmaf(s[mt][2 * q], mul[0], ref0)), exp2_fast(fmaf(s[mt][2 * q + 1], mul[1], ref1)));
         // ---- O^T += V^T P^T
-        if constexpr (GEO::SPLIT) {
-          cp_wait<0>();
-          __syncwarp();
-        }
         bool plain = true;
         if constexpr (!FP4) {
           // A masked position's value may be infinite or NaN, and 0 times it would reach rows that do not see it: such a

@@ -943,3 +943,100 @@ def test_loopspec_samples_by_the_acceptance_rule(monkeypatch):
         model.loop_embedding.zero_()
     _, stats = loopspec.LoopSpec(model).generate(prompt, doc, dec, 8, greedy=False, generator=torch.Generator().manual_seed(3))
     assert stats.acceptance == 1.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_kernel_scales_that_are_no_numbers_reach_only_who_sees_them(hd):
+    """4 bits: one value scale of a row's last new token is NaN. Its own query gets NaN in that block of 16 channels; the two before it, which
+    do not see it (their weights there are zero before and after), and every other channel keep what they had."""
+    rows, page, block = [(21, 3, 5), (40, 1, 0)], 16, 2
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    cache, _ = _random_cache(n_pages, page, 2, hd, "fp4")
+    q = torch.randn(n, 8, hd, device="cuda").bfloat16()
+    args = (q, cache, *(t.cuda() for t in (pages, q_start, lens)))
+    before = ops.paged_attention(*args, start=start.cuda())
+    cache.v_scale.view(torch.uint8)[int(pages[0, 23 // page]), 1, 23 % page, block] = 0x7f
+    got = ops.paged_attention(*args, start=start.cuda())
+    hit = torch.zeros(n, 8, hd, dtype=torch.bool, device="cuda")
+    hit[2, 4:, 16 * block:16 * block + 16] = True               # query heads 4 .. 7 read key head 1
+    assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], before[~hit])
+    cache.v_scale.view(torch.uint8)[int(pages[0, 8 // page]), 0, 8 % page, 0] = 0xff          # in a place that all of the row's queries see
+    got = ops.paged_attention(*args, start=start.cuda())
+    assert bool(got[:3, :4, :16].isnan().all()) and torch.equal(got[3], before[3]) and bool(torch.isfinite(got[:3, :4, 16:]).all())
+    _status_clean()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,hd", [("fp4", 64), ("bf16", 128)])
+def test_more_rows_than_a_block_has_threads(fmt, hd):
+    """1100 ragged rows (the tables' search leaves shared memory, the attention's prefix sum takes several steps), every third without new
+    tokens, pairs of rows over the same pages."""
+    page = 8
+    rows = [((7 * b) % 31, 0 if b % 3 == 2 else 1 + b % 2, 0) for b in range(1100)]
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    for b in range(0, 1100, 6):
+        total, new = rows[b][0] + rows[b][1], rows[b + 1][1]
+        if total >= new:
+            pages[b + 1], rows[b + 1], lens[b + 1] = pages[b], (total - new, new, 0), total
+    cache, cpu = _random_cache(n_pages, page, 1, hd, fmt)
+    q = torch.randn(n, 2, hd).bfloat16()
+    _check_attention(q, cache, cpu, rows, pages, q_start, lens, start, _tables(64, 8), None, page=page)
+    dev = [t.cuda() for t in (pages, q_start, lens)]
+    back = ops.paged_read(cache, *dev, n)
+    for x, y in zip(back, ops.paged_read(cpu, pages, q_start, lens, n)):
+        assert torch.equal(x.cpu(), y)
+    _status_clean()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,V,dtype,with_draft", [(140, 2, 4100, "float32", True), (700, 1, 1003, "float32", True), (170, 3, 6001, "bfloat16", False), (2, 2, 3, "float32", True),
+                                                    (60, 2, 12288, "bfloat16", True), (3, 1, 5, "bfloat16", True)])
+def test_verify_kernel_at_every_split_of_a_row(B, N, V, dtype, with_draft):
+    """Batches that take 8, 4 and 2 CTAs a row, of 8 and of 16 warps, and vocabularies of less than a group of four."""
+    test_verify_kernel(B, N, V, dtype, with_draft)
+
+
+@pytest.mark.gpu
+def test_forward_only_and_refused_caches():
+    rows, page = [(20, 1, 0)], 16
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page, device="cuda")
+    cache, _ = _random_cache(n_pages, page, 2, 64, "fp4")
+    q = torch.randn(n, 4, 64, device="cuda", requires_grad=True)
+    k = torch.randn(n, 2, 64, device="cuda", requires_grad=True)
+    for call in (lambda: ops.paged_attention(q, cache, pages, q_start, lens), lambda: ops.paged_append(cache, k, k.detach(), pages, q_start, lens),
+                 lambda: ops.paged_append(cache, k.detach(), k, pages, q_start, lens)):
+        with pytest.raises(RuntimeError, match="forward only"):
+            call()
+    with torch.no_grad():
+        assert not ops.paged_attention(q, cache, pages, q_start, lens).requires_grad
+    big = torch.zeros(5 * 2 * 16 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+    x = big[:-8].view(5, 2, 16, 64)
+    for match, bad in {"power of two": (x[:, :, :12].contiguous(),) * 2, "32-byte": (big[8:].view(5, 2, 16, 64),) * 2, "contiguous": (x.transpose(1, 2),) * 2, "one type": (x, x.float()),
+                       "bfloat16, or uint8": (x.half(), x.half()), "alone": (cache.k, cache.v), "float8": (cache.k, cache.v, cache.k_scale.float(), cache.v_scale.float())}.items():
+        with pytest.raises(ValueError, match=match):
+            ops.PagedKV(*bad)
+    with pytest.raises(RuntimeError, match="16-byte"):
+        t = torch.zeros(65 * 8 + 4, device="cuda")[1:521].view(65, 8)
+        ops.paged_attention(q.detach(), cache, pages, q_start, lens, rope=(t, t))
+
+
+@pytest.mark.gpu
+def test_two_caches_on_two_streams_at_once():
+    """Attention over two caches launched side by side on two streams, many times: each equals its own result alone."""
+    rows, page = [(900, 1, 0), (77, 2, 5)], 32
+    tabs = _batch(rows, page, device="cuda")
+    caches = [_random_cache(tabs[5], page, 2, 64, f, seed=i)[0] for i, f in enumerate(("fp4", "bf16"))]
+    q = torch.randn(tabs[4], 8, 64, device="cuda").bfloat16()
+    alone = [ops.paged_attention(q, c, *tabs[:3], start=tabs[3]) for c in caches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in caches]
+    outs = [[], []]
+    for _ in range(20):
+        for i, (s, c) in enumerate(zip(streams, caches)):
+            with torch.cuda.stream(s):
+                outs[i].append(ops.paged_attention(q, c, *tabs[:3], start=tabs[3]))
+    torch.cuda.synchronize()
+    for o, want in zip(outs, alone):
+        assert all(torch.equal(x, want) for x in o)
+    _status_clean()
