@@ -51,6 +51,7 @@ def parse():
                     help="GEMM precision of the layers' projections: bf16 (the headline), block-scaled MXFP8 on the tensor cores, or the NVFP4 recipe")
     ap.add_argument("--mode", default="train", choices=["train", "decode"], help="decode: static-cache greedy decode tokens/s")
     ap.add_argument("--kv", default="gqa", choices=["gqa", "grid"], help="decode: KV sharing of the attention layers")
+    ap.add_argument("--kv-cache", default="static", choices=["static", "paged", "paged_fp4"], help="decode: contiguous cache, or pages in bfloat16 or 4 bits")
     ap.add_argument("--prompt", type=int, default=32768, help="decode: prompt length")
     ap.add_argument("--batch", type=int, default=64, help="decode: rows per GPU")
     return ap.parse_args()
@@ -232,7 +233,7 @@ def run_decode(args) -> dict:
     model = build_model(cfg).to(dev)
     flat, _ = build_optimizer(model, C.OptimConfig(), dev, torch.bfloat16)      # bf16 weight copies for the GEMMs
     B, P = args.batch, args.prompt
-    eng = DecodeEngine(model, B, P + 2 * args.steps + args.warmup + 8)      # device-timed and end-to-end loops both generate `steps` tokens
+    eng = DecodeEngine(model, B, P + 2 * args.steps + args.warmup + 8, kv_cache=args.kv_cache)      # device-timed and end-to-end loops both generate `steps` tokens
     g = torch.Generator().manual_seed(1 + (0 if dp is None else dp.rank))
     prompts = torch.randint(0, VOCAB, (B, P), generator=g).pin_memory().to(dev, non_blocking=True)
     t0 = time.time()
@@ -274,6 +275,8 @@ def run_decode(args) -> dict:
            "clocks": clocks, "e2e": {"value": B * world / (e2e_ms / 1e3), "unit": "tokens/s", "ms_per_step": e2e_ms,
                                     "h2d_bytes_per_step": B * 8, "d2h_bytes_per_step": B * 8},
            "gpu_launches": args.steps, "impl": "ours"}
+    if args.kv_cache != "static":
+        out["config"]["kv_cache"] = args.kv_cache
     if dp is not None:
         dp.close()
     return out

@@ -28,6 +28,11 @@
 // the loop; one more warp that loads for all the others ties them to the slowest. Both were measured slower.) What no
 // row sees gets scales of zero (4 bits), so that its values are zero; in bfloat16 a tile with masked infinities or NaN is summed
 // position by position.
+//
+// Measured: 64 rows of 32k positions, 16 heads over 4 of 64, under a cap: 4 bits 155 us (604 MB, 0.59 of the copy's rate; 60% of the issue
+// slots: the conversion of every entry for each block of 8 query rows bounds it), bfloat16 362 us (0.90). About 20 us of a call are fixed (the
+// share, the queries, the first tiles, joining warps and CTAs): 12 rows of up to 9k positions of 2 heads of 256 in bfloat16 35 us
+// for 17 us of bytes, one row 11 us.
 #include <atomic>
 
 #include "paged.cuh"

@@ -13,6 +13,9 @@
 // owns one contiguous range of the vocabulary, sums it (pass 1: all bytes of the row, once), the totals of all warps meet
 // in the shared memory of every CTA of the cluster, each warp finds the range that the threshold falls into, and the one
 // warp that owns it walks it again (pass 2: its range alone, from L1 / L2). No workspace, no atomics, one launch.
+//
+// Bound by latency: which row is read follows from three dependent loads, and each of the clusters' meetings waits for its slowest
+// warp. 96 rows of 64,000 float32 probabilities with a draft's (49 MB): 16 us from L2, 26 us from memory (floor 7.5).
 #include <cooperative_groups.h>
 
 #include "paged.cuh"

@@ -5,6 +5,8 @@
     python scripts/op_bench.py gdn_prep --B 2 --L 4096
     python scripts/op_bench.py gemm --M 65536 --N 1024 --K 1024 --layout nt
     python scripts/op_bench.py rmsnorm --rows 65536 --d 1024
+    python scripts/op_bench.py paged --cache fp4 --B 64 --L 32768 --Hkv 4 --cap 2048
+    python scripts/op_bench.py verify --B 96 --drafts 5 --vocab 64000
 
 Prints one JSON line per op with milliseconds per call and the achieved rate against the op's algorithmic FLOPs or
 bytes. `--iters 1 --warmup 0` gives a run short enough to capture under a profiler. Inputs are larger than the L2
@@ -278,9 +280,50 @@ def bench_decode_attention(a):
     return {"op": "decode_attention", "B": B, "T": T, "Hq": Hq, "Hkv": Hkv, "ms": ms, "gbs": nb / ms / 1e6}
 
 
+def bench_paged(a):
+    """One decode step's cache calls over B rows of L cached positions: a token a row appended, attention over the pages, and the
+    read-back of the whole cache."""
+    from gdn_hybrid_architecture_ideas_b200 import ops
+    B, T, hd, page = a.B, a.L, a.hd, 64
+    width = -(-T // page)
+    cache = ops.PagedKV.zeros(B * width, page, a.Hkv, hd, a.cache, "cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    pages = torch.randperm(B * width, device="cuda").to(torch.int32).view(B, width)
+    one, full, lens = torch.arange(B + 1, **i32), torch.arange(B + 1, **i32) * T, torch.full((B,), T, **i32)
+    k, v = (torch.randn(B * T, a.Hkv, hd, device="cuda", dtype=BF16) for _ in range(2))
+    ang = torch.arange(max(T, a.cap + 1), device="cuda")[:, None] * (1e7 ** (-torch.arange(8, device="cuda") / 8))[None]
+    rope = (ang.cos().float().contiguous(), ang.sin().float().contiguous())
+    cap = a.cap if a.cap > 0 else None
+    q = torch.randn(B, a.Hq, hd, device="cuda", dtype=BF16)
+    key_rope = rope if cap is None else None
+    ms_p = timed(lambda: ops.paged_append(cache, k, v, pages, full, lens, rope=key_rope), a.iters, a.warmup)
+    ms_s = timed(lambda: ops.paged_append(cache, k[:B], v[:B], pages, one, lens, rope=key_rope), a.iters, a.warmup)
+    ms_a = timed(lambda: ops.paged_attention(q, cache, pages, one, lens, rope=rope, cap=cap), a.iters, a.warmup)
+    del v
+    out = (k, torch.empty_like(k))
+    ms_r = timed(lambda: ops.paged_read(cache, pages, full, lens, B * T, out=out), a.iters, a.warmup)
+    entry = 2 * a.Hkv * (hd * 2 if a.cache == "bf16" else hd // 2 + hd // 16)
+    return {"op": "paged", "cache": a.cache, "B": B, "T": T, "Hq": a.Hq, "Hkv": a.Hkv, "hd": hd, "cap": cap, "append_all_ms": ms_p, "append_step_ms": ms_s,
+            "attention_ms": ms_a, "attention_gbs": B * T * entry / ms_a / 1e6, "read_all_ms": ms_r,
+            "append_gbs": B * T * (entry + 4 * a.Hkv * hd) / ms_p / 1e6, "read_gbs": B * T * (entry + 4 * a.Hkv * hd) / ms_r / 1e6}
+
+
+def bench_verify(a):
+    from gdn_hybrid_architecture_ideas_b200 import ops
+    B, N, V = a.B, a.drafts, a.vocab
+    target, draft = torch.softmax(torch.randn(B, N + 1, V, device="cuda"), -1), torch.softmax(torch.randn(B, N, V, device="cuda"), -1)
+    drafts = torch.randint(0, V, (B, N), device="cuda")
+    u, us = torch.rand(B, N, device="cuda"), torch.rand(B, device="cuda")
+    ms = timed(lambda: ops.verify_drafts(target, draft, drafts, u, us), a.iters, a.warmup)
+    return {"op": "verify", "B": B, "drafts": N, "vocab": V, "ms": ms, "gbs": 2 * B * V * 4 / ms / 1e6}
+
+
 def main():
     p = argparse.ArgumentParser()
-    p.add_argument("op", choices=["attention", "gdn", "gdn_prep", "gemm", "gemm_mx", "rmsnorm", "depth_mix", "swiglu", "lm_head", "adamw", "decode_attention"])
+    p.add_argument("op", choices=["attention", "gdn", "gdn_prep", "gemm", "gemm_mx", "rmsnorm", "depth_mix", "swiglu", "lm_head", "adamw", "decode_attention", "paged", "verify"])
+    p.add_argument("--cache", choices=["bf16", "fp4"], default="fp4", help="paged: what the pages hold")
+    p.add_argument("--hd", type=int, default=64, choices=[64, 128, 256], help="paged: channels of a head")
+    p.add_argument("--drafts", type=int, default=5, help="verify: drafted tokens a row")
     p.add_argument("--kv", choices=["gqa", "grid"], default="gqa", help="decode_attention: grouped KV heads or the 4 x 4 grid's raw components")
     p.add_argument("--sources", type=int, default=4)
     p.add_argument("--ffn", type=int, default=2816)
@@ -306,7 +349,7 @@ def main():
     a = p.parse_args()
     res = {"attention": bench_attention, "gdn": bench_gdn, "gdn_prep": bench_gdn_prep, "gemm": bench_gemm, "gemm_mx": bench_gemm_mx, "rmsnorm": bench_rmsnorm,
            "depth_mix": bench_depth_mix, "swiglu": bench_swiglu, "lm_head": bench_lm_head, "adamw": bench_adamw,
-           "decode_attention": bench_decode_attention}[a.op](a)
+           "decode_attention": bench_decode_attention, "paged": bench_paged, "verify": bench_verify}[a.op](a)
     print(json.dumps(res))
 
 
