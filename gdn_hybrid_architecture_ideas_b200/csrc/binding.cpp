@@ -462,6 +462,7 @@ Rope rope_of(const c10::optional<Tensor>& cos, const c10::optional<Tensor>& sin,
   TORCH_CHECK(sin.has_value() && cos->dim() == 2 && cos->sizes() == sin->sizes() && is_f32(*cos) && is_f32(*sin) && cos->is_contiguous() && sin->is_contiguous() &&
               cos->device() == like.device() && sin->device() == like.device(), what, ": rope is (cos, sin), each contiguous float32 [positions, rotary pairs] on the cache's device");
   const int64_t half = cos->size(1);
+  TORCH_CHECK(cos->size(0) > 0, what, ": a rope table without positions");
   TORCH_CHECK(half > 0 && half % 8 == 0 && 2 * half <= hd, what, ": ", 2 * half, " rotary channels (a multiple of 16, at most the head dimension, on a GPU)");
   for (const Tensor* t : {&*cos, &*sin}) TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, what, ": rope tables start on a 16-byte boundary");
   return {cos->data_ptr<float>(), sin->data_ptr<float>(), static_cast<int>(half), static_cast<int>(std::min<int64_t>(cos->size(0), 0x7fffffff))};

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 3) paged_append_kernel(PagedRo
   Spot s;
   if (!spot_of(r, qs, j, s) || s.entry < 0) return;
   const bool turns = blk * 16 < 2 * half;
-  if (half > 0 && z0 < r.Hkv) {
+  if (half > 0) {                        // (for the values too: a token without a rotation is left out whole)
     const int p = s.t - s.start;
     if (p < 0 || p >= n_pos) { *r.err = p < 0 ? ST_START : ST_ROPE; return; }
     cos += static_cast<long>(p) * half;

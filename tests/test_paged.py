@@ -1040,3 +1040,29 @@ def test_two_caches_on_two_streams_at_once():
     for o, want in zip(outs, alone):
         assert all(torch.equal(x, want) for x in o)
     _status_clean()
+
+
+@pytest.mark.gpu
+def test_empty_tables_and_tokens_without_a_rotation():
+    """A rope table without positions is refused; a batch of no rows leaves zeros; a token behind the rope table is left out whole, its value as
+    well as its key, however its heads are spread over threads."""
+    from gdn_hybrid_architecture_ideas_b200.ops import native
+
+    rows, page = [(20, 1, 0)], 16
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page, device="cuda")
+    cache, _ = _random_cache(n_pages, page, 2, 64, "bf16")
+    q = torch.randn(n, 4, 64, device="cuda").bfloat16()
+    k = torch.randn(n, 2, 64, device="cuda").bfloat16()
+    none = tuple(torch.zeros(0, 8, device="cuda") for _ in range(2))
+    for call in (lambda: ops.paged_attention(q, cache, pages, q_start, lens, rope=none), lambda: ops.paged_append(cache, k, k, pages, q_start, lens, rope=none)):
+        with pytest.raises(RuntimeError, match="without positions"):
+            call()
+    before = cache.k.clone(), cache.v.clone()
+    no_rows = (pages[:0], q_start[:1], lens[:0])
+    assert not ops.paged_attention(q, cache, *no_rows).any() and not ops.paged_read(cache, *no_rows, n)[0].any()
+    ops.paged_append(cache, k, k, *no_rows)
+    _status_clean()
+    ops.paged_append(cache, k, k, pages, q_start, lens, rope=tuple(t.cuda() for t in _tables(20, 8)))          # position 20 needs 21 entries
+    with pytest.raises(RuntimeError, match="status 305"):
+        native.check_status()
+    assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1])
