@@ -915,24 +915,41 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
   }
 }
 
+// Zeros for the packed tokens that no row owns (those a row owns are written where its units are joined), by all blocks of a launch side
+// by side. With q_start in order they lie before q_start[0] and behind q_start[B]. Out of order (status 301), the rows whose own range is
+// right keep their tokens, so every token asks all rows.
+template <int HD>
+__device__ __forceinline__ void zero_unowned(const AttnK& p, int block, int blocks) {
+  const PagedRows& R = p.r;
+  const long per = static_cast<long>(p.a.Hq) * HD / 8, stride = static_cast<long>(blocks) * blockDim.x, at = static_cast<long>(block) * blockDim.x + threadIdx.x;
+  uint4* out = reinterpret_cast<uint4*>(p.a.out);
+  bool wrong = false;
+  for (int b = threadIdx.x; b <= R.B; b += blockDim.x) { const int q = R.q_start[b]; wrong |= q < 0 || q > R.n || (b < R.B && R.q_start[b + 1] < q); }
+  wrong = __syncthreads_or(wrong);
+  if (!wrong) {
+    const long lead = R.q_start[0] * per, gap = R.q_start[R.B] * per - lead, n = R.n * per - gap;
+    for (long x = at; x < n; x += stride) out[x < lead ? x : x + gap] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  for (long x = at; x < R.n * per; x += stride) {
+    const int j = static_cast<int>(x / per);
+    bool owned = false;
+    for (int b = 0; b < R.B && !owned; ++b) { const int q0 = R.q_start[b], q1 = R.q_start[b + 1]; owned = q0 >= 0 && q1 <= R.n && j >= q0 && j < q1; }
+    if (!owned) out[x] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // Joins the parts of every unit that CTA borders cut: part one is the last thing its first CTA did (slot 1), the others are the
 // first thing that the following CTAs did (slot 0). Block (i, r) joins query row r of the unit whose first part CTA i holds. Also the zeros of
-// the packed tokens behind the last row, where the output is this call's own.
+// the packed tokens that no row owns, where the output is this call's own.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_constant__ AttnK p, int n_ctas) {
   constexpr int LANES = HD / 4, GROUPS = 256 / LANES, UR = UNIT_ROWS;
   __shared__ float4 s_o[GROUPS][LANES];
   __shared__ float s_m[GROUPS], s_l[GROUPS];
   const int i = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  if (p.a.fill) zero_unowned<HD>(p, i * gridDim.y + r, gridDim.x * gridDim.y);        // (the first kernel writes none of these)
   asm volatile("griddepcontrol.wait;" ::: "memory");          // launched while the first kernel ends; from here on that is complete
-  if (p.a.fill) {
-    const int q_end = p.r.B ? p.r.q_start[p.r.B] : 0;
-    if (q_end >= 0) {
-      const long per = static_cast<long>(p.a.Hq) * HD / 8, n = (p.r.n - static_cast<long>(q_end)) * per;
-      uint4* o = reinterpret_cast<uint4*>(p.a.out) + q_end * per;
-      for (long x = (static_cast<long>(i) * gridDim.y + r) * blockDim.x + tid; x < n; x += static_cast<long>(gridDim.x) * gridDim.y * blockDim.x) o[x] = make_uint4(0, 0, 0, 0);
-    }
-  }
   const int* head = p.meta + i * 8;
   const int parts = head[0];
   if (parts == 0 || r >= head[3]) return;

@@ -20,8 +20,9 @@ Rows. Every op takes the same description of a batch: `pages` int32 [B, width], 
 position (entries past the row's last page are not read); `q_start` int32 [B + 1], row b's NEW tokens are the packed
 tokens q_start[b] .. q_start[b + 1]; `lens` int32 [B], the row's cached positions including those, so its packed token j sits
 at position lens[b] - (q_start[b + 1] - j); `start` int32 [B] (default 0), the row's first visible position, from which its
-rotary positions count. Packed tokens from q_start[B] on are padding: no op reads or writes for them, except that an op
-which allocates its own output leaves zeros there. Rows may have no tokens.
+rotary positions count. Packed tokens that no row owns (before q_start[0], from q_start[B] on, of a row whose range is refused) are
+padding: no op reads or writes for them, except that an op which allocates its own output leaves zeros there. Rows may have
+no tokens.
 """
 
 from __future__ import annotations
