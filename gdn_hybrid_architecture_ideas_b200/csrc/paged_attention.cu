@@ -77,12 +77,7 @@ struct Geo : Cfg<FP4, HD> {
   static constexpr int DATA = BESIDE ? RING + MERGE : RING > MERGE ? RING : MERGE;
   static constexpr int QCOPIES = FP4 ? 1 : 2;        // bfloat16: high and low part
   static constexpr int QB = UR * HD * 2;             // bytes of one copy of the queries
-  // under a cap: near and far queries, the near ones' rotary channels in float32 and as each warp rotated them, a tile of rotations
-  __host__ __device__ static constexpr int q_bytes(bool cap) { return (cap ? 2 : 1) * QCOPIES * QB; }
-  __host__ __device__ static constexpr int turned_bytes(int half) { return (half / 8) * 256 * QCOPIES; }      // of a warp
-  __host__ __device__ static constexpr int smem(int cap_half) {
-    return DATA + q_bytes(cap_half > 0) + UR * 2 * cap_half * 4 + TILE * cap_half * 8 + B::W * turned_bytes(cap_half);
-  }
+  static constexpr int smem(bool cap) { return DATA + (cap ? 2 : 1) * QCOPIES * QB; }      // under a cap: queries by the cap and by their positions
   static constexpr int THREADS = B::W * 32;
 };
 
@@ -240,9 +235,11 @@ __device__ __forceinline__ long block_scan(long x, long* s_warp, long* total) {
   return before + inc - x;      // exclusive
 }
 
-template <bool FP4, int HD, bool CAP>
+// STEPS: 0 without a cap, else half / 8: the groups of 8 rotary pairs of the keys that are rotated here (1, 2 or 4).
+template <bool FP4, int HD, int STEPS>
 __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) paged_attention_kernel(const __grid_constant__ AttnK p) {
   using GEO = Geo<FP4, HD>;
+  constexpr bool CAP = STEPS > 0;
   constexpr int H = GEO::H, MT = GEO::MT, TILE = GEO::TILE, UR = GEO::UR, W = GEO::W, ST = GEO::ST;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long s_warp[W];
@@ -250,7 +247,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
   __shared__ Row s_row;
   __shared__ float s_mul[UR];                 // a query row's factor on its scores: scale * log2(e) * its power of two
   __shared__ float s_m[W][UR], s_l[W][UR];
-  __shared__ int s_pos[UR];                   // a query row's position
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const PagedRows& R = p.r;
   const int n_ctas = gridDim.x, cta = blockIdx.x, Hkv = R.Hkv, G = p.G;
@@ -300,10 +296,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
   uint8_t* ring = smem + warp * (ST * GEO::STAGE);
   const uint32_t ring_u = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   uint8_t* sq = smem + GEO::DATA;
-  const int half = p.a.half;
-  float* sq_base = reinterpret_cast<float*>(sq + GEO::q_bytes(CAP));                       // [UR][2 half]
-  float4* s_turn = reinterpret_cast<float4*>(sq_base + UR * 2 * half);                     // [TILE][half / 2]: cos, cos, sin, sin of two pairs
-  uint8_t* s_turned = reinterpret_cast<uint8_t*>(s_turn + TILE * (half >> 1)) + warp * GEO::turned_bytes(half);
+  const int half = CAP ? 8 * STEPS : p.a.half;
   // ---- the part of a unit that this CTA does next
   struct Part { int b, q0, start, h, r0, n_rows, p0, n_pieces, pieces, pos0, p_first, p_last, tile0; long last_cost; };
   long at = lo;
@@ -426,12 +419,13 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
     int stage = 0;                             // of tile k
 
     // ---- the unit's queries, a warp a row: all loads first (they and the first tiles are under way together), then rotated (by their
-    // positions; under a cap by the cap, the near rotation follows tile by tile), brought to about one, in the products' order
+    // positions; under a cap one copy by the cap and one by the positions), brought to about one, in the products' order
     // (a lane takes HD / 32 neighbouring channels: 2, 4 or 8, which divides half, so that their partners are neighbours too)
     constexpr int RPW = (UR + W - 1) / W, CPL = HD / 32;
     const int c0 = lane * CPL;
     const bool turns = c0 < 2 * half, low = c0 < half;
-    float x[RPW][CPL], y[RPW][CPL], co[RPW][CPL], si[RPW][CPL];
+    constexpr int TURNS = CAP ? 2 : 1;         // the copies' rotations: of the plain products, of the rotating ones
+    float x[RPW][CPL], y[RPW][CPL], co[TURNS][RPW][CPL], si[TURNS][RPW][CPL];
 #pragma unroll
     for (int j = 0; j < RPW; ++j) {
       const int r = warp + j * W, rr = r0 + r;
@@ -441,7 +435,6 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
       const long off = (static_cast<long>(q0) + i) * p.a.q_ts + head * p.a.q_hs;
       int at_pos = pos0 + i - start;
       if (live && half > 0 && at_pos >= p.a.n_pos) { *R.err = ST_ROPE; at_pos = p.a.n_pos - 1; }
-      if (lane == 0 && r < UR) s_pos[r] = live ? pos0 + i : -1;
       const int partner = turns ? (low ? c0 + half : c0 - half) : c0;
       if (p.a.q_f32) {
         load_channels<CPL>(static_cast<const float*>(p.a.q) + off + c0, x[j]);
@@ -451,19 +444,15 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
         load_channels<CPL>(static_cast<const __nv_bfloat16*>(p.a.q) + off + partner, y[j]);
       }
       if (half > 0) {
-        const long e = static_cast<long>(CAP ? p.a.cap : max(0, min(at_pos, p.a.n_pos - 1))) * half + (turns ? (low ? c0 : c0 - half) : 0);
-        load_channels<CPL>(p.a.cos + e, co[j]);
-        load_channels<CPL>(p.a.sin + e, si[j]);
+#pragma unroll
+        for (int w = 0; w < TURNS; ++w) {
+          const long e = static_cast<long>(CAP && w == 0 ? p.a.cap : max(0, min(at_pos, p.a.n_pos - 1))) * half + (turns ? (low ? c0 : c0 - half) : 0);
+          load_channels<CPL>(p.a.cos + e, co[w][j]);
+          load_channels<CPL>(p.a.sin + e, si[w][j]);
+        }
       }
     }
     if (!begun) begin();
-    if (CAP && !begun) {
-      for (int i = tid; i < TILE * (half >> 1); i += GEO::THREADS) {
-        const int d = min(i / (half >> 1), p.a.n_pos - 1), j = i % (half >> 1);
-        const float2 c = *reinterpret_cast<const float2*>(p.a.cos + static_cast<long>(d) * half + 2 * j), sn = *reinterpret_cast<const float2*>(p.a.sin + static_cast<long>(d) * half + 2 * j);
-        s_turn[i] = make_float4(c.x, c.y, sn.x, sn.y);
-      }
-    }
     begun = true;
 #pragma unroll
     for (int j = 0; j < RPW; ++j) {
@@ -482,12 +471,11 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
       ex = max(-120, min(120, ex));
       const float down = exp2f(static_cast<float>(-ex));
       if (lane == 0) s_mul[r] = p.a.scale * 1.44269504088896340736f * exp2f(static_cast<float>(ex));
-      float turned[CPL];
+      float turned[TURNS][CPL];
 #pragma unroll
-      for (int i = 0; i < CPL; ++i) {
-        turned[i] = (turns ? x[j][i] * co[j][i] + y[j][i] * (low ? -si[j][i] : si[j][i]) : x[j][i]) * down;
-        x[j][i] *= down;
-      }
+      for (int i = 0; i < CPL; ++i)
+#pragma unroll
+        for (int w = 0; w < TURNS; ++w) turned[w][i] = (turns ? x[j][i] * co[w][j][i] + y[j][i] * (low ? -si[w][j][i] : si[w][j][i]) : x[j][i]) * down;
       // Two channels at a time to their places: in the order of the plain products (a lane owns the 16 channels 16 t .. of each slice),
       // and of the rotating ones (its channels are 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16).
       auto put = [&](uint8_t* to, int idx, float a, float z) {
@@ -501,11 +489,8 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
 #pragma unroll
       for (int i = 0; i < CPL; i += 2) {
         const int c = c0 + i, cc = c & 63;
-        put(sq, ((((c >> 6) * 4 + ((cc & 15) >> 2)) * 32 + r * 4 + (cc >> 4)) << 2) + (cc & 3), turned[i], turned[i + 1]);
-        if constexpr (CAP) {
-          put(sq + GEO::QCOPIES * GEO::QB, (((c >> 4) * 32 + r * 4 + ((c & 7) >> 1)) << 2) + ((c >> 2) & 2), x[j][i], x[j][i + 1]);      // (its rotary channels are not read)
-          if (turns) *reinterpret_cast<float2*>(sq_base + r * 2 * half + c) = make_float2(x[j][i], x[j][i + 1]);
-        }
+        put(sq, ((((c >> 6) * 4 + ((cc & 15) >> 2)) * 32 + r * 4 + (cc >> 4)) << 2) + (cc & 3), turned[0][i], turned[0][i + 1]);
+        if constexpr (CAP) put(sq + GEO::QCOPIES * GEO::QB, (((c >> 4) * 32 + r * 4 + ((c & 7) >> 1)) << 2) + ((c >> 2) & 2), turned[1][i], turned[1][i + 1]);
       }
     }
     __syncthreads();
@@ -633,39 +618,32 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
         }
         if constexpr (CAP) {
           if (near_any) {
-            // ---- keys within the cap. R(p) q . R(t) k = R(p - t0) q . R(t - t0) k with t0 the tile's first position: the keys take
-            // one of TILE rotations that stay in shared memory, the queries' rotary channels are rotated once a tile. A lane owns channels
-            // 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16, so that both channels of a rotary pair (half 8, 16 or 32
-            // apart) are its own.
-            const int t0 = max(first, start);
-            const int steps = half >> 3, slot_low = steps * 256;          // rotary k16 steps; bytes of the high parts
-            {
-              const long d = max(0, min(s_pos[g] - t0, p.a.n_pos - 1));
-              const float* co = p.a.cos + d * half + 2 * t;
-              const float* si = p.a.sin + d * half + 2 * t;
-              const float* qb = sq_base + g * 2 * half + 2 * t;
+            // ---- keys within the cap, R(p) q . R(t) k: the keys are rotated here by the table's rows of their positions (any rows: nothing
+            // is assumed of how they follow one another). A lane owns channels 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of every block of 16, so
+            // that both channels of a rotary pair (half 8, 16 or 32 apart) are its own. A key's row is read by the four lanes that hold its
+            // channels, 32 bytes at a time, for the next 16 positions while these are scored.
+            float2 co[2][STEPS], si[2][STEPS], co_next[2][STEPS], si_next[2][STEPS];
+            auto load_rows = [&](int mt) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if (i >= steps) break;
-                const float2 c = *reinterpret_cast<const float2*>(co + 8 * i), sn = *reinterpret_cast<const float2*>(si + 8 * i);
-                const float2 u = *reinterpret_cast<const float2*>(qb + 8 * i), v = *reinterpret_cast<const float2*>(qb + half + 8 * i);
-                const float2 a = make_float2(u.x * c.x - v.x * sn.x, u.y * c.y - v.y * sn.y), z = make_float2(v.x * c.x + u.x * sn.x, v.y * c.y + u.y * sn.y);
-                auto put = [&](int eight, float2 x) {         // group of 8 channels -> (step, register) of this lane
-                  uint8_t* to = s_turned + (eight >> 1) * 256 + lane * 8 + (eight & 1) * 4;
-                  const uint32_t hi = pack<FP4>(x.x, x.y);
-                  *reinterpret_cast<uint32_t*>(to) = hi;
-                  if constexpr (!FP4) {
-                    const float2 f = unpack<FP4>(hi);
-                    *reinterpret_cast<uint32_t*>(to + slot_low) = pack<FP4>(isfinite(x.x) ? x.x - f.x : 0.f, isfinite(x.y) ? x.y - f.y : 0.f);
-                  }
-                };
-                put(i, a);
-                put(steps + i, z);
+              for (int e = 0; e < 2; ++e) {
+                const int d = max(0, min(first + mt * 16 + e * 8 + place<FP4>(g) - start, p.a.n_pos - 1));
+                const long at = static_cast<long>(d) * half + 2 * t;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                  co_next[e][i] = __ldg(reinterpret_cast<const float2*>(p.a.cos + at + 8 * i));
+                  si_next[e][i] = __ldg(reinterpret_cast<const float2*>(p.a.sin + at + 8 * i));
+                }
               }
-            }
+            };
+            load_rows(0);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               float acc[CHAINS][4];
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) { co[e][i] = co_next[e][i]; si[e][i] = si_next[e][i]; }
+              if (mt + 1 < MT) load_rows(mt + 1);
 #pragma unroll
               for (int hs = 0; hs < H; ++hs) {
                 uint32_t x[2][4][2];           // [row][block of the slice][channels 2 t.. or 2 t + 8 ..]
@@ -693,24 +671,20 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
                         x[e][bl][c] = *reinterpret_cast<const uint32_t*>(st + hs * (TILE * 128) + pos * 128 + (((2 * bl + c) ^ (pos & 7)) << 4) + t * 4);
                   }
                   if (hs == 0) {
-                    const float4* tr = s_turn + max(0, first + pos - t0) * (half >> 1) + t;
-                    auto turn = [&](uint32_t& a, uint32_t& bb, int i) {          // pair channels i + 2 t .. of the first half
-                      const float4 cs = tr[i >> 1];
-                      const float2 u = unpack<FP4>(a), v = unpack<FP4>(bb);
-                      a = pack<FP4>(u.x * cs.x - v.x * cs.z, u.y * cs.y - v.y * cs.w);
-                      bb = pack<FP4>(v.x * cs.x + u.x * cs.z, v.y * cs.y + u.y * cs.w);
-                    };
-                    if (half == 8) turn(x[e][0][0], x[e][0][1], 0);
-                    else if (half == 16) { turn(x[e][0][0], x[e][1][0], 0); turn(x[e][0][1], x[e][1][1], 8); }
-                    else { turn(x[e][0][0], x[e][2][0], 0); turn(x[e][0][1], x[e][2][1], 8); turn(x[e][1][0], x[e][3][0], 16); turn(x[e][1][1], x[e][3][1], 24); }
+                    // group i of 8 pairs: channels 8 i + 2 t .. with those `half` further
+#pragma unroll
+                    for (int i = 0; i < STEPS; ++i) {
+                      uint32_t &a = x[e][i >> 1][i & 1], &bb = x[e][(i + STEPS) >> 1][(i + STEPS) & 1];
+                      const float2 u = unpack<FP4>(a), v = unpack<FP4>(bb), c = co[e][i], n = si[e][i];
+                      a = pack<FP4>(u.x * c.x - v.x * n.x, u.y * c.y - v.y * n.y);
+                      bb = pack<FP4>(v.x * c.x + u.x * n.x, v.y * c.y + u.y * n.y);
+                    }
                   }
                 }
 #pragma unroll
                 for (int bl = 0; bl < 4; ++bl) {
                   const uint32_t a[4] = {x[0][bl][0], x[1][bl][0], x[0][bl][1], x[1][bl][1]};
-                  const int ks = hs * 4 + bl;
-                  const bool own = hs == 0 && bl < steps;
-                  step(acc, a, own ? s_turned + ks * 256 : sq + GEO::QCOPIES * GEO::QB + ks * 256, own ? slot_low : GEO::QB, hs, hs < 2 && bl == 0);
+                  step(acc, a, sq + GEO::QCOPIES * GEO::QB + (hs * 4 + bl) * 256, GEO::QB, hs, hs < 2 && bl == 0);
                 }
               }
 #pragma unroll
@@ -993,19 +967,18 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_
 
 namespace {
 
-template <bool FP4, int HD, bool CAP>
+template <bool FP4, int HD, int STEPS>
 int launch(const AttnK& k, int ctas, cudaStream_t st) {
   using GEO = Geo<FP4, HD>;
-  const int bytes = GEO::smem(CAP ? k.a.half : 0);
-  // (the largest size this kernel can ask for, set once per device)
-  static std::atomic<uint64_t> ready[4];
+  constexpr int bytes = GEO::smem(STEPS > 0);
+  static std::atomic<uint64_t> ready[4];         // devices on which the size is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 4;
   if (dev > 255 || !(ready[dev >> 6].load(std::memory_order_acquire) >> (dev & 63) & 1)) {
-    if (cudaFuncSetAttribute(paged_attention_kernel<FP4, HD, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEO::smem(CAP ? 32 : 0)) != cudaSuccess) return 4;
+    if (cudaFuncSetAttribute(paged_attention_kernel<FP4, HD, STEPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return 4;
     if (dev <= 255) ready[dev >> 6].fetch_or(uint64_t(1) << (dev & 63), std::memory_order_release);
   }
-  paged_attention_kernel<FP4, HD, CAP><<<ctas, GEO::THREADS, bytes, st>>>(k);
+  paged_attention_kernel<FP4, HD, STEPS><<<ctas, GEO::THREADS, bytes, st>>>(k);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, GEO::UR);
   cfg.blockDim = dim3(256);
@@ -1019,7 +992,10 @@ int launch(const AttnK& k, int ctas, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 template <bool FP4, int HD>
-int launch(const AttnK& k, int ctas, cudaStream_t st) { return k.a.cap ? launch<FP4, HD, true>(k, ctas, st) : launch<FP4, HD, false>(k, ctas, st); }
+int launch(const AttnK& k, int ctas, cudaStream_t st) {
+  if (!k.a.cap) return launch<FP4, HD, 0>(k, ctas, st);
+  return k.a.half == 8 ? launch<FP4, HD, 1>(k, ctas, st) : k.a.half == 16 ? launch<FP4, HD, 2>(k, ctas, st) : launch<FP4, HD, 4>(k, ctas, st);
+}
 
 template <bool FP4>
 int dispatch(const AttnK& k, int hd, int ctas, cudaStream_t st) {

@@ -69,3 +69,52 @@ def test_tokens_of_refused_rows_are_zeros(q_start, owned):
     rest = [j for j in range(n) if j not in owned]
     assert torch.equal(got[owned], out[owned]) and not got[rest].any() and bool((out[rest] == 3).all())
     assert all(bool(got[j].any()) for j in owned)
+
+
+# ------------------------------------------------------------------------------------------------------------ rope tables
+
+def _any_rows(n, pairs, seed=0):
+    """A rope table whose rows are rotations by any angles: nothing relates one to another."""
+    ang = torch.rand(n, pairs, generator=torch.Generator().manual_seed(seed), dtype=torch.float64) * 2 * math.pi
+    return ang.cos().float(), ang.sin().float()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "fp4"])
+@pytest.mark.parametrize("hd,group,rot,cap,page,qdt", [(64, 4, 16, 20, 16, "bf16"), (64, 8, 64, 33, 8, "bf16"), (64, 3, 32, 1, 64, "fp32"), (128, 5, 32, 40, 64, "bf16"),
+                                                       (128, 2, 64, 300, 16, "fp32"), (256, 8, 64, 100, 16, "bf16"), (256, 1, 16, 7, 32, "bf16")])
+def test_capped_scores_take_the_tables_rows_as_they_are(fmt, hd, group, rot, cap, page, qdt):
+    """R(p)q . R(t)k with the table's rows at p and t, R(C)q . k beyond the cap, whatever the rows are."""
+    rows = [(0, 1, 0), (37, 5, 9), (0, 0, 0), (250, 1, 0), (15, 4, 17), (0, 21, 0), (300, 2, 290)]
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page, seed=group)
+    cache, cpu = _random_cache(n_pages, page, 2, hd, fmt, seed=rot)
+    q = (torch.randn(n, 2 * group, hd) * 1.5).to({"bf16": torch.bfloat16, "fp32": torch.float32}[qdt])
+    _check_attention(q, cache, cpu, rows, pages, q_start, lens, start, _any_rows(310, rot // 2), cap, page=page)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,hd,new", [("fp4", 64, 2), ("fp4", 128, 1), ("bf16", 64, 1), ("bf16", 256, 3)])
+def test_capped_scores_over_many_ctas(fmt, hd, new):
+    """The same where rows are cut over many CTAs."""
+    rows, page = [(5000, new, 0), (3, new, 0), (2777, new, 1201)], 64
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    cache, cpu = _random_cache(n_pages, page, 1, hd, fmt)
+    q = torch.randn(n, 2, hd).bfloat16()
+    _check_attention(q, cache, cpu, rows, pages, q_start, lens, start, _any_rows(5100, 16), 700, page=page)
+
+
+@pytest.mark.parametrize("cap", [None, 7])
+def test_capped_statement_takes_the_tables_rows_as_they_are_cpu(cap):
+    rows, page, hd = [(37, 5, 9), (0, 1, 0)], 8, 32
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    cache = pg.PagedKV(*(torch.randn(n_pages, 1, page, hd, dtype=torch.float64) for _ in range(2)))
+    cos, sin = (t.double() for t in _any_rows(50, 8))
+    q = torch.randn(n, 2, hd, dtype=torch.float64)
+    got = ops.paged_attention(q, cache, pages, q_start, lens, start=start, rope=(cos, sin), cap=cap)
+    for b, (a, m, c) in enumerate(rows):
+        for i in range(m):
+            j = int(q_start[b]) + i
+            ids, slots = zip(*[(int(pages[b, p // page]), p % page) for p in range(c, a + i + 1)])
+            for h in range(2):
+                want = _dense_attention(q[j, h].numpy(), cache.k.numpy()[ids, 0, slots], cache.v.numpy()[ids, 0, slots], a + i, c, cos.numpy(), sin.numpy(), cap, hd ** -0.5)[0]
+                assert np.abs(got[j, h].numpy() - want).max() < 1e-12
