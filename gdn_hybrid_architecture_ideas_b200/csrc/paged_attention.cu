@@ -867,6 +867,9 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
         ll += s_l[w][r] * f;
         oo.x += z.x * f; oo.y += z.y * f; oo.z += z.z * f; oo.w += z.w * f;
       }
+      if (half > 0 && pos0 + (r0 + r) / G - start >= p.a.n_pos) {        // a query behind the rope table (reported above): left out, zeros
+        mm = -INFINITY; ll = 0.f; oo = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
       if (begins && ends) {
         const int rr = r0 + r;
         const float inv = ll == 0.f ? 0.f : 1.f / ll;          // a row without a score above -inf has no weights: zeros

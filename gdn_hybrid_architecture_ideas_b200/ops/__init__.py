@@ -279,8 +279,9 @@ def paged_attention(q, cache, pages, q_start, lens, start=None, rope=None, cap=N
     first): token at position p sees start .. p; Hq is a multiple of the cache's heads. q is unrotated. rope without cap: q is
     rotated at its position, the cached keys are taken as `paged_append` rotated them. rope with cap C (the rotary distance
     cap): the cache holds unrotated keys, a key at distance d <= C is scored R(p)q . R(t)k, beyond it R(C)q . k. R(i) is the
-    table's row i (positions count from start); its angles may be any. No rope: position-free. A token that sees nothing gets zeros. scale: default hd ** -0.5. Forward only; on CUDA q is bfloat16 or
-    float32, the output bfloat16, under a cap 16, 32 or 64 rotary channels."""
+    table's row i (positions count from start); its angles may be any. No rope: position-free. A token that sees nothing gets zeros, on
+    CUDA also one behind the rope table (with a status, as for every wrong table value). scale: default hd ** -0.5. Forward
+    only; on CUDA q is bfloat16 or float32, the output bfloat16, under a cap 16, 32 or 64 rotary channels."""
     if cache._k.is_cuda and _MODE == "native":
         return _native().paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out)
     return paged.paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out)

@@ -118,3 +118,26 @@ def test_capped_statement_takes_the_tables_rows_as_they_are_cpu(cap):
             for h in range(2):
                 want = _dense_attention(q[j, h].numpy(), cache.k.numpy()[ids, 0, slots], cache.v.numpy()[ids, 0, slots], a + i, c, cos.numpy(), sin.numpy(), cap, hd ** -0.5)[0]
                 assert np.abs(got[j, h].numpy() - want).max() < 1e-12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,hd", [("fp4", 64), ("bf16", 64), ("bf16", 128), ("fp4", 256)])
+@pytest.mark.parametrize("cap", [None, 10])
+@pytest.mark.parametrize("before", [20, 5000])
+def test_queries_behind_the_rope_table_are_zeros(fmt, hd, cap, before):
+    """Three new tokens of which the last two lie behind the table, a row behind it whole, one inside: status 305; zeros for those, the others
+    as with a table that is long enough (rows of 5000 positions are cut over CTAs)."""
+    from gdn_hybrid_architecture_ideas_b200.ops import native
+
+    rows, page = [(before, 3, 0), (before + 30, 1, 0), (9, 1, 0), (before + 30, 1, 40)], 64
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    cache, _ = _random_cache(n_pages, page, 2, hd, fmt)
+    q = torch.randn(n, 8, hd, device="cuda").bfloat16()
+    args = [t.cuda() for t in (pages, q_start, lens)]
+    rope = tuple(t.cuda() for t in _tables(before + 40, 16))
+    whole = ops.paged_attention(q, cache, *args, start=start.cuda(), rope=rope, cap=cap)
+    _status_clean()
+    got = ops.paged_attention(q, cache, *args, start=start.cuda(), rope=tuple(t[:before + 1].contiguous() for t in rope), cap=cap)
+    with pytest.raises(RuntimeError, match="status 305"):
+        native.check_status()
+    assert not got[[1, 2, 3]].any() and torch.equal(got[[0, 4, 5]], whole[[0, 4, 5]])
