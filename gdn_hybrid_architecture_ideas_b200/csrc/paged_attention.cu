@@ -13,7 +13,7 @@
 // 4 bits: a lane's 16 channels of a key are one block with one scale. Codes become f16 pairs (cvt.f16x2.e2m1x2), times the
 // scale: exact in f16 (2 + 4 significant bits, 2^-10 .. 2688). Queries are rounded to f16 once (2^-12 relative), after a
 // power of two per query row has brought them to about one, probabilities to f16 (2^-12, scaled up: PSHIFT below). bfloat16 cache:
-// queries as the sum of two bfloat16 (2^-17), keys as they are, probabilities to bfloat16 (2^-9). The sum of the probabilities is
+// queries and probabilities as the sum of two bfloat16 (2^-16), keys as they are. The sum of the probabilities is
 // taken over the rounded ones. All sums are float32 in the accumulators.
 //
 // Work: the pieces (one tile of positions for each warp) of all (row, KV head, block of query rows) units form one sequence,
@@ -733,13 +733,17 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
           }
         }
         // ---- probabilities
-        uint32_t pk[MT][2];
+        constexpr int PARTS = FP4 ? 1 : 2;         // bfloat16: what the rounding leaves as a second part (2^-16 together)
+        uint32_t pk[PARTS][MT][2];
         const float ref0 = (m[0] == -INFINITY ? 0.f : -m[0]) + (FP4 ? PSHIFT : 0.f), ref1 = (m[1] == -INFINITY ? 0.f : -m[1]) + (FP4 ? PSHIFT : 0.f);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
-            pk[mt][q] = pack<FP4>(exp2_fast(fmaf(s[mt][2 * q], mul[0], ref0)), exp2_fast(fmaf(s[mt][2 * q + 1], mul[1], ref1)));
+          for (int q = 0; q < 2; ++q) {
+            const float a = exp2_fast(fmaf(s[mt][2 * q], mul[0], ref0)), z = exp2_fast(fmaf(s[mt][2 * q + 1], mul[1], ref1));
+            pk[0][mt][q] = pack<FP4>(a, z);
+            if constexpr (PARTS > 1) { const float2 f = unpack<FP4>(pk[0][mt][q]); pk[1][mt][q] = pack<FP4>(a - f.x, z - f.y); }
+          }
         // ---- O^T += V^T P^T
         bool plain = true;
         if constexpr (!FP4) {
@@ -759,7 +763,9 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
           if (!plain) {
             for (int j = 0; j < TILE; ++j) {
               if (!((on >> (j >> c_shift)) & 1) || first + j < start) continue;
-              const float2 pp = unpack<FP4>(__shfl_sync(0xffffffffu, j < 8 ? pk[0][0] : pk[0][1], (j & 7) * 4 + t));
+              const float2 p1 = unpack<FP4>(__shfl_sync(0xffffffffu, j < 8 ? pk[0][0][0] : pk[0][0][1], (j & 7) * 4 + t));
+              const float2 p2 = unpack<FP4>(__shfl_sync(0xffffffffu, j < 8 ? pk[1][0][0] : pk[1][0][1], (j & 7) * 4 + t));
+              const float2 pp = make_float2(p1.x + p2.x, p1.y + p2.y);
               const bool see0 = first + j <= prow[0], see1 = first + j <= prow[1];
               if (see0) { l[0] += pp.x; l[2] += pp.x; }
               if (see1) { l[1] += pp.y; l[3] += pp.y; }
@@ -781,15 +787,19 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
         if (plain) {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            const uint32_t pb[2] = {transpose8(pk[mt][0]), transpose8(pk[mt][1])};
+            uint32_t pb[PARTS][2];
+#pragma unroll
+            for (int w = 0; w < PARTS; ++w) { pb[w][0] = transpose8(pk[w][mt][0]); pb[w][1] = transpose8(pk[w][mt][1]); }
             constexpr uint32_t ONE2 = FP4 ? 0x3c003c00u : 0x3f803f80u;
             const uint32_t ones[4] = {ONE2, ONE2, ONE2, ONE2};
-            mma<FP4>(l, ones, pb[0], pb[1]);
+#pragma unroll
+            for (int w = 0; w < PARTS; ++w) mma<FP4>(l, ones, pb[w][0], pb[w][1]);
             const int u0 = mt * 16 + place<FP4>(2 * t), u1 = mt * 16 + place<FP4>(2 * t + 1);
 #pragma unroll
             for (int hs = 0; hs < H; ++hs) {
               uint32_t a4[4][4];                   // [channel 8 g + 2 i of the slice][operand register]
               uint32_t sc[2];
+              bool second = PARTS > 1;
               if constexpr (FP4) {
                 // the codes of positions u0, u1 side by side in a byte, even channels and odd ones: one conversion gives the pair
                 const uint8_t* vb = st + GEO::KB + hs * 32 + g * 4;
@@ -816,6 +826,13 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
                   const uint4 w = *reinterpret_cast<const uint4*>(vb + us[c] * 128 + ((g ^ (us[c] & 7)) << 4));
                   v[c][0] = w.x; v[c][1] = w.y; v[c][2] = w.z; v[c][3] = w.w;
                 }
+                // An infinite value stays infinite: a weight's second part may be zero or negative, and is left out beside one.
+                __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f), odd = zero;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) odd = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v[c][i]), zero, odd);      // NaN from there on
+                second = !__any_sync(0xffffffffu, (*reinterpret_cast<const uint32_t*>(&odd) & 0x7fff7fffu) != 0u);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   a4[i][0] = prmt(v[0][i], v[1][i], 0x5410); a4[i][1] = prmt(v[0][i], v[1][i], 0x7632);
@@ -823,7 +840,11 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
                 }
               }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) mma<FP4>(o[hs * 4 + i], a4[i], pb[0], pb[1]);
+              for (int i = 0; i < 4; ++i) mma<FP4>(o[hs * 4 + i], a4[i], pb[0][0], pb[0][1]);
+              if (second) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma<FP4>(o[hs * 4 + i], a4[i], pb[PARTS - 1][0], pb[PARTS - 1][1]);
+              }
             }
           }
         }

@@ -141,3 +141,61 @@ def test_queries_behind_the_rope_table_are_zeros(fmt, hd, cap, before):
     with pytest.raises(RuntimeError, match="status 305"):
         native.check_status()
     assert not got[[1, 2, 3]].any() and torch.equal(got[[0, 4, 5]], whole[[0, 4, 5]])
+
+
+# ------------------------------------------------------------------------------------------------------------ what is kept of weights and keys
+
+def _bound(o, mass, big, cap):
+    """bfloat16 pages: probabilities in two parts 2^-16, queries and rotated keys in two parts 2^-16 each (sqrt 2 for a rotated pair),
+    float32 sums and exp2 2^-18; the output's own rounding 2^-8."""
+    d = 2.0 ** -16 + big * (2.0 ** -16 * 1.42 * (1 if cap is None else 2) + 2.0 ** -18) + 2.0 ** -18
+    return 2.0 ** -8 * np.abs(o) + (math.exp(2 * d) - 1) * 2 * mass * (1 + 2.0 ** -8) + 1e-30
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("odd", [False, True])
+def test_bfloat16_pages_keep_the_weights_in_two_parts(hd, odd):
+    """Values that cancel in the weighted sum: an error of the weights stands out there. odd: a later token of the row holds NaN, so that its
+    tile is summed position by position."""
+    for before in (1, 9, 23, 200):
+        rows, page = [(before, 2 if odd else 1, 0)], 16
+        pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+        _, cpu = _random_cache(n_pages, page, 2, hd, "bf16", seed=before)
+        q = torch.randn(n, 2, hd).bfloat16()
+        at = [(int(pages[0, p // page]), p % page) for p in range(before + 1)]
+        ids, slots = np.array([x for x, _ in at]), np.array([y for _, y in at])
+        for h in range(2):           # the likeliest position's value makes the sum (nearly) zero
+            k, v = cpu.k.double().numpy()[ids, h, slots], cpu.v.double().numpy()[ids, h, slots]
+            s = hd ** -0.5 * k @ q[0, h].double().numpy()
+            w = np.exp(s - s.max())
+            top = int(w.argmax())
+            cpu.v[ids[top], h, slots[top]] = torch.from_numpy(-(w @ v - w[top] * v[top]) / w[top]).bfloat16()
+        cache = pg.PagedKV(cpu.k.cuda(), cpu.v.cuda())
+        if odd:
+            cache.v[int(pages[0, (before + 1) // page]), :, (before + 1) % page] = float("nan")
+        got = ops.paged_attention(q.cuda(), cache, *(t.cuda() for t in (pages, q_start, lens)))
+        _status_clean()
+        for h in range(2):
+            k, v = cpu.k.double().numpy()[ids, h, slots], cpu.v.double().numpy()[ids, h, slots]
+            o, mass, big = _dense_attention(q[0, h].double().numpy(), k, v, before, 0, None, None, None, hd ** -0.5)
+            diff = np.abs(got[0, h].double().cpu().numpy() - o)
+            assert (diff <= _bound(o, mass, big, None)).all(), (before, h, diff.max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 256])
+def test_an_infinite_value_gives_an_infinite_output(hd):
+    """bfloat16 pages, a value of plus or minus infinity in a place that every query sees: that channel is infinite, the others of the slice are finite."""
+    rows, page = [(40, 1, 0), (100, 1, 0)], 16
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    cache, cpu = _random_cache(n_pages, page, 2, hd, "bf16")
+    for c in (cache, cpu):
+        c.v[int(pages[0, 0]), 0, 5, 3], c.v[int(pages[1, 2]), 1, 5, 40] = float("inf"), float("-inf")
+    q = torch.randn(n, 4, hd).bfloat16() * 0.2
+    got = ops.paged_attention(q.cuda(), cache, *(t.cuda() for t in (pages, q_start, lens))).cpu()
+    want = ops.paged_attention(q, cpu, pages, q_start, lens)
+    _status_clean()
+    assert int(want.isinf().sum()) == 4 and not want.isnan().any()
+    odd = want.isinf()
+    assert torch.equal(got[odd], want[odd]) and bool(torch.isfinite(got[~odd]).all())
