@@ -13,7 +13,7 @@
 // 4 bits: a lane's 16 channels of a key are one block with one scale. Codes become f16 pairs (cvt.f16x2.e2m1x2), times the
 // scale: exact in f16 (2 + 4 significant bits, 2^-10 .. 2688). Queries are rounded to f16 once (2^-12 relative), after a
 // power of two per query row has brought them to about one, probabilities to f16 (2^-12, scaled up: PSHIFT below). bfloat16 cache:
-// queries and probabilities as the sum of two bfloat16 (2^-16), keys as they are. The sum of the probabilities is
+// queries, probabilities and the keys that are rotated here as the sum of two bfloat16 (2^-16), other keys as they are. The sum of the probabilities is
 // taken over the rounded ones. All sums are float32 in the accumulators.
 //
 // Work: the pieces (one tile of positions for each warp) of all (row, KV head, block of query rows) units form one sequence,
@@ -152,6 +152,11 @@ template <bool FP4>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   if constexpr (FP4) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
   else { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+}
+// what rounding a pair to bfloat16 left, as bfloat16 (an infinity has no remainder)
+__device__ __forceinline__ uint32_t rest(float2 x, uint32_t rounded) {
+  const float2 f = unpack<false>(rounded);
+  return pack<false>(isfinite(x.x) ? x.x - f.x : 0.f, isfinite(x.y) ? x.y - f.y : 0.f);
 }
 // a byte's low half of a, its high half of b
 __device__ __forceinline__ uint32_t low_nibbles(uint32_t a, uint32_t b) {
@@ -481,10 +486,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
       auto put = [&](uint8_t* to, int idx, float a, float z) {
         const uint32_t hi = pack<FP4>(a, z);
         *reinterpret_cast<uint32_t*>(to + idx * 2) = hi;
-        if constexpr (!FP4) {
-          const float2 f = unpack<FP4>(hi);       // (an infinity has no remainder)
-          *reinterpret_cast<uint32_t*>(to + GEO::QB + idx * 2) = pack<FP4>(isfinite(a) ? a - f.x : 0.f, isfinite(z) ? z - f.y : 0.f);
-        }
+        if constexpr (!FP4) *reinterpret_cast<uint32_t*>(to + GEO::QB + idx * 2) = rest(make_float2(a, z), hi);
       };
 #pragma unroll
       for (int i = 0; i < CPL; i += 2) {
@@ -647,6 +649,7 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
 #pragma unroll
               for (int hs = 0; hs < H; ++hs) {
                 uint32_t x[2][4][2];           // [row][block of the slice][channels 2 t.. or 2 t + 8 ..]
+                uint32_t low[2][4][2];         // bfloat16: what rounding the rotated channels left (the blocks below STEPS)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const int pos = mt * 16 + e * 8 + place<FP4>(g);
@@ -676,15 +679,25 @@ __global__ void __launch_bounds__(Geo<FP4, HD>::THREADS, Geo<FP4, HD>::CTAS) pag
                     for (int i = 0; i < STEPS; ++i) {
                       uint32_t &a = x[e][i >> 1][i & 1], &bb = x[e][(i + STEPS) >> 1][(i + STEPS) & 1];
                       const float2 u = unpack<FP4>(a), v = unpack<FP4>(bb), c = co[e][i], n = si[e][i];
-                      a = pack<FP4>(u.x * c.x - v.x * n.x, u.y * c.y - v.y * n.y);
-                      bb = pack<FP4>(v.x * c.x + u.x * n.x, v.y * c.y + u.y * n.y);
+                      const float2 ra = make_float2(u.x * c.x - v.x * n.x, u.y * c.y - v.y * n.y), rb = make_float2(v.x * c.x + u.x * n.x, v.y * c.y + u.y * n.y);
+                      a = pack<FP4>(ra.x, ra.y);
+                      bb = pack<FP4>(rb.x, rb.y);
+                      if constexpr (!FP4) { low[e][i >> 1][i & 1] = rest(ra, a); low[e][(i + STEPS) >> 1][(i + STEPS) & 1] = rest(rb, bb); }
                     }
                   }
                 }
 #pragma unroll
                 for (int bl = 0; bl < 4; ++bl) {
                   const uint32_t a[4] = {x[0][bl][0], x[1][bl][0], x[0][bl][1], x[1][bl][1]};
-                  step(acc, a, sq + GEO::QCOPIES * GEO::QB + (hs * 4 + bl) * 256, GEO::QB, hs, hs < 2 && bl == 0);
+                  const uint8_t* qs = sq + GEO::QCOPIES * GEO::QB + (hs * 4 + bl) * 256;
+                  step(acc, a, qs, GEO::QB, hs, hs < 2 && bl == 0);
+                  if constexpr (!FP4) {
+                    if (hs == 0 && bl < STEPS) {
+                      const uint32_t a2[4] = {low[0][bl][0], low[1][bl][0], low[0][bl][1], low[1][bl][1]};
+                      const uint2 q1 = *reinterpret_cast<const uint2*>(qs + lane * 8);
+                      mma<FP4>(acc[1], a2, q1.x, q1.y);
+                    }
+                  }
                 }
               }
 #pragma unroll

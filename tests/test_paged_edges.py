@@ -199,3 +199,29 @@ def test_an_infinite_value_gives_an_infinite_output(hd):
     assert int(want.isinf().sum()) == 4 and not want.isnan().any()
     odd = want.isinf()
     assert torch.equal(got[odd], want[odd]) and bool(torch.isfinite(got[~odd]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,rot,page", [(64, 16, 16), (64, 32, 8), (64, 64, 64), (128, 64, 16), (256, 64, 32), (256, 16, 16)])
+def test_bfloat16_pages_keep_rotated_keys_in_two_parts(hd, rot, page):
+    """Under a cap the keys are rotated while they are scored: large queries along the rotary channels show what the rotated keys lost."""
+    rows, cap = [(60, 2, 0), (130, 1, 21)], 50
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    cache, cpu = _random_cache(n_pages, page, 2, hd, "bf16")
+    q = torch.randn(n, 4, hd) * 0.5
+    q[..., :rot] *= 12 * (64 / rot) ** 0.5
+    q = q.bfloat16()
+    rope = _tables(140, rot // 2)
+    got = ops.paged_attention(q.cuda(), cache, *(t.cuda() for t in (pages, q_start, lens)), start=start.cuda(), rope=tuple(t.cuda() for t in rope), cap=cap)
+    _status_clean()
+    kv = [t.double().numpy() for t in _values(cpu)]
+    cs = tuple(t.double().numpy() for t in rope)
+    for b, (a, m, c) in enumerate(rows):
+        for i in range(m):
+            at = [(int(pages[b, p // page]), p % page) for p in range(c, a + i + 1)]
+            ids, slots = np.array([x for x, _ in at]), np.array([y for _, y in at])
+            j = int(q_start[b]) + i
+            for h in range(4):
+                o, mass, big = _dense_attention(q[j, h].double().numpy(), kv[0][ids, h // 2, slots], kv[1][ids, h // 2, slots], a + i, c, *cs, cap, hd ** -0.5)
+                diff = np.abs(got[j, h].double().cpu().numpy() - o)
+                assert (diff <= _bound(o, mass, big, cap)).all(), (b, i, h, diff.max())
