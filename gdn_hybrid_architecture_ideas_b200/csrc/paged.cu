@@ -60,15 +60,16 @@ __device__ __forceinline__ void load8(const float* p, float* x) {
   x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
 }
 
-// x c - y s and the like, rounded once: both products with their exact remainders (fused multiply-add), their sum with its remainder
-// (Knuth's two-sum), the remainders added last. About 48 bits, in float32 instructions: conversions to 64 bits run at a
-// sixteenth of their rate.
+// x c - y s and the like, rounded once: both products with what their rounding added (fused multiply-add), their sum with what its
+// rounding added (Knuth's two-sum), the three taken off last. About 48 bits, in float32 instructions: conversions to 64 bits run at a
+// sixteenth of their rate. (The remainders stand the other way round, taken off and not added: one that is zero is then +0, and a sum of -0 stays
+// -0 without it.)
 __device__ __forceinline__ float two_products(float a, float c, float b, float s) {
   const float p = __fmul_rn(a, c), q = __fmul_rn(b, s);
-  const float ep = __fmaf_rn(a, c, -p), eq = __fmaf_rn(b, s, -q);
+  const float ep = __fmaf_rn(-a, c, p), eq = __fmaf_rn(-b, s, q);
   const float sum = __fadd_rn(p, q), bb = __fadd_rn(sum, -p);
-  const float es = __fadd_rn(__fadd_rn(p, -__fadd_rn(sum, -bb)), __fadd_rn(q, -bb));
-  const float r = __fadd_rn(sum, __fadd_rn(es, __fadd_rn(ep, eq)));
+  const float es = __fadd_rn(__fadd_rn(__fadd_rn(sum, -bb), -p), __fadd_rn(bb, -q));
+  const float r = __fadd_rn(sum, -__fadd_rn(es, __fadd_rn(ep, eq)));
   return isfinite(r) ? r : sum;          // (a remainder of an infinity is not a number)
 }
 
@@ -97,14 +98,15 @@ __device__ __forceinline__ float quotient(float a, float b, float inv) {
   const float q = __fmul_rn(a, inv);
   return __fmaf_rn(__fmaf_rn(-q, b, a), inv, q);
 }
-// Two at once in the packed instructions: a is two values, nb is -b twice, inv its reciprocal twice.
+// -a / b of two at once in the packed instructions: b twice, and minus its reciprocal twice. Negated, because the sum with a
+// remainder of +0 then keeps the sign of a zero: for a = -0 it is +0 + -0, for a = +0 it is -0 + -0.
 __device__ __forceinline__ uint64_t both(float lo, float hi) { uint64_t p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi)); return p; }
-__device__ __forceinline__ float2 quotients(uint64_t a, uint64_t nb, uint64_t inv) {
+__device__ __forceinline__ float2 minus_quotients(uint64_t a, uint64_t b, uint64_t ninv) {
   uint64_t q, r;
   float2 y;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(a), "l"(inv));
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(nb), "l"(a));
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(r), "l"(inv), "l"(q));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(a), "l"(ninv));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(b), "l"(a));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(r), "l"(ninv), "l"(q));
   asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(r));
   return y;
 }
@@ -126,13 +128,14 @@ __device__ __forceinline__ uint8_t quantize16(float* x, uint2& codes) {
   const float s = e4m3_to_float(sb);
   uint32_t w[2] = {0u, 0u};
   if (s > 0.f) {
-    const float inv = __frcp_rn(s);
-    const uint64_t nb = both(-s, -s), inv2 = both(inv, inv);
+    const float ninv = -__frcp_rn(s);
+    const uint64_t s2 = both(s, s), ninv2 = both(ninv, ninv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 y = quotients(both(x[2 * i], x[2 * i + 1]), nb, inv2);
+      const float2 y = minus_quotients(both(x[2 * i], x[2 * i + 1]), s2, ninv2);
       w[i >> 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(y, __NV_E2M1, cudaRoundNearest)) << (8 * (i & 3));
     }
+    w[0] ^= 0x88888888u; w[1] ^= 0x88888888u;
   }
   codes = make_uint2(w[0], w[1]);
   return sb;

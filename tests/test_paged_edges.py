@@ -225,3 +225,39 @@ def test_bfloat16_pages_keep_rotated_keys_in_two_parts(hd, rot, page):
                 o, mass, big = _dense_attention(q[j, h].double().numpy(), kv[0][ids, h // 2, slots], kv[1][ids, h // 2, slots], a + i, c, *cs, cap, hd ** -0.5)
                 diff = np.abs(got[j, h].double().cpu().numpy() - o)
                 assert (diff <= _bound(o, mass, big, cap)).all(), (b, i, h, diff.max())
+
+
+# ------------------------------------------------------------------------------------------------------------ zeros and their signs
+
+def _bytes(cache):
+    return [t.cpu().view(torch.int16 if t.dtype == torch.bfloat16 else torch.uint8) for t in (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "fp4"])
+@pytest.mark.parametrize("rot", [0, 16, 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_appended_bytes_equal_the_statements_to_the_sign_of_zero(fmt, rot, dtype):
+    """Zeros of both signs, values that round to zero, ordinary ones, rotated (by rows with exact zeros and ones too) or not: every byte of the
+    cache is the statement's."""
+    rows, page, hkv, hd = [(0, 40, 0), (7, 25, 2)], 16, 2, 64
+    pages, q_start, lens, start, n, n_pages = _batch(rows, page)
+    cpu = pg.PagedKV.zeros(n_pages, page, hkv, hd, fmt)
+    gpu = pg.PagedKV.zeros(n_pages, page, hkv, hd, fmt, "cuda")
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(n, hkv, hd, generator=g).to(dtype) for _ in range(2))
+    for t in (k, v):
+        what = torch.randint(0, 5, t.shape, generator=g)
+        t[what == 0], t[what == 1] = 0.0, -0.0
+        t[what == 2] *= 2.0 ** -10
+    rope = None
+    if rot:
+        cos, sin = _tables(64, rot // 2)
+        cos[1::4], sin[1::4] = 0.0, 1.0
+        cos[2::4], sin[2::4] = -1.0, -0.0
+        rope = cos, sin
+    ops.paged_append(cpu, k, v, pages, q_start, lens, start=start, rope=rope)
+    ops.paged_append(gpu, k.cuda(), v.cuda(), *(t.cuda() for t in (pages, q_start, lens)), start=start.cuda(), rope=rope and tuple(t.cuda() for t in rope))
+    _status_clean()
+    for got, want in zip(_bytes(gpu), _bytes(cpu)):
+        assert torch.equal(got, want)
