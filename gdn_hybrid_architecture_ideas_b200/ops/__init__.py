@@ -45,9 +45,11 @@ def _native():
     return _native_module
 
 
-def _check_cache(cache) -> None:
-    if _MODE == "native":
-        _native()._cache(cache)
+def _check_cache(cache) -> bool:
+    if _MODE != "native":
+        return False
+    _native()._cache(cache)
+    return True
 
 
 paged.NATIVE_CHECK = _check_cache

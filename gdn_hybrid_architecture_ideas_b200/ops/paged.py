@@ -35,7 +35,7 @@ E2M1_GRID = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 E4M3 = torch.float8_e4m3fn
 BLOCK = 16
 LARGEST = 6.0 * 448.0
-NATIVE_CHECK = None             # set by `ops`: checks a cache on a GPU (in the binding, once)
+NATIVE_CHECK = None             # set by `ops`: where the kernels run, checks a cache on a GPU (in the binding, once) and says so
 
 
 class PagedKV:
@@ -46,9 +46,7 @@ class PagedKV:
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
         self._k, self._v, self._ks, self._vs = k, v, k_scale, v_scale          # (fixed: the binding holds them too)
         self.native = None              # the CUDA binding's form of these tensors (ops/native.py)
-        if k.is_cuda:
-            if NATIVE_CHECK is not None:
-                NATIVE_CHECK(self)      # in the binding
+        if k.is_cuda and NATIVE_CHECK is not None and NATIVE_CHECK(self):
             return
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise ValueError(f"PagedKV: k and v are [pages, kv heads, page size, channels] of one type on one device, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")

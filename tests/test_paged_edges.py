@@ -261,3 +261,25 @@ def test_appended_bytes_equal_the_statements_to_the_sign_of_zero(fmt, rot, dtype
     _status_clean()
     for got, want in zip(_bytes(gpu), _bytes(cpu)):
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------------------ refusals
+
+@pytest.mark.gpu
+def test_reference_mode_checks_a_cache_on_the_gpu():
+    """With the reference mode chosen the statements run on CUDA tensors: their caches are checked as on the CPU."""
+    x = torch.zeros(4, 2, 16, 64, device="cuda")
+    codes, scales = torch.zeros(4, 2, 16, 32, dtype=torch.uint8, device="cuda"), torch.zeros(4, 2, 16, 4, device="cuda").to(E4M3)
+    ops.set_mode("reference")
+    try:
+        for match, bad in {"power of two": (x[:, :, :12].contiguous(),) * 2, "contiguous": (x.transpose(1, 2),) * 2, "one type": (x, x.half()), "come with": (codes, codes),
+                           "scales are": (codes, codes, scales.float(), scales.float()), "floating type": (x.to(torch.int32),) * 2}.items():
+            with pytest.raises(ValueError, match=match):
+                ops.PagedKV(*bad)
+        cache = ops.PagedKV(x, x.clone())
+        i32 = lambda t: torch.tensor(t, dtype=torch.int32, device="cuda")          # noqa: E731
+        k = torch.randn(3, 2, 64, device="cuda")
+        ops.paged_append(cache, k, -k, i32([[2, 0]]), i32([0, 3]), i32([17 + 3]))
+        assert torch.equal(cache.k[0, :, 1:4], k.transpose(0, 1)) and torch.equal(ops.paged_read(cache, i32([[2, 0]]), i32([0, 3]), i32([20]), 3)[1], -k)
+    finally:
+        ops.set_mode("native")
