@@ -94,6 +94,11 @@ class DecodeEngine:
             width = -(-T // page_size)         # every row owns its pages; the tables are the ops', so that rows may hold any of them
             self.pages = z("pages", (B, width), torch.int32)
             self.pages.copy_(torch.arange(B * width, device=dev, dtype=torch.int32).view(B, width))
+            for m in (l.mixer for l in model.encoder.layers if l.kind == "attention" and self.native):
+                rot = rotary_dims(m.cfg.head_dim, m.cfg.rope_fraction)
+                if rot % 16 or (m.cap is not None and rot not in (16, 32, 64)):
+                    raise ValueError(f"kv_cache {kv_cache!r} on a GPU takes a multiple of 16 rotary channels, under a distance cap 16, 32 or 64, got {rot} rotary channels: "
+                                     "kv_cache 'static'")
             self.q_start = z("q_start", B + 1, torch.int32)
             self.q_start.copy_(torch.arange(B + 1, device=dev))
         for li, layer in enumerate(model.encoder.layers):

@@ -283,3 +283,21 @@ def test_reference_mode_checks_a_cache_on_the_gpu():
         assert torch.equal(cache.k[0, :, 1:4], k.transpose(0, 1)) and torch.equal(ops.paged_read(cache, i32([[2, 0]]), i32([0, 3]), i32([20]), 3)[1], -k)
     finally:
         ops.set_mode("native")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fraction,cap,match", [(0.125, None, "8 rotary channels"), (0.125, 96, "8 rotary channels"), (0.75, 96, "48 rotary channels")])
+def test_engine_refuses_rotary_widths_that_the_paged_kernels_do_not_take(fraction, cap, match):
+    """At construction, not at the first step behind a prefill; the static cache takes them."""
+    from gdn_hybrid_architecture_ideas_b200 import config as C
+    from gdn_hybrid_architecture_ideas_b200.infer.engine import DecodeEngine
+    from gdn_hybrid_architecture_ideas_b200.models import build_model
+
+    cfg = C.hybrid_model_config("60m", full=False)
+    cfg.encoder.n_layers, cfg.encoder.nope_global_layers, cfg.vocab_size = 8, (1,), 512
+    cfg.encoder.attention.rope_fraction, cfg.encoder.attention.rope_max_distance = fraction, cap
+    model = build_model(cfg).cuda().eval()
+    for kv in ("paged", "paged_fp4"):
+        with pytest.raises(ValueError, match=match):
+            DecodeEngine(model, 1, 32, kv_cache=kv)
+    DecodeEngine(model, 1, 32)
