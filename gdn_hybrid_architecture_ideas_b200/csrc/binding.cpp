@@ -430,6 +430,7 @@ PagedCache paged_cache(const Tensor& k, const Tensor& v, const c10::optional<Ten
                     "PagedKV: k and v are [pages, kv heads, page size, channels] of one type on one device, got ", k.sizes(), " and ", v.sizes());
   TORCH_CHECK_VALUE(fp4 || is_bf16(k), "PagedKV: the cache on a GPU is bfloat16, or uint8 codes with scales");
   TORCH_CHECK_VALUE(k.is_contiguous() && v.is_contiguous(), "PagedKV: k and v are contiguous");
+  TORCH_CHECK_VALUE(k.size(1) >= 1, "PagedKV: at least one head");
   const int64_t hd = k.size(3) * (fp4 ? 2 : 1), page = k.size(2);
   TORCH_CHECK_VALUE(page >= 8 && (page & (page - 1)) == 0, "PagedKV: the page size is a power of two from 8 on, got ", page);
   TORCH_CHECK_VALUE(hd == 64 || hd == 128 || hd == 256, "PagedKV: head dimension ", hd, " (64, 128 or 256 on a GPU)");

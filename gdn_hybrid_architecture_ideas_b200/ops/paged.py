@@ -61,6 +61,8 @@ class PagedKV:
                     raise ValueError(f"PagedKV: scales are contiguous float8_e4m3fn {want} beside the codes, got {tuple(s.shape)} {s.dtype}")
         elif not k.dtype.is_floating_point or k.dtype.itemsize < 2 or k_scale is not None or v_scale is not None:
             raise ValueError(f"PagedKV: uint8 codes with scales, or values of a floating type without, got {k.dtype}")
+        if k.shape[1] < 1:
+            raise ValueError("PagedKV: at least one head")
         page = k.shape[2]
         if page < 8 or page & (page - 1):
             raise ValueError(f"PagedKV: the page size is a power of two from 8 on, got {page}")

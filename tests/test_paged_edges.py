@@ -301,3 +301,11 @@ def test_engine_refuses_rotary_widths_that_the_paged_kernels_do_not_take(fractio
         with pytest.raises(ValueError, match=match):
             DecodeEngine(model, 1, 32, kv_cache=kv)
     DecodeEngine(model, 1, 32)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("fmt", ["bf16", "fp4"])
+def test_a_cache_without_heads_is_refused(device, fmt):
+    """(Its group of query heads would be a division by zero.)"""
+    with pytest.raises(ValueError, match="one head"):
+        ops.PagedKV.zeros(4, 16, 0, 64, fmt, device)
