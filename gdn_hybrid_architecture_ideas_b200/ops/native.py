@@ -57,6 +57,17 @@ def err_flag(device) -> torch.Tensor:
     return _err[key]
 
 
+def status_word(device: torch.device) -> torch.Tensor:
+    """`err_flag` for the ops that report wrong table values there. Its zeros are written by the device's first call; inside a capture
+    they would be the graph's (every replay would clear what other calls reported), so that call is refused."""
+    word = _err.get(device.index)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a device allocates its status word: make one call before a capture")
+        word = err_flag(device)
+    return word
+
+
 # What the kernels over row tables that live on the device report (csrc/paged.cuh); every other code is a wait's.
 STATUS = {301: "paged cache: q_start is not a sequence of ranges of the packed tokens", 302: "paged cache: a row's length is below its new tokens or beyond its pages",
           303: "paged cache: a start outside the row, or a rotated position before it", 304: "paged cache: a page id outside the cache",
@@ -701,7 +712,7 @@ def _cache(cache):
     """The binding's checked form of a PagedKV's tensors (with its device's status word), made on first use."""
     c = cache.native
     if c is None:
-        c = cache.native = ext().paged_cache(cache.k, cache.v, cache.k_scale, cache.v_scale, err_flag(cache.k.device))
+        c = cache.native = ext().paged_cache(cache.k, cache.v, cache.k_scale, cache.v_scale, status_word(cache.k.device))
     return c
 
 
@@ -730,6 +741,6 @@ def paged_attention(q, cache, pages, q_start, lens, start, rope, cap, scale, out
 
 
 def verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts):
-    r = ext().verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts, err_flag(target.device))
+    r = ext().verify_drafts(target, draft, drafts, u_accept, u_sample, n_drafts, status_word(target.device))
     _count()
     return r

@@ -309,3 +309,30 @@ def test_a_cache_without_heads_is_refused(device, fmt):
     """(Its group of query heads would be a division by zero.)"""
     with pytest.raises(ValueError, match="one head"):
         ops.PagedKV.zeros(4, 16, 0, 64, fmt, device)
+
+
+@pytest.mark.gpu
+def test_the_first_call_on_a_device_is_not_captured(monkeypatch):
+    """The device's status word is allocated by the first call. Inside a capture its zeros would belong to the graph: every replay would clear what other
+    calls reported, and until the first replay it would hold anything."""
+    from gdn_hybrid_architecture_ideas_b200.ops import native
+
+    p = torch.softmax(torch.randn(1, 2, 100, device="cuda"), -1)
+    args = p, None, torch.zeros(1, 1, dtype=torch.long, device="cuda"), torch.zeros(1, 1, device="cuda"), torch.zeros(1, device="cuda")
+    x = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    want = ops.verify_drafts(*args)
+    monkeypatch.setattr(native, "_err", {})
+    for call in (lambda: ops.verify_drafts(*args), lambda: ops.PagedKV(x, x)):
+        with pytest.raises(RuntimeError, match="before a capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                y = args[-1] + 1
+                call()
+        assert not native._err
+    ops.verify_drafts(*args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.verify_drafts(*args)
+        ops.PagedKV(x, x)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    native.check_status()
