@@ -336,3 +336,116 @@ def test_the_first_call_on_a_device_is_not_captured(monkeypatch):
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     native.check_status()
+
+
+# ------------------------------------------------------------------------------------------------------------ callers
+
+def _rounded(x):
+    return pg.fp4_values(*pg.fp4_quantize(x)).to(x.dtype)
+
+
+@pytest.mark.parametrize("kind", ["full", "plain"])
+def test_engine_over_4_bit_pages_is_the_engine_over_rounded_entries_cpu(kind, monkeypatch):
+    """Steps over 4-bit pages give the logits of steps over float32 pages whose entries are rounded to the 4-bit values as they are cached."""
+    from gdn_hybrid_architecture_ideas_b200.infer import engine
+    from tests.helpers import make_model
+    from tests.test_paged import _engine_cfg
+
+    model = make_model(_engine_cfg(kind), dtype=torch.float32).eval()
+    B, P, steps = 3, 40, 6
+    g = torch.Generator().manual_seed(0)
+    prompts = torch.randint(0, 256, (B, P), generator=g)
+    docs = torch.zeros(B, P, dtype=torch.long)
+    docs[1, 11:] = 1
+    feed = torch.randint(0, 256, (steps, B), generator=g)
+
+    def logits(kv_cache):
+        eng = engine.DecodeEngine(model, B, P + steps + 2, device="cpu", use_graph=False, kv_cache=kv_cache, page_size=8)
+        eng.prefill(prompts, docs, rows_per_pass=2)
+        out = []
+        for t in feed:
+            eng.tokens.copy_(t)
+            eng.step()
+            out.append(eng.logits.clone())
+        eng.check_guards()
+        return torch.stack(out)
+    got, plain = logits("paged_fp4"), logits("paged")
+    real = ops.paged_append
+
+    def append(cache, k, v, pages, q_start, lens, start=None, rope=None):
+        real(cache, k, v, pages, q_start, lens, start=start, rope=rope)
+        k, v = ops.paged_read(cache, pages, q_start, lens, k.shape[0])
+        real(cache, _rounded(k), _rounded(v), pages, q_start, lens)
+    monkeypatch.setattr(engine.ops, "paged_append", append)
+    want = logits("paged")
+    assert (got - want).abs().max() < 1e-4 and (want - plain).abs().max() > 1e-2
+
+
+@pytest.mark.gpu
+def test_engine_over_4_bit_pages_is_the_engine_over_rounded_entries_gpu(monkeypatch):
+    """The same on the kernels, against bfloat16 pages (which hold the 4-bit values exactly) under a cap: what remains is bfloat16 noise."""
+    from gdn_hybrid_architecture_ideas_b200 import config as C
+    from gdn_hybrid_architecture_ideas_b200.infer import engine
+    from gdn_hybrid_architecture_ideas_b200.models import build_model
+
+    torch.manual_seed(0)
+    cfg = C.hybrid_model_config("60m", full=True)
+    cfg.encoder.n_layers, cfg.encoder.nope_global_layers, cfg.vocab_size = 8, (1,), 2048
+    cfg.encoder.attention.rope_max_distance = 96
+    model = build_model(cfg).cuda().eval()
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(torch.randn_like(p) * 0.02)
+    prompts, feed = torch.randint(0, 2048, (4, 256), device="cuda"), torch.randint(0, 2048, (4, 4), device="cuda")
+
+    def logits(kv_cache):
+        eng = engine.DecodeEngine(model, 4, 280, use_graph=False, kv_cache=kv_cache)
+        eng.prefill(prompts)
+        out = []
+        for t in feed:
+            eng.tokens.copy_(t)
+            eng.step()
+            out.append(eng.logits.clone())
+        return torch.stack(out)
+    got, real = logits("paged_fp4"), ops.paged_append
+
+    def append(cache, k, v, *a, rope=None, **kw):
+        assert rope is None              # (under a cap, and in layers without positions)
+        real(cache, _rounded(k), _rounded(v), *a, **kw)
+    monkeypatch.setattr(engine.ops, "paged_append", append)
+    want = logits("paged")
+    _status_clean()
+    assert float((got - want).norm() / want.norm()) < 0.05
+
+
+@pytest.mark.gpu
+def test_loopspec_samples_on_the_gpu_as_the_statement_decides(monkeypatch):
+    """Sampled decoding of the looped encoder-decoder on the GPU (its forwards through the reference mode in float32, the verification by the
+    kernel): every verification equals the statement's on the same numbers, and the tokens are its."""
+    from gdn_hybrid_architecture_ideas_b200.infer import loopspec
+    from gdn_hybrid_architecture_ideas_b200.ops import native
+    from tests.test_paged import _looped
+
+    model, prompt, doc, dec = _looped()
+    model = model.float().cuda()
+    seen, real = [], ops.verify_drafts
+
+    def verify(*args):
+        ops.set_mode("native")
+        try:
+            seen.append((args, real(*args)))
+        finally:
+            ops.set_mode("reference")
+        return seen[-1][1]
+    monkeypatch.setattr(loopspec.ops, "verify_drafts", verify)
+    before = native.launch_count()
+    ops.set_mode("reference")
+    try:
+        toks, stats = loopspec.LoopSpec(model).generate(prompt.cuda(), doc.cuda(), dec.cuda(), 24, greedy=False, generator=torch.Generator(device="cuda").manual_seed(7))
+    finally:
+        ops.set_mode("native")
+    _status_clean()
+    assert len(toks) == 24 and stats.steps == len(seen) == native.launch_count() - before == 23 and len(set(stats.flags)) == 2
+    for i, (args, (tokens, kept)) in enumerate(seen):
+        want = pg.verify_drafts(*(t.cpu() for t in args))
+        assert torch.equal(tokens.cpu(), want[0]) and torch.equal(kept.cpu(), want[1]) and toks[i + 1] == int(tokens[0, 0])
