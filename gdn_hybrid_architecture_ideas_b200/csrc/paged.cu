@@ -21,6 +21,9 @@ constexpr int APPEND_THREADS = 256;
 constexpr int ROWS_IN_SMEM = 1024;          // q_start entries kept in shared memory (beyond it: searched in global memory)
 
 __device__ __forceinline__ const int* stage_q_start(const PagedRows& r, int* s) {
+  // Out of order, the search may find no row for a token and never look at the row that is wrong: one CTA looks at all of them.
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < r.B; i += blockDim.x) { const int q = r.q_start[i], next = r.q_start[i + 1]; if (q < 0 || next < q || next > r.n) *r.err = ST_Q_START; }
   if (r.B + 1 > ROWS_IN_SMEM) return r.q_start;
   for (int i = threadIdx.x; i <= r.B; i += blockDim.x) s[i] = r.q_start[i];
   __syncthreads();
@@ -142,14 +145,15 @@ __device__ __forceinline__ uint8_t quantize16(float* x, uint2& codes) {
 }
 
 // Where a thread works: packed token j, its row and position, the entry of the position in head 0 (head h: h pages' slots further), or
-// none. Looked up once for all the heads that the thread does.
+// none. Looked up once for all the heads that the thread does. False: no row owns the token.
 struct Spot { int b, t, start; long entry; };
 __device__ __forceinline__ bool spot_of(const PagedRows& r, const int* qs, long j, Spot& s) {
   s.entry = -1;
   s.b = row_of(qs, r.B, static_cast<int>(j));
   if (s.b < 0) return false;             // padding
   const Row row = load_row(r, s.b);
-  if (row.len == 0 || j < row.q0 || j >= row.q0 + row.nq) return true;
+  if (j < row.q0 || j >= row.q0 + row.nq) return false;          // (its range is refused)
+  if (row.len == 0) return true;
   s.t = row.len - (row.q0 + row.nq - static_cast<int>(j));
   s.start = row.start;
   s.entry = entry_of(r, s.b, s.t, 0);

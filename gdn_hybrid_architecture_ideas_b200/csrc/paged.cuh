@@ -51,8 +51,8 @@ __device__ __forceinline__ long entry_of(const PagedRows& r, int b, int t, int h
   return ((static_cast<long>(page) * r.Hkv + h) << r.page_shift) + (t & ((1 << r.page_shift) - 1));
 }
 
-// The row that packed token j belongs to: the last b with q_start[b] <= j < q_start[b + 1], or -1 (padding, or a table
-// out of order). qs is q_start, in shared memory where it fits.
+// The row that packed token j belongs to: the last b with q_start[b] <= j < q_start[b + 1], or -1 (padding; in a table out of order
+// perhaps a token that a row does own). qs is q_start, in shared memory where it fits.
 __device__ __forceinline__ int row_of(const int* qs, int B, int j) {
   int lo = 0, hi = B;                  // rows lo .. hi - 1 may hold j
   while (lo < hi) {

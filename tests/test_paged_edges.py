@@ -449,3 +449,49 @@ def test_loopspec_samples_on_the_gpu_as_the_statement_decides(monkeypatch):
     for i, (args, (tokens, kept)) in enumerate(seen):
         want = pg.verify_drafts(*(t.cpu() for t in args))
         assert torch.equal(tokens.cpu(), want[0]) and torch.equal(kept.cpu(), want[1]) and toks[i + 1] == int(tokens[0, 0])
+
+
+# ------------------------------------------------------------------------------------------------------------ ranges out of order
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "fp4"])
+@pytest.mark.parametrize("q_start", [[2, 4, 0, 1], [0, 9, 3, 4], [-3, 1, 3, 4], [0, 1, 3, 9], [4, 4, 4, 2]])
+@pytest.mark.parametrize("more", [0, 1200])
+def test_wrong_ranges_are_reported_by_append_and_read(fmt, q_start, more):
+    """Status 301 whichever tokens the search finds a row for (with 1200 rows without tokens behind it does not run in shared memory); a token that gets no
+    row is not cached, and stays as it is in an `out`; what is cached or read lies where the accepted rows have it."""
+    from gdn_hybrid_architecture_ideas_b200.ops import native
+
+    rows, page, n = [(20, 1, 0), (33, 2, 0), (9, 1, 0)] + [(3, 0, 0)] * more, 16, 5
+    pages, _, lens, _, _, n_pages = _batch(rows, page)
+    cache, cpu = _random_cache(n_pages, page, 2, 64, fmt)
+    tables = pages.cuda(), torch.tensor(q_start + q_start[-1:] * more, dtype=torch.int32, device="cuda"), lens.cuda()
+
+    def reported():
+        with pytest.raises(RuntimeError, match="status 301"):
+            native.check_status()
+    out = tuple(torch.full((n, 2, 64), 3.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ops.paged_read(cache, *tables, n, out=out)
+    reported()
+    at = {}                          # packed token -> (page, slot), of the rows whose range is right
+    for b in range(3):
+        q0, q1 = q_start[b], q_start[b + 1]
+        if 0 <= q0 <= q1 <= n:
+            for j in range(q0, q1):
+                p = int(lens[b]) - (q1 - j)
+                at[j] = int(pages[b, p // page]), p % page
+    for j in range(n):
+        for o, t in zip(out, _values(cpu)):
+            kept = bool((o[j] == 3).all())
+            assert kept or (j in at and torch.equal(o[j].float().cpu(), t[at[j][0], :, at[j][1]].float()))
+    before = [t.clone() for t in _values(cache)]
+    k, v = (torch.randn(n, 2, 64, device="cuda").bfloat16() for _ in range(2))
+    ops.paged_append(cache, k, v, *tables)
+    reported()
+    for x, t, new in zip(before, _values(cache), (k, v)):
+        want = (_rounded(new.float().cpu()) if fmt == "fp4" else new.cpu()).to(t.dtype)
+        for j, (page_id, slot) in at.items():
+            got = t[page_id, :, slot]
+            assert torch.equal(got, want[j]) or torch.equal(got, x[page_id, :, slot])
+            x[page_id, :, slot] = got
+        assert torch.equal(x, t)
