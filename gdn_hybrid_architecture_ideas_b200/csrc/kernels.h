@@ -140,7 +140,7 @@ struct PagedAttn {
   const float* cos; const float* sin; int half, n_pos, cap;      // cap 0: none (keys are cached rotated)
   int Hq; float scale; bool fill;
 };
-// Work space of one call: floats of partial results and ints of their descriptions (both may be 0 long).
+// Work space of one call: floats of partial results and ints of their descriptions (for one CTA at least).
 struct PagedAttnPlan { int ctas; long ws_floats, ws_ints; };
 int paged_attention_plan(const PagedRows& r, const PagedPool& c, int Hq, int sms, PagedAttnPlan* plan);
 int paged_attention(const PagedRows& r, const PagedPool& c, const PagedAttn& a, const PagedAttnPlan& plan, float* ws, int* meta, cudaStream_t st);

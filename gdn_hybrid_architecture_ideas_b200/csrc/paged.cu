@@ -11,8 +11,8 @@
 //
 // Read: the same split; a code times its scale is exact in bfloat16.
 //
-// Measured: 2.1 M positions of 4 heads of 64, bfloat16 661 us to append and 656 us to read (6.5 TB/s, the copy's rate), 4 bits 627 us (the
-// rounding's instructions: 63% of the issue slots) and 445 us (6.2 TB/s); one token a row of 64 rows 9 us with a cold cache.
+// Measured: 2.1 M positions of 4 heads of 64, bfloat16 665 us to append and 658 us to read (6.5 TB/s, the copy's rate), 4 bits 634 us (the
+// rounding's instructions: 63% of the issue slots) and 457 us (6.0 TB/s); one token a row of 64 rows 9 us with a cold cache.
 #include "paged.cuh"
 
 namespace ghb {

@@ -11,10 +11,12 @@
 // the softmax's running maximum and sum are registers, and only the maximum needs shuffles (over the 8 lane groups).
 //
 // 4 bits: a lane's 16 channels of a key are one block with one scale. Codes become f16 pairs (cvt.f16x2.e2m1x2), times the
-// scale: exact in f16 (2 + 4 significant bits, 2^-10 .. 2688). Queries are rounded to f16 once (2^-12 relative), after a
-// power of two per query row has brought them to about one, probabilities to f16 (2^-12, scaled up: PSHIFT below). bfloat16 cache:
-// queries, probabilities and the keys that are rotated here as the sum of two bfloat16 (2^-16), other keys as they are. The sum of the probabilities is
-// taken over the rounded ones. All sums are float32 in the accumulators.
+// scale: exact in f16 (2 + 4 significant bits, 2^-10 .. 2688). Queries are rounded to f16 once (at most 2^-11 of the value), after a
+// power of two per query row has brought them to about one, probabilities to f16 (2^-11, scaled up: PSHIFT below), keys that are rotated
+// here to f16 (2^-11): beside the 2^-3 that 4 bits cost a value, and the output's own 2^-8 in bfloat16, none of it shows (0.0017 of the outputs' norm
+// from 64 bits, the plain form 0.0016). bfloat16 cache: queries, probabilities and the keys that are rotated here as the sum of two
+// bfloat16 (2^-16), other keys as they are. The sum of the probabilities is taken over the rounded ones. All sums are float32 in
+// the accumulators.
 //
 // Work: the pieces (one tile of positions for each warp) of all (row, KV head, block of query rows) units form one sequence,
 // and every CTA takes an equal share of it, so that rows of any lengths load the SMs evenly. Each CTA finds its share by
@@ -29,10 +31,10 @@
 // row sees gets scales of zero (4 bits), so that its values are zero; in bfloat16 a tile with masked infinities or NaN is summed
 // position by position.
 //
-// Measured: 64 rows of 32k positions, 16 heads over 4 of 64, under a cap: 4 bits 155 us (604 MB, 0.59 of the copy's rate; 60% of the issue
-// slots: the conversion of every entry for each block of 8 query rows bounds it), bfloat16 362 us (0.90). About 20 us of a call are fixed (the
-// share, the queries, the first tiles, joining warps and CTAs): 12 rows of up to 9k positions of 2 heads of 256 in bfloat16 35 us
-// for 17 us of bytes, one row 11 us.
+// Measured: 64 rows of 32k positions, 16 heads over 4 of 64, under a cap of 2048: 4 bits 155 us (604 MB, 0.59 of the copy's rate; 66% of the
+// issue slots: the conversion of every entry for each block of 8 query rows bounds it), bfloat16 363 us (0.90). 8 to 256 such rows in 4 bits
+// are 24.6 us and 2.02 us a row, without a cap 19.8 and 1.82 (0.79 of the copy's rate): the fixed part is the share, the queries, the first
+// tiles, joining warps and CTAs. 12 rows of up to 9k positions of 2 heads of 256 in bfloat16 35 us for 17 us of bytes, one row 11 us.
 #include <atomic>
 
 #include "paged.cuh"
@@ -191,7 +193,8 @@ template <bool FP4> __device__ __forceinline__ int place(int rho) {
 }
 
 // The units of a row: how many for a head, how many pieces each, and what a unit costs. Under a cap, pieces with keys to rotate count
-// 3 where the others, which come first, count 2 (618 against 408 instructions for 32 positions).
+// 3 where the others, which come first, count 2 (548 against 343 instructions for 32 positions of a head of 64 in 4 bits, 804 against 567
+// in bfloat16; 64 rows of 8192 positions in 4 bits, all within the cap 77 us, all beyond 54).
 template <bool CAP>
 struct RowWork {
   static constexpr int FAR = CAP ? 2 : 1, NEAR = CAP ? 3 : 1;
@@ -1050,9 +1053,11 @@ template <bool FP4> Shape shape_of(int hd) { return hd == 64 ? shape<FP4, 64>() 
 
 }  // namespace
 
-// How many CTAs run: as many as are resident, fewer where even full tables have fewer pieces. A unit is always 8 query rows: units of
-// 16 and 24, which convert each entry once for more rows, were measured and are slower (24 rows of up to 5 drafts, 32 heads over 8:
-// 94 us against 65; of up to 16: 212 against 162), because their accumulators leave room for fewer warps and shorter tiles.
+// How many CTAs run: as many as are resident, fewer where even full tables have fewer pieces. A unit is always 8 query rows, so that every
+// further block of them loads and converts the row's entries again: 24 rows of 16k positions in 4 bits, 32 heads over 8, under a cap
+// take 77 us for 1 or 2 new tokens a row, 132 for 4, 179 for 6, 234 for 8. Units of 16 and 24 rows leave room for fewer
+// warps and shorter tiles; they were slower than 8 in an earlier form of this loop and are not in the code, so that no figure compares
+// them with this one.
 int paged_attention_plan(const PagedRows& r, const PagedPool& c, int Hq, int sms, PagedAttnPlan* plan) {
   if (c.hd != 64 && c.hd != 128 && c.hd != 256) return 1;
   const int G = Hq / r.Hkv;

@@ -22,7 +22,8 @@ tokens q_start[b] .. q_start[b + 1]; `lens` int32 [B], the row's cached position
 at position lens[b] - (q_start[b + 1] - j); `start` int32 [B] (default 0), the row's first visible position, from which its
 rotary positions count. Packed tokens that no row owns (before q_start[0], from q_start[B] on, of a row whose range is refused) are
 padding: no op reads or writes for them, except that an op which allocates its own output leaves zeros there. Rows may have
-no tokens.
+no tokens. What a token does not see may hold anything; a cached value that is infinite or NaN reaches the tokens that see it (on CUDA a
+key of that kind makes their outputs NaN).
 """
 
 from __future__ import annotations
